@@ -24,7 +24,8 @@
  *   scales [rows, K / group_size] bf16;  biases [rows, K / group_size] bf16 or NULL;
  *   dequantised value = scale * q + bias.
  * The CUDA kernels implement bits = 4 with group_size = 64 (the configuration of
- * every model on this path); other valid MLX values return MOE_ERR_UNSUPPORTED.
+ * every model on this path); other valid MLX values return MOE_ERR_UNSUPPORTED. The
+ * matrix product and the dense feed-forward block take group_size 32, 64 and 128.
  */
 #ifndef MOE_B200_H
 #define MOE_B200_H
@@ -115,13 +116,89 @@ int moe_abi_version(void);
  * Replaces Array::quantized_matmul (crates/mlx-core/src/ops.rs:592-637), i.e.
  * mlx_quantized_matmul(&out, x, w, scales, biases, transpose, gs, bits, "affine", s)
  * at ops.rs:622-633, as called by Linear::forward (crates/mlx-nn/src/linear.rs:117-128).
- * transpose must be nonzero (the only form the reference calls). M >= 32 rows (with
- * N % 128 == 0) run on the tcgen05 GEMM, fewer on the GEMV; the tcgen05 path rounds each
- * dequantised weight to bf16 before the multiply (MLX's GPU qmm does the same).
+ * The form the reference calls, transpose nonzero and group_size 64, runs M >= 32 rows
+ * (with N % 128 == 0) on the tcgen05 GEMM, fewer on the GEMV; the tcgen05 path rounds each
+ * dequantised weight to bf16 before the multiply (MLX's GPU qmm does the same). Other
+ * group sizes and transpose = 0 are moe_quantized_matmul_ex with the context's scratch as
+ * its workspace.
  */
 int moe_quantized_matmul(moe_ctx* ctx, const void* x, int64_t M, int64_t K, const uint32_t* w,
                          const void* scales, const void* biases, int64_t N, int transpose,
                          int group_size, int bits, void* out);
+
+/* Element types of the dense operators below (scales and biases have the activations'). */
+enum moe_dtype { MOE_DTYPE_BF16 = 0, MOE_DTYPE_F16 = 1, MOE_DTYPE_F32 = 2 };
+
+/*
+ * The 4-bit matrix product in full: bf16 or f16, group_size 32, 64 or 128, any M and N.
+ *   transpose != 0: out[M, N] = x[M, K] . dequant(w)^T, w [N, K / 8], scales [N, K / gs];
+ *   transpose == 0: out[M, N] = x[M, K] . dequant(w),   w [K, N / 8], scales [K, N / gs]
+ * (the second is the gradient of the first with respect to its input). K (N when transpose
+ * is 0) must be a multiple of group_size; all pointers 16-byte aligned; out overlaps no
+ * input. The workspace (moe_quantized_matmul_workspace bytes, 16-byte aligned, contents
+ * irrelevant) belongs to the call until it has run: calls that may overlap need one each.
+ * Array::quantized_matmul, crates/mlx-core/src/ops.rs:592-637.
+ */
+int moe_quantized_matmul_workspace(int dtype, int64_t M, int64_t K, int64_t N, int transpose, int group_size,
+                                   int bits, size_t* bytes);
+int moe_quantized_matmul_ex(moe_ctx* ctx, int dtype, const void* x, int64_t M, int64_t K,
+                            const uint32_t* w, const void* scales, const void* biases, int64_t N,
+                            int transpose, int group_size, int bits, void* out, void* workspace,
+                            size_t workspace_bytes);
+
+/*
+ * The dense gated feed-forward block of a decoder layer without experts (DenseMlp of
+ * qwen3_moe_python_port.rs and lfm2_moe_python_port.rs), on 4-bit weights:
+ *   g = x . gate^T, u = x . up^T, h = act(g) * u, out = h . down^T (+ residual)
+ * gate and up [inter, hidden], down [hidden, inter]; x, out, residual [T, hidden].
+ * g, u and act are taken in fp32; h is rounded once to dtype (the down projection's
+ * operand), out once. hidden and inter must be multiples of group_size; pointers are
+ * 16-byte aligned; out may be residual itself, and overlaps nothing else.
+ * With gate_out / up_out [T, inter] (both or neither), g and u are stored, rounded to
+ * dtype, for the backward pass:
+ *   dh = dy . down, dup = dh * act(g), dgate = dh * u * act'(g), dx = dgate . gate + dup . up
+ * (the weights are frozen; dgate, dup [T, inter] are the gradients of the projections'
+ * outputs, for adapters beside them). Workspace as for moe_quantized_matmul_ex.
+ */
+enum moe_activation { MOE_ACT_SILU = 0, MOE_ACT_GELU = 1 /* tanh form */ };
+typedef struct moe_ffn_config {
+    int32_t hidden, inter;
+    int32_t activation; /* enum moe_activation */
+    int32_t group_size; /* 32, 64 or 128 */
+    int32_t bits;       /* 4 */
+    int32_t dtype;      /* MOE_DTYPE_BF16 or MOE_DTYPE_F16 */
+} moe_ffn_config;
+typedef struct moe_ffn_weights {
+    moe_qweight gate, up, down;
+} moe_ffn_weights;
+int moe_gated_ffn_workspace(const moe_ffn_config* cfg, int64_t T, int backward, size_t* bytes);
+int moe_gated_ffn_forward(moe_ctx* ctx, const moe_ffn_config* cfg, const moe_ffn_weights* wts,
+                          const void* x, int64_t T, const void* residual, void* gate_out, void* up_out,
+                          void* out, void* workspace, size_t workspace_bytes);
+int moe_gated_ffn_backward(moe_ctx* ctx, const moe_ffn_config* cfg, const moe_ffn_weights* wts,
+                           const void* gate, const void* up, const void* dy, int64_t T, void* dgate,
+                           void* dup, void* dx, void* workspace, size_t workspace_bytes);
+
+/*
+ * Rotary positions of x [B, H, L, D] (mlx_fast_rope): position p = offset (or offsets[b])
+ * + l, angle of pair i = p * scale / wavelength_i, wavelength_i = base^(2 i / dims) or
+ * freqs[i] ([dims / 2] device floats; base is then ignored). traditional: pairs (2 i, 2 i + 1), else
+ * (i, i + dims / 2). The rotated channels are multiplied by mscale; channels from dims on
+ * are copied. inverse: the transposed rotation (the gradient). Angles are formed in 64 bits.
+ * x_strides / out_strides: element strides of B, H and L (host arrays; D is contiguous);
+ * out is x itself with the same strides, or overlaps it nowhere. offsets: [B] device
+ * integers of offsets_bits 32 or 64, or NULL. D <= 4096.
+ */
+typedef struct moe_rope_config {
+    int32_t dtype;
+    int32_t dims; /* rotated channels, even, <= D */
+    int32_t traditional;
+    int32_t inverse;
+    double base, scale, mscale;
+} moe_rope_config;
+int moe_fast_rope(moe_ctx* ctx, const moe_rope_config* cfg, const void* x, const int64_t* x_strides,
+                  int64_t B, int64_t H, int64_t L, int64_t D, int64_t offset, const void* offsets,
+                  int offsets_bits, const float* freqs, void* out, const int64_t* out_strides);
 
 /*
  * out[i, N] (bf16) = x[row(i), K] . dequant(w[rhs_indices[i]])^T for i < batch,
@@ -238,7 +315,8 @@ int moe_block_profile(moe_ctx* ctx, const moe_block_config* cfg, const moe_block
 /*
  * Status word of the context's device work: nonzero after a bounded device-side wait
  * expired in a kernel launched on this context (the kernel then stopped early and its
- * outputs are invalid). Synchronises the context's stream. No counterpart in the
+ * outputs are invalid; for the dense operators' kernels: launched by any context on its
+ * device). Synchronises the context's stream. No counterpart in the
  * reference (MLX kernels do not wait on barriers with a time limit).
  */
 int moe_ctx_status(moe_ctx* ctx, int32_t* status);

@@ -54,6 +54,23 @@ class BlockWeights(C.Structure):
                 ("shared_expert_gate", QWeight)]
 
 
+DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
+ACT_SILU, ACT_GELU = 0, 1
+
+
+class FfnConfig(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("hidden", "inter", "activation", "group_size", "bits", "dtype")]
+
+
+class FfnWeights(C.Structure):
+    _fields_ = [("gate", QWeight), ("up", QWeight), ("down", QWeight)]
+
+
+class RopeConfig(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "dims", "traditional", "inverse")] +
+                [(n, C.c_double) for n in ("base", "scale", "mscale")])
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -107,6 +124,21 @@ SIGNATURES = {
                                       C.c_void_p]),
     "moe_ep_finish_bf16": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int64,
                                      C.c_void_p, C.c_void_p, C.c_float, C.c_void_p]),
+    "moe_quantized_matmul_workspace": (C.c_int, [C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int,
+                                                 C.c_int, C.POINTER(C.c_size_t)]),
+    "moe_quantized_matmul_ex": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p,
+                                          C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_int,
+                                          C.c_void_p, C.c_void_p, C.c_size_t]),
+    "moe_gated_ffn_workspace": (C.c_int, [C.POINTER(FfnConfig), C.c_int64, C.c_int, C.POINTER(C.c_size_t)]),
+    "moe_gated_ffn_forward": (C.c_int, [C.c_void_p, C.POINTER(FfnConfig), C.POINTER(FfnWeights), C.c_void_p,
+                                        C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                        C.c_size_t]),
+    "moe_gated_ffn_backward": (C.c_int, [C.c_void_p, C.POINTER(FfnConfig), C.POINTER(FfnWeights), C.c_void_p,
+                                         C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
+                                         C.c_void_p, C.c_size_t]),
+    "moe_fast_rope": (C.c_int, [C.c_void_p, C.POINTER(RopeConfig), C.c_void_p, C.POINTER(C.c_int64), C.c_int64,
+                                C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int, C.c_void_p,
+                                C.c_void_p, C.POINTER(C.c_int64)]),
 }
 
 
@@ -132,6 +164,7 @@ class Context:
 
     def __init__(self, device: int):
         self.device = device
+        self.lock = threading.Lock()  # held from binding a stream to the end of the call on it
         h = C.c_void_p()
         rc = library().moe_ctx_create(device, None, C.byref(h))
         if rc != MOE_OK:

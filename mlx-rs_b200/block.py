@@ -5,6 +5,8 @@
   SparseMoeBlock    <- SparseMoeBlock::forward (qwen3_moe_python_port.rs:420-488)
   MoeFeedForward    <- MoeFeedForward::forward (lfm2_moe_python_port.rs:541-740)
   RmsNorm           <- RmsNorm::forward (crates/mlx-nn/src/rms_norm.rs:30-34)
+  DenseMlp          <- DenseMlp (qwen3_moe_python_port.rs, lfm2_moe_python_port.rs): the
+                       feed-forward block of the layers without experts
   MoeStack          <- a stack of blocks with RMSNorm between them
 
 ``forward`` of a block is one call of moe_block_forward (include/moe_b200.h): the
@@ -205,6 +207,65 @@ class Gemma4MoeBlock(_Block):
     __call__ = forward
 
 
+class DenseMlp:
+    """The dense gated feed-forward block of a decoder layer without experts, on 4-bit
+    weights: down(act(gate(x)) * up(x)), activation "silu" or "gelu" (tanh form); gate, up
+    [I, H] and down [H, I], bf16 or f16, group_size 32, 64 or 128. ``forward`` is one call of
+    moe_gated_ffn_forward. For training through the frozen weights ``forward_saved`` keeps
+    what ``vjp`` needs."""
+
+    def __init__(self, gate: QWeight, up: QWeight, down: QWeight, activation: str = "silu", group_size: int = 64,
+                 bits: int = 4):
+        fn = "moe_gated_ffn_forward"
+        if activation not in ops.ACTIVATIONS:
+            raise MlxError(fn, 1, f"activation {activation!r} is not one of {sorted(ops.ACTIVATIONS)}")
+        if bits != 4 or group_size not in (32, 64, 128):
+            raise MlxError(fn, 2, f"bits={bits}, group_size={group_size} is not implemented")
+        if gate.w.dim() != 2 or gate.scales.dtype not in (torch.bfloat16, torch.float16):
+            raise MlxError(fn, 1, "gate must be a packed matrix with bf16 or f16 scales")
+        self.gate, self.up, self.down = gate, up, down
+        self.activation, self.group_size, self.bits = activation, group_size, bits
+        self.inter, self.hidden = gate.w.shape[0], gate.w.shape[1] * 32 // bits
+        self.dtype, self.device = gate.scales.dtype, gate.w.device
+        if self.inter == 0 or self.hidden == 0 or self.inter % group_size or self.hidden % group_size:
+            raise MlxError(fn, 1, f"hidden={self.hidden} and inter={self.inter} must be positive multiples of "
+                                  f"group_size={group_size}")
+        for name, q, rows, cols in (("gate", gate, self.inter, self.hidden), ("up", up, self.inter, self.hidden),
+                                    ("down", down, self.hidden, self.inter)):
+            ops.check_qweight(fn, name, q, rows, cols, self.dtype, self.device, group_size)
+        self._cfg, self._wts = ops.ffn_structs(self.hidden, self.inter, self.dtype, gate, up, down, activation,
+                                               group_size, bits)
+
+    def _check(self, fn, x):
+        if x.dtype != self.dtype or x.device != self.device or not x.is_contiguous() or x.shape[-1] != self.hidden:
+            raise MlxError(fn, 1, f"contiguous {self.dtype} [..., {self.hidden}] on {self.device} expected, "
+                                  f"got {x.dtype} {tuple(x.shape)} on {x.device}")
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        self._check("moe_gated_ffn_forward", x)
+        return ops._ffn_forward(self._cfg, self._wts, x, None, False)
+
+    __call__ = forward
+
+    def forward_layer(self, x: torch.Tensor, norm_weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
+        """The feed-forward half of a decoder layer, x + block(RmsNorm(x)); the residual is
+        added in the down projection's epilogue, before its one rounding. bf16."""
+        self._check("moe_gated_ffn_forward", x)
+        return ops._ffn_forward(self._cfg, self._wts, ops.fast_rms_norm(x, norm_weight, eps), x, False)
+
+    def forward_saved(self, x: torch.Tensor):
+        """(forward(x), saved): the same call, which also stores the two projections' outputs."""
+        self._check("moe_gated_ffn_forward", x)
+        out, g, u = ops._ffn_forward(self._cfg, self._wts, x, None, True)
+        return out, (g, u)
+
+    def vjp(self, saved, dy: torch.Tensor):
+        """(dx, dg, du): gradients with respect to x and to the two projections' outputs (for
+        adapters beside the frozen weights), given the gradient dy of the output."""
+        self._check("moe_gated_ffn_backward", dy)
+        return ops._ffn_backward(self._cfg, self._wts, saved[0], saved[1], dy)
+
+
 class RmsNorm:
     def __init__(self, weight: torch.Tensor, eps: float = 1e-6):
         self.weight, self.eps = weight, eps
@@ -240,5 +301,5 @@ class MoeStack:
     __call__ = forward
 
 
-__all__ = ["SwitchLinear", "SparseMoeBlock", "MoeFeedForward", "Gemma4MoeBlock", "RmsNorm", "MoeStack", "infer_bits",
+__all__ = ["SwitchLinear", "SparseMoeBlock", "MoeFeedForward", "Gemma4MoeBlock", "DenseMlp", "RmsNorm", "MoeStack", "infer_bits",
            "SCORING_SOFTMAX", "SCORING_SOFTMAX_BIAS", "SCORING_SIGMOID_BIAS_SELECT"]

@@ -17,6 +17,7 @@
 #include <string>
 
 #include "../../include/moe_b200.h"
+#include "dense.cuh"
 #include "kernels.cuh"
 
 struct moe_ctx {
@@ -954,9 +955,20 @@ int moe_quantized_matmul(moe_ctx* ctx, const void* x, int64_t M, int64_t K, cons
   if (!ctx) return MOE_ERR_INVALID;
   ctx->last_error.clear();
   const char* fn = "moe_quantized_matmul";
+  if (bits == 4 && (group_size == 32 || group_size == 128 || (group_size == 64 && !transpose))) {
+    size_t ws = 0;
+    int rc = moe_quantized_matmul_workspace(MOE_DTYPE_BF16, M, K, N, transpose, group_size, bits, &ws);
+    if (rc == MOE_OK && ws > 0) {
+      DeviceGuard g(ctx->device);
+      if (!g.ok) return fail(ctx, MOE_ERR_CUDA, "cudaSetDevice(%d) failed", ctx->device);
+      rc = ensure_scratch(ctx, 256 + ws);  // the first 256 bytes are the status block
+      if (rc) return rc;
+    }
+    return moe_quantized_matmul_ex(ctx, MOE_DTYPE_BF16, x, M, K, w, scales, biases, N, transpose, group_size, bits,
+                                   out, ws ? static_cast<char*>(ctx->scratch) + 256 : nullptr, ws);
+  }
   int rc = check_quant(ctx, fn, K, group_size, bits);
   if (rc) return rc;
-  if (!transpose) return fail(ctx, MOE_ERR_UNSUPPORTED, "%s: transpose=false is not implemented", fn);
   if (M < 0 || N <= 0 || N > INT32_MAX || M > INT32_MAX) return fail(ctx, MOE_ERR_INVALID, "%s: bad M/N", fn);
   if (M == 0) return MOE_OK;
   if (!x || !w || !scales || !out) return fail(ctx, MOE_ERR_INVALID, "%s: null pointer", fn);
@@ -1469,11 +1481,15 @@ int moe_ep_finish_bf16(moe_ctx* ctx, const void* partials, int32_t world, int64_
 int moe_ctx_status(moe_ctx* ctx, int32_t* status) {
   if (!ctx || !status) return MOE_ERR_INVALID;
   *status = 0;
-  if (!ctx->scratch) return MOE_OK;
   DeviceGuard g(ctx->device);
   if (!g.ok) return fail(ctx, MOE_ERR_CUDA, "cudaSetDevice(%d) failed", ctx->device);
-  MOE_CUDA(ctx, cudaMemcpyAsync(status, ctx->scratch, sizeof(int32_t), cudaMemcpyDeviceToHost, ctx->stream));
-  MOE_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+  int32_t dense = 0;  // the dense operators' kernels share one word per device
+  MOE_CUDA(ctx, moe::dense_status(&dense, ctx->stream));
+  if (ctx->scratch) {
+    MOE_CUDA(ctx, cudaMemcpyAsync(status, ctx->scratch, sizeof(int32_t), cudaMemcpyDeviceToHost, ctx->stream));
+    MOE_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+  }
+  *status |= dense;
   return MOE_OK;
 }
 

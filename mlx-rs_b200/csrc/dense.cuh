@@ -1,0 +1,143 @@
+// dense.cuh — argument blocks, launchers and device helpers of the dense operators: 4-bit
+// matrix products at every MLX group size, the gated feed-forward block with its backward
+// pass, and the rotary positions. Activations are bf16 or f16 (the rotary positions f32
+// too); scales and biases have the activations' type.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "kernels.cuh"
+
+namespace moe {
+
+enum DenseType { kBf16 = 0, kF16 = 1, kF32 = 2 };
+
+// One packed matrix [rows][cols]: cols / 8 words and cols / group scales (biases) per row.
+struct PackedMatrix {
+  const uint32_t* w;
+  const uint16_t* s;
+  const uint16_t* b;  // may be null
+  int64_t rows;
+  int cols;
+  int w_pitch, s_pitch;  // words and scales from one row to the next (cols may be a part)
+};
+
+// ---- dequantisation into 16-bit rows (dense_dequant.cu)
+struct DequantJob {
+  PackedMatrix m;
+  uint16_t* out;   // [rows][ld], or [cols][ld] when transposed
+  int64_t ld;
+};
+struct DequantArgs {
+  DequantJob job[3];
+  int jobs;
+  int group;
+  int transposed;
+  int type;
+};
+cudaError_t launch_dequant(const DequantArgs& a, cudaStream_t st);
+// out[r][0..cols) = x[r][0..cols), rows ld elements apart, the rest of each row zero.
+cudaError_t launch_pad_rows(const uint16_t* x, int64_t rows, int64_t cols, uint16_t* out, int64_t ld, cudaStream_t st);
+
+// ---- 16-bit matrix product with fused epilogues (dense_gemm.cu)
+enum DenseEpilogue { kEpiPlain = 0, kEpiGated = 1, kEpiGatedBackward = 2 };
+struct DenseEpi {
+  int64_t ldo;               // row pitch of every tensor below
+  uint16_t* out;             // plain: [M][N]; gated: h = act(g) * u [M][N]
+  const uint16_t* residual;  // plain: [M][N] added before the rounding, or null
+  uint16_t* gate;            // gated: g and u [M][N] stored when non-null; backward: read
+  uint16_t* up;
+  uint16_t* dgate;           // backward: [M][N]
+  uint16_t* dup;
+  int act;                   // 0 SiLU, 1 GELU (tanh form)
+};
+struct DenseGemm {
+  // D[M, N] = sum over the operand pairs p of A_p[M, K_p] . B_p[N, K_p]^T (one or two
+  // pairs); in the gated form one A and two B: g = A . B_0^T, u = A . B_1^T.
+  const uint16_t* a[2];
+  const uint16_t* b[2];
+  int64_t lda[2], ldb[2];
+  int pairs;
+  int64_t M;
+  int N, K;
+  int type;      // kBf16 / kF16
+  int epilogue;  // DenseEpilogue
+  DenseEpi e;
+  float* partial;        // split-K partial sums (dense_partial_bytes), or null: never split
+  size_t partial_bytes;
+};
+size_t dense_partial_bytes(int64_t M, int N, int K, int pairs, bool gated);
+cudaError_t launch_dense_gemm(const DenseGemm& g, cudaStream_t st);
+// Device status word of the dense kernels on the current device (bounded waits).
+cudaError_t dense_status(int32_t* status, cudaStream_t st);
+
+// ---- rotary positions (rope.cu)
+struct RopeArgs {
+  const void* x;
+  void* out;
+  int64_t xs[3], os[3];  // element strides of batch, head, position
+  int64_t B, H, L;
+  int D, dims;
+  int type;
+  int interleaved;
+  double base, scale;
+  float mscale, sign;    // sign -1: the transposed rotation
+  int64_t offset;
+  const void* offsets;   // [B] int32 or int64 (offsets64), or null
+  int offsets64;
+  const float* freqs;    // [dims / 2] or null
+};
+cudaError_t launch_rope(const RopeArgs& a, cudaStream_t st);
+
+// ---- device helpers
+template <int TYPE>
+struct Elem;  // conversions of the 16-bit element types
+template <>
+struct Elem<kBf16> {
+  static MOE_DEV float to_f(uint16_t v) { return bf2f(v); }
+  static MOE_DEV uint32_t pack(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+  }
+  static MOE_DEV float lo(uint32_t v) { return bf_lo(v); }
+  static MOE_DEV float hi(uint32_t v) { return bf_hi(v); }
+};
+template <>
+struct Elem<kF16> {
+  static MOE_DEV float to_f(uint16_t v) { return __half2float(__ushort_as_half(v)); }
+  static MOE_DEV uint32_t pack(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+  }
+  static MOE_DEV float lo(uint32_t v) { return to_f((uint16_t)(v & 0xffffu)); }
+  static MOE_DEV float hi(uint32_t v) { return to_f((uint16_t)(v >> 16)); }
+};
+
+// 1 / (1 + exp(-x)) from the hardware base-2 exponential and reciprocal (relative error a
+// few fp32 ulps, far below the 16-bit rounding that follows).
+MOE_DEV float sigmoid_hw(float x) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(e) : "f"(x * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(1.0f + e));
+  return r;
+}
+// The activation and its derivative. Both are x * sigmoid(z): SiLU with z = x, GELU's tanh
+// form with z = 2 sqrt(2/pi) (x + 0.044715 x^3), since (1 + tanh(y)) / 2 = sigmoid(2 y);
+// the derivative is sig + x sig (1 - sig) z'.
+MOE_DEV float act_val(float x, int act) {
+  const float z = act ? 1.5957691216057308f * x * __fmaf_rn(0.044715f * x, x, 1.0f) : x;
+  return x * sigmoid_hw(z);
+}
+MOE_DEV void act_grad(float x, int act, float& val, float& grad) {
+  const float z = act ? 1.5957691216057308f * x * __fmaf_rn(0.044715f * x, x, 1.0f) : x;
+  const float zp = act ? 1.5957691216057308f * __fmaf_rn(0.134145f * x, x, 1.0f) : 1.0f;
+  const float s = sigmoid_hw(z);
+  val = x * s;
+  grad = __fmaf_rn(val * (1.0f - s), zp, s);
+}
+
+}  // namespace moe

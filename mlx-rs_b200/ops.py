@@ -5,10 +5,12 @@ Mirrors the reference's Array methods (crates/mlx-core/src/ops.rs):
   gather_qmm(x, w, scales, biases, lhs_indices, rhs_indices, transpose,
              group_size, bits, sorted_indices)                           ops.rs:830-891
   fast_rms_norm(x, weight, eps)                                          ops.rs:691-701
+  fast_rope(x, dims, traditional, base, scale, offset, freqs)            mlx_fast_rope
 Failures raise MlxError("<mlx fn> failed (rc=N): reason"), the Error::Mlx message
 of crates/mlx-core/src/array.rs:43-49.
 
-Tensor conventions: activations and scales/biases are torch.bfloat16; packed weights
+Tensor conventions: activations and scales/biases are torch.bfloat16 (quantized_matmul,
+gated_ffn: or float16; fast_rope: or float32 too); packed weights
 are 32-bit words (torch.int32 holding the uint32 bit patterns, or torch.uint32);
 indices are 32-bit integers (uint32 semantics). All tensors live on one CUDA device
 and calls are ordered on torch's current stream.
@@ -19,7 +21,8 @@ import ctypes as C
 
 import torch
 
-from ._lib import MlxError, context_for, library
+from ._lib import (ACT_GELU, ACT_SILU, DTYPE_BF16, DTYPE_F16, DTYPE_F32, FfnConfig, FfnWeights, MlxError, QWeight,
+                   RopeConfig, context_for, library)
 
 _WORD_DTYPES = {torch.int32} | ({torch.uint32} if hasattr(torch, "uint32") else set())
 
@@ -45,8 +48,87 @@ def _need(t, dtypes, name):
         raise MlxError("moe_b200", 1, f"{name}: must be contiguous")
 
 
+_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.float32: DTYPE_F32}
+ACTIVATIONS = {"silu": ACT_SILU, "gelu": ACT_GELU}
+
+
+def _bound(fn, t):
+    """The device's context with its lock held, bound to torch's current stream there. The
+    caller releases the lock after its call: another thread may bind another stream."""
+    if not t.is_cuda:
+        raise MlxError(fn, 1, "tensors must be on a CUDA device")
+    ctx = context_for(t.device.index)
+    ctx.lock.acquire()
+    ctx.bind_stream(torch.cuda.current_stream(t.device).cuda_stream)
+    return ctx
+
+
+def _workspace(nbytes, device):
+    # from torch's allocator on the current stream: each call and each captured graph has its own
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def check_qweight(fn, name, q, rows, cols, dtype, device, group_size, bits=4):
+    """A packed matrix [rows, cols] with scales and biases of `dtype`, all on `device`."""
+    want = {"w": (rows, cols * bits // 32), "scales": (rows, cols // group_size), "biases": (rows, cols // group_size)}
+    for part, shape in want.items():
+        t = getattr(q, part)
+        if t is None and part == "biases":
+            continue
+        if t is None or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+            got = "missing" if t is None else f"{tuple(t.shape)} on {t.device}"
+            raise MlxError(fn, 1, f"{name}.{part}: contiguous {shape} on {device} expected, got {got}")
+        if t.dtype not in (_WORD_DTYPES if part == "w" else {dtype}):
+            raise MlxError(fn, 1, f"{name}.{part}: dtype {t.dtype}")
+
+
+class _Q:
+    __slots__ = ("w", "scales", "biases")
+
+    def __init__(self, w, scales, biases):
+        self.w, self.scales, self.biases = w, scales, biases
+
+
+def _quantized_matmul_ex(x, w, scales, biases, transpose, group_size, bits):
+    fn = "mlx_quantized_matmul"
+    if x.dtype not in (torch.bfloat16, torch.float16) or x.dim() < 1 or not x.is_contiguous():
+        raise MlxError(fn, 1, "x must be contiguous bf16 or f16 [..., K]")
+    if bits != 4 or group_size not in (32, 64, 128):
+        raise MlxError(fn, 2, f"bits={bits}, group_size={group_size} is not implemented")
+    if w.dim() != 2:
+        raise MlxError(fn, 1, "w must be [rows, cols*bits/32]")
+    K = x.shape[-1]
+    cols = w.shape[1] * 8
+    N = w.shape[0] if transpose else cols
+    if (cols if transpose else w.shape[0]) != K or cols % group_size:
+        raise MlxError(fn, 1, f"x [..., {K}] does not fit w {tuple(w.shape)} (transpose={bool(transpose)}, "
+                              f"group_size={group_size})")
+    check_qweight(fn, "w", _Q(w, scales, biases), w.shape[0], cols, x.dtype, x.device, group_size)
+    M = x.numel() // K if K else 0
+    out = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
+    lib, dt, tr = library(), _DTYPES[x.dtype], int(bool(transpose))
+    need = C.c_size_t()
+    rc = lib.moe_quantized_matmul_workspace(dt, M, K, N, tr, group_size, bits, C.byref(need))
+    if rc:
+        raise MlxError(fn, rc, f"unsupported call: M={M}, K={K}, N={N}")
+    ws = _workspace(need.value, x.device)
+    ctx = _bound(fn, x)
+    try:
+        rc = lib.moe_quantized_matmul_ex(ctx.handle, dt, x.data_ptr(), M, K, w.data_ptr(), scales.data_ptr(),
+                                         biases.data_ptr() if biases is not None else None, N, tr, group_size, bits,
+                                         out.data_ptr(), ws.data_ptr() if ws is not None else None, need.value)
+        ctx.check(fn, rc)
+    finally:
+        ctx.lock.release()
+    return out
+
+
 def quantized_matmul(x, w, scales, biases=None, transpose=True, group_size=64, bits=4):
-    """out[..., N] = x[..., K] @ dequant(w)^T (transpose=True)."""
+    """out[..., N] = x[..., K] @ dequant(w)^T (transpose=True), or x[..., K] @ dequant(w)
+    for w [K, N*bits/32] (transpose=False: the gradient of the first with respect to x).
+    bf16 or f16, group_size 32, 64 or 128, bits 4."""
+    if x.dtype != torch.bfloat16 or not transpose or group_size in (32, 128):
+        return _quantized_matmul_ex(x, w, scales, biases, transpose, group_size, bits)
     _need(x, {torch.bfloat16}, "x")
     _need(w, _WORD_DTYPES, "w")
     _need(scales, {torch.bfloat16}, "scales")
@@ -141,4 +223,163 @@ def fast_rms_norm(x, weight, eps):
     rc = library().moe_fast_rms_norm(ctx.handle, _ptr(x), _ptr(weight), float(eps), rows, dim,
                                      _ptr(out))
     ctx.check("mlx_fast_rms_norm", rc)
+    return out
+
+
+def _ffn_call(fn, x, gate, up, down, activation, group_size, bits):
+    """Config and weight structs of a checked feed-forward call."""
+    if activation not in ACTIVATIONS:
+        raise MlxError(fn, 1, f"activation {activation!r} is not one of {sorted(ACTIVATIONS)}")
+    if x.dtype not in (torch.bfloat16, torch.float16) or x.dim() < 1 or not x.is_contiguous():
+        raise MlxError(fn, 1, "x must be contiguous bf16 or f16 [..., hidden]")
+    if bits != 4 or group_size not in (32, 64, 128):
+        raise MlxError(fn, 2, f"bits={bits}, group_size={group_size} is not implemented")
+    H, I = x.shape[-1], gate.w.shape[0]
+    if H == 0 or H % group_size or I == 0 or I % group_size:
+        raise MlxError(fn, 1, f"hidden={H} and inter={I} must be positive multiples of group_size={group_size}")
+    for name, q, rows, cols in (("gate", gate, I, H), ("up", up, I, H), ("down", down, H, I)):
+        check_qweight(fn, name, q, rows, cols, x.dtype, x.device, group_size)
+    return ffn_structs(H, I, x.dtype, gate, up, down, activation, group_size, bits)
+
+
+def ffn_structs(H, I, dtype, gate, up, down, activation, group_size, bits):
+    cfg = FfnConfig(H, I, ACTIVATIONS[activation], group_size, bits, _DTYPES[dtype])
+    ptrs = [QWeight(q.w.data_ptr(), q.scales.data_ptr(), None if q.biases is None else q.biases.data_ptr())
+            for q in (gate, up, down)]
+    return cfg, FfnWeights(*ptrs)
+
+
+def _like(fn, name, t, shape, x):
+    if tuple(t.shape) != tuple(shape) or t.dtype != x.dtype or t.device != x.device or not t.is_contiguous():
+        raise MlxError(fn, 1, f"{name}: contiguous {x.dtype} {tuple(shape)} on {x.device} expected")
+
+
+def _ffn_forward(cfg, wts, x, residual, save):
+    fn = "moe_gated_ffn_forward"
+    T = x.numel() // cfg.hidden
+    out = torch.empty_like(x)
+    g = u = None
+    if save:
+        g = torch.empty(*x.shape[:-1], cfg.inter, dtype=x.dtype, device=x.device)
+        u = torch.empty_like(g)
+    lib = library()
+    need = C.c_size_t()
+    lib.moe_gated_ffn_workspace(C.byref(cfg), T, 0, C.byref(need))
+    ws = _workspace(need.value, x.device)
+    ctx = _bound(fn, x)
+    try:
+        rc = lib.moe_gated_ffn_forward(ctx.handle, C.byref(cfg), C.byref(wts), x.data_ptr(), T,
+                                       residual.data_ptr() if residual is not None else None,
+                                       g.data_ptr() if save else None, u.data_ptr() if save else None,
+                                       out.data_ptr(), ws.data_ptr() if ws is not None else None, need.value)
+        ctx.check(fn, rc)
+    finally:
+        ctx.lock.release()
+    return (out, g, u) if save else out
+
+
+def _ffn_backward(cfg, wts, g, u, dy):
+    fn = "moe_gated_ffn_backward"
+    T = dy.numel() // cfg.hidden
+    _like(fn, "gate", g, (*dy.shape[:-1], cfg.inter), dy)
+    _like(fn, "up", u, (*dy.shape[:-1], cfg.inter), dy)
+    dx, dgate, dup = torch.empty_like(dy), torch.empty_like(g), torch.empty_like(u)
+    lib = library()
+    need = C.c_size_t()
+    lib.moe_gated_ffn_workspace(C.byref(cfg), T, 1, C.byref(need))
+    ws = _workspace(need.value, dy.device)
+    ctx = _bound(fn, dy)
+    try:
+        rc = lib.moe_gated_ffn_backward(ctx.handle, C.byref(cfg), C.byref(wts), g.data_ptr(), u.data_ptr(),
+                                        dy.data_ptr(), T, dgate.data_ptr(), dup.data_ptr(), dx.data_ptr(),
+                                        ws.data_ptr() if ws is not None else None, need.value)
+        ctx.check(fn, rc)
+    finally:
+        ctx.lock.release()
+    return dx, dgate, dup
+
+
+def gated_ffn(x, gate, up, down, activation="silu", group_size=64, bits=4, residual=None, save=False):
+    """(act(x gate^T) * (x up^T)) down^T (+ residual): the dense feed-forward block on 4-bit
+    weights (QWeight triples; gate, up [I, H], down [H, I]), activation "silu" or "gelu"
+    (tanh form). With save, (out, g, u): the two projections' outputs, what gated_ffn_vjp
+    takes. bf16 or f16, group_size 32, 64 or 128."""
+    cfg, wts = _ffn_call("moe_gated_ffn_forward", x, gate, up, down, activation, group_size, bits)
+    if residual is not None:
+        _like("moe_gated_ffn_forward", "residual", residual, x.shape, x)
+    return _ffn_forward(cfg, wts, x, residual, save)
+
+
+def gated_ffn_vjp(g, u, dy, gate, up, down, activation="silu", group_size=64, bits=4):
+    """(dx, dg, du): the gradients of gated_ffn with respect to x and to the projections'
+    outputs g, u (as saved by it), for the gradient dy of its output. The quantised weights
+    are frozen."""
+    cfg, wts = _ffn_call("moe_gated_ffn_backward", dy, gate, up, down, activation, group_size, bits)
+    return _ffn_backward(cfg, wts, g, u, dy)
+
+
+def fast_rope(x, dims, traditional=False, base=10000.0, scale=1.0, offset=0, freqs=None, mscale=1.0, inverse=False,
+              out=None):
+    """Rotary positions of x [..., L, D] (the axes before L: any batch and heads; two of them,
+    [B, H, L, D], may have any strides). Pair i of the first `dims` channels at position
+    offset + l is turned by (offset + l) * scale / wavelength_i, wavelength_i =
+    base**(2 i / dims) or freqs[i] (float32 [dims/2]), and scaled by mscale; traditional:
+    pairs (2i, 2i+1), else (i, i + dims/2); channels from dims on are copied. offset: an
+    int, or an int32 / int64 tensor [B] with one offset per batch element. inverse: the
+    transposed rotation, the gradient with respect to x. out: where to write, x itself
+    included (default: a new contiguous tensor). bf16, f16 or f32."""
+    fn = "mlx_fast_rope"
+    if x.dtype not in _DTYPES or x.dim() < 2:
+        raise MlxError(fn, 1, "x must be bf16, f16 or f32 [..., L, D]")
+    xv = x
+    if x.dim() != 4:
+        if isinstance(offset, torch.Tensor) and offset.dim() and x.dim() != 3:
+            raise MlxError(fn, 1, "offsets per batch element need x [B, H, L, D] or [B, L, D]")
+        if x.dim() == 3:
+            xv = x[:, None]
+        else:
+            if not x.is_contiguous():
+                raise MlxError(fn, 1, "x: must be contiguous unless [B, H, L, D] or [B, L, D]")
+            xv = x.reshape(1, -1, *x.shape[-2:])
+    B, H, L, D = xv.shape
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        raise MlxError(fn, 1, f"out: {x.dtype} {tuple(x.shape)} on {x.device} expected")
+    if out is x or out.data_ptr() == x.data_ptr():
+        if out.stride() != x.stride():
+            raise MlxError(fn, 1, "out shares x's memory with other strides")
+    if x.dim() == 4:
+        ov = out
+    elif x.dim() == 3:
+        ov = out[:, None]
+    else:
+        if not out.is_contiguous():
+            raise MlxError(fn, 1, "out: must be contiguous unless [B, H, L, D] or [B, L, D]")
+        ov = out.view(1, -1, L, D)
+    xs, os_ = xv.stride(), ov.stride()
+    if D > 1 and (xs[3] != 1 or os_[3] != 1):
+        raise MlxError(fn, 1, "the channels of x and out must be contiguous")
+    offs, offs_bits, off = None, 0, 0
+    if isinstance(offset, torch.Tensor):
+        if offset.dtype not in (torch.int32, torch.int64) or offset.device != x.device or not offset.is_contiguous() \
+                or offset.numel() != B or offset.dim() > 1:
+            raise MlxError(fn, 1, f"offset: contiguous int32 or int64 [{B}] on {x.device} expected")
+        offs, offs_bits = offset.data_ptr(), 32 if offset.dtype == torch.int32 else 64
+    else:
+        off = int(offset)
+    if freqs is not None and (freqs.dtype != torch.float32 or freqs.device != x.device or
+                              tuple(freqs.shape) != (dims // 2,) or not freqs.is_contiguous()):
+        raise MlxError(fn, 1, f"freqs: contiguous float32 [{dims // 2}] on {x.device} expected")
+    cfg = RopeConfig(_DTYPES[x.dtype], dims, int(bool(traditional)), int(bool(inverse)),
+                     float(base) if base is not None else 0.0, scale, mscale)
+    i3 = C.c_int64 * 3
+    ctx = _bound(fn, x)
+    try:
+        rc = library().moe_fast_rope(ctx.handle, C.byref(cfg), x.data_ptr(), i3(*xs[:3]), B, H, L, D, off, offs,
+                                     offs_bits, freqs.data_ptr() if freqs is not None else None, out.data_ptr(),
+                                     i3(*os_[:3]))
+        ctx.check(fn, rc)
+    finally:
+        ctx.lock.release()
     return out
