@@ -145,6 +145,8 @@ SIGNATURES = {
 def library():
     """Load (building first if needed) and return the ctypes handle."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not os.path.exists(library_path):
@@ -172,7 +174,7 @@ class Context:
         self.handle = h
 
     def bind_stream(self, stream_handle: int):
-        library().moe_ctx_set_stream(self.handle, C.c_void_p(stream_handle))
+        library().moe_ctx_set_stream(self.handle, stream_handle)
 
     def check(self, fn: str, rc: int):
         if rc != MOE_OK:

@@ -232,7 +232,7 @@ class DenseMlp:
                                   f"group_size={group_size}")
         for name, q, rows, cols in (("gate", gate, self.inter, self.hidden), ("up", up, self.inter, self.hidden),
                                     ("down", down, self.hidden, self.inter)):
-            ops.check_qweight(fn, name, q, rows, cols, self.dtype, self.device, group_size)
+            ops.check_qweight(fn, name, q, rows, cols, self.dtype, gate.w.get_device(), group_size)
         self._cfg, self._wts = ops.ffn_structs(self.hidden, self.inter, self.dtype, gate, up, down, activation,
                                                group_size, bits)
 

@@ -104,9 +104,10 @@ struct QmmWs {
   float* partial;
   size_t partial_bytes, bytes;
 };
-QmmWs carve_qmm(void* base, int64_t M, int64_t N, int64_t K) {
+QmmWs carve_qmm(void* base, int64_t M, int64_t N, int64_t K, int transpose) {
   Carve cv{static_cast<char*>(base)};
   QmmWs w{};
+  if (transpose && M <= moe::kQmvMaxM) return w;  // straight from the packed weights
   const int64_t piece = qmm_piece(N, K);
   w.w = cv.take<uint16_t>(piece * up8(K));
   if (K % 8) w.xpad = cv.take<uint16_t>(M * up8(K));
@@ -164,6 +165,11 @@ FfnWs carve_ffn(void* base, const moe_ffn_config* c, int64_t T, bool backward) {
   FfnWs w{};
   const size_t n = (size_t)c->hidden * c->inter;
   const int H = c->hidden, I = c->inter;
+  if (!backward && T <= moe::kQmvMaxM) {  // straight from the packed weights
+    w.h = cv.take<uint16_t>((size_t)T * I);
+    w.bytes = cv.off;
+    return w;
+  }
   w.wg = cv.take<uint16_t>(n);
   w.wu = cv.take<uint16_t>(n);
   w.wd = cv.take<uint16_t>(n);
@@ -198,7 +204,7 @@ int moe_quantized_matmul_workspace(int dtype, int64_t M, int64_t K, int64_t N, i
   int rc = check_format(nullptr, "", dtype, group_size, bits);
   if (!rc) rc = check_qmm_sizes(nullptr, "", M, K, N, transpose, group_size);
   if (rc || M == 0) return rc;
-  *bytes = carve_qmm(nullptr, M, N, K).bytes;
+  *bytes = carve_qmm(nullptr, M, N, K, transpose).bytes;
   return MOE_OK;
 }
 
@@ -216,14 +222,27 @@ int moe_quantized_matmul_ex(moe_ctx* ctx, int dtype, const void* x, int64_t M, i
   rc = check_weight(ctx, fn, "w", q);
   if (rc) return rc;
   if (!aligned16(x) || !aligned16(out)) return fail(ctx, MOE_ERR_INVALID, "%s: x and out must be 16-byte aligned", fn);
-  const QmmWs need = carve_qmm(nullptr, M, N, K);
+  const QmmWs need = carve_qmm(nullptr, M, N, K, transpose);
   rc = check_workspace(ctx, fn, workspace, workspace_bytes, need.bytes);
   if (rc) return rc;
-  const QmmWs ws = carve_qmm(workspace, M, N, K);
+  const QmmWs ws = carve_qmm(workspace, M, N, K, transpose);
   DeviceGuard g(moe_internal::ctx_device(ctx));
   if (!g.ok) return fail(ctx, MOE_ERR_CUDA, "%s: cudaSetDevice failed", fn);
   const cudaStream_t st = static_cast<cudaStream_t>(moe_internal::ctx_stream(ctx));
 
+  if (transpose && M <= moe::kQmvMaxM) {
+    moe::QmvArgs a{};
+    a.x = static_cast<const uint16_t*>(x);
+    a.m[0] = packed(q, N, K);
+    a.M = (int)M;
+    a.N = N;
+    a.K = (int)K;
+    a.group = group_size;
+    a.type = dtype;
+    a.out = static_cast<uint16_t*>(out);
+    DENSE_CUDA(ctx, fn, moe::launch_qmv(a, false, st));
+    return MOE_OK;
+  }
   const int64_t ld = up8(K);
   const uint16_t* xs = static_cast<const uint16_t*>(x);
   if (ws.xpad) {
@@ -305,6 +324,35 @@ int moe_gated_ffn_forward(moe_ctx* ctx, const moe_ffn_config* cfg, const moe_ffn
   const cudaStream_t st = static_cast<cudaStream_t>(moe_internal::ctx_stream(ctx));
   const int H = cfg->hidden, I = cfg->inter;
 
+  if (T <= moe::kQmvMaxM) {
+    moe::QmvArgs a{};
+    a.x = static_cast<const uint16_t*>(x);
+    a.m[0] = packed(wts->gate, I, H);
+    a.m[1] = packed(wts->up, I, H);
+    a.M = (int)T;
+    a.N = I;
+    a.K = H;
+    a.group = cfg->group_size;
+    a.type = cfg->dtype;
+    a.out = ws.h;
+    a.gate = static_cast<uint16_t*>(gate);
+    a.up = static_cast<uint16_t*>(up);
+    a.act = cfg->activation;
+    DENSE_CUDA(ctx, fn, moe::launch_qmv(a, true, st));
+    moe::QmvArgs d{};
+    d.x = ws.h;
+    d.m[0] = packed(wts->down, H, I);
+    d.M = (int)T;
+    d.N = H;
+    d.K = I;
+    d.group = cfg->group_size;
+    d.type = cfg->dtype;
+    d.out = static_cast<uint16_t*>(out);
+    d.residual = static_cast<const uint16_t*>(residual);
+    d.early = 1;
+    DENSE_CUDA(ctx, fn, moe::launch_qmv(d, false, st));
+    return MOE_OK;
+  }
   moe::DequantArgs da{};
   da.jobs = 3;
   da.group = cfg->group_size;

@@ -73,6 +73,23 @@ cudaError_t launch_dense_gemm(const DenseGemm& g, cudaStream_t st);
 // Device status word of the dense kernels on the current device (bounded waits).
 cudaError_t dense_status(int32_t* status, cudaStream_t st);
 
+// ---- 4-bit products for few tokens (qmv.cu): out = x m[0]^T, or gated out = act(g) * u
+struct QmvArgs {
+  const uint16_t* x;  // [M][K]
+  PackedMatrix m[2];
+  int M, K, group, type;
+  int64_t N;
+  uint16_t* out;             // [M][N]
+  const uint16_t* residual;  // [M][N] added before the rounding, or null (not gated)
+  uint16_t* gate;            // gated: g and u [M][N] stored when non-null
+  uint16_t* up;
+  int act;
+  int early;                 // the weights may be read before the launch before has completed
+};
+// Tokens up to which these kernels are used instead of dequantisation and dense_gemm.cu.
+constexpr int kQmvMaxM = 32;
+cudaError_t launch_qmv(const QmvArgs& a, bool gated, cudaStream_t st);
+
 // ---- rotary positions (rope.cu)
 struct RopeArgs {
   const void* x;

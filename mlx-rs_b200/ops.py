@@ -18,6 +18,7 @@ and calls are ordered on torch's current stream.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -49,77 +50,96 @@ def _need(t, dtypes, name):
 
 
 _DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.float32: DTYPE_F32}
+_I64x3 = C.c_int64 * 3
 ACTIVATIONS = {"silu": ACT_SILU, "gelu": ACT_GELU}
 
 
-def _bound(fn, t):
-    """The device's context with its lock held, bound to torch's current stream there. The
-    caller releases the lock after its call: another thread may bind another stream."""
-    if not t.is_cuda:
+# The raw handle of torch's current stream on a device; through the stream object where this
+# torch has no direct way (that costs a few microseconds of each call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _context(fn, t):
+    """The context of the tensor's device. Its lock is held from binding torch's current
+    stream to the end of the call: another thread may bind another stream."""
+    index = t.get_device()
+    if index < 0:
         raise MlxError(fn, 1, "tensors must be on a CUDA device")
-    ctx = context_for(t.device.index)
-    ctx.lock.acquire()
-    ctx.bind_stream(torch.cuda.current_stream(t.device).cuda_stream)
-    return ctx
+    return context_for(index)
 
 
 def _workspace(nbytes, device):
     # from torch's allocator on the current stream: each call and each captured graph has its own
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
-def check_qweight(fn, name, q, rows, cols, dtype, device, group_size, bits=4):
-    """A packed matrix [rows, cols] with scales and biases of `dtype`, all on `device`."""
-    want = {"w": (rows, cols * bits // 32), "scales": (rows, cols // group_size), "biases": (rows, cols // group_size)}
-    for part, shape in want.items():
-        t = getattr(q, part)
+@functools.lru_cache(maxsize=4096)
+def _qmm_workspace(dtype, M, K, N, transpose, group_size, bits):
+    need = C.c_size_t()
+    rc = library().moe_quantized_matmul_workspace(dtype, M, K, N, transpose, group_size, bits, C.byref(need))
+    if rc:
+        raise MlxError("mlx_quantized_matmul", rc, f"unsupported call: M={M}, K={K}, N={N}")
+    return need.value
+
+
+@functools.lru_cache(maxsize=4096)
+def _ffn_workspace(hidden, inter, group_size, dtype, T, backward):
+    need = C.c_size_t()
+    cfg = FfnConfig(hidden, inter, ACT_SILU, group_size, 4, dtype)
+    rc = library().moe_gated_ffn_workspace(C.byref(cfg), T, backward, C.byref(need))
+    if rc:
+        raise MlxError("moe_gated_ffn", rc, f"unsupported call: T={T}, hidden={hidden}, inter={inter}")
+    return need.value
+
+
+def _check_packed(fn, name, w, scales, biases, rows, cols, dtype, index, group_size):
+    """A packed matrix [rows, cols] with scales and biases of `dtype`, all on device `index`."""
+    if w.shape != (rows, cols // 8) or w.dtype not in _WORD_DTYPES or not w.is_contiguous() or w.get_device() != index:
+        raise MlxError(fn, 1, f"{name}.w: contiguous 32-bit words {(rows, cols // 8)} on the input's device expected, "
+                              f"got {w.dtype} {tuple(w.shape)} on {w.device}")
+    shape = (rows, cols // group_size)
+    for part, t in (("scales", scales), ("biases", biases)):
         if t is None and part == "biases":
             continue
-        if t is None or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
-            got = "missing" if t is None else f"{tuple(t.shape)} on {t.device}"
-            raise MlxError(fn, 1, f"{name}.{part}: contiguous {shape} on {device} expected, got {got}")
-        if t.dtype not in (_WORD_DTYPES if part == "w" else {dtype}):
-            raise MlxError(fn, 1, f"{name}.{part}: dtype {t.dtype}")
+        if t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.get_device() != index:
+            raise MlxError(fn, 1, f"{name}.{part}: contiguous {dtype} {shape} on the input's device expected, "
+                                  f"got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-class _Q:
-    __slots__ = ("w", "scales", "biases")
-
-    def __init__(self, w, scales, biases):
-        self.w, self.scales, self.biases = w, scales, biases
+def check_qweight(fn, name, q, rows, cols, dtype, index, group_size):
+    _check_packed(fn, name, q.w, q.scales, q.biases, rows, cols, dtype, index, group_size)
 
 
 def _quantized_matmul_ex(x, w, scales, biases, transpose, group_size, bits):
     fn = "mlx_quantized_matmul"
-    if x.dtype not in (torch.bfloat16, torch.float16) or x.dim() < 1 or not x.is_contiguous():
+    dt = _DTYPES.get(x.dtype)
+    if dt is None or dt == DTYPE_F32 or x.dim() < 1 or not x.is_contiguous():
         raise MlxError(fn, 1, "x must be contiguous bf16 or f16 [..., K]")
     if bits != 4 or group_size not in (32, 64, 128):
         raise MlxError(fn, 2, f"bits={bits}, group_size={group_size} is not implemented")
     if w.dim() != 2:
         raise MlxError(fn, 1, "w must be [rows, cols*bits/32]")
     K = x.shape[-1]
-    cols = w.shape[1] * 8
-    N = w.shape[0] if transpose else cols
-    if (cols if transpose else w.shape[0]) != K or cols % group_size:
+    rows, words = w.shape
+    cols = words * 8
+    N = rows if transpose else cols
+    if (cols if transpose else rows) != K or cols % group_size or K == 0:
         raise MlxError(fn, 1, f"x [..., {K}] does not fit w {tuple(w.shape)} (transpose={bool(transpose)}, "
                               f"group_size={group_size})")
-    check_qweight(fn, "w", _Q(w, scales, biases), w.shape[0], cols, x.dtype, x.device, group_size)
-    M = x.numel() // K if K else 0
-    out = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
-    lib, dt, tr = library(), _DTYPES[x.dtype], int(bool(transpose))
-    need = C.c_size_t()
-    rc = lib.moe_quantized_matmul_workspace(dt, M, K, N, tr, group_size, bits, C.byref(need))
-    if rc:
-        raise MlxError(fn, rc, f"unsupported call: M={M}, K={K}, N={N}")
-    ws = _workspace(need.value, x.device)
-    ctx = _bound(fn, x)
-    try:
-        rc = lib.moe_quantized_matmul_ex(ctx.handle, dt, x.data_ptr(), M, K, w.data_ptr(), scales.data_ptr(),
-                                         biases.data_ptr() if biases is not None else None, N, tr, group_size, bits,
-                                         out.data_ptr(), ws.data_ptr() if ws is not None else None, need.value)
+    _check_packed(fn, "w", w, scales, biases, rows, cols, x.dtype, x.get_device(), group_size)
+    M = x.numel() // K
+    tr = 1 if transpose else 0
+    out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    need = _qmm_workspace(dt, M, K, N, tr, group_size, bits)
+    ws = _workspace(need, x.device) if need else None
+    ctx = _context(fn, x)
+    with ctx.lock:
+        ctx.bind_stream(_raw_stream(ctx.device))
+        rc = library().moe_quantized_matmul_ex(ctx.handle, dt, x.data_ptr(), M, K, w.data_ptr(), scales.data_ptr(),
+                                               biases.data_ptr() if biases is not None else None, N, tr, group_size, bits,
+                                               out.data_ptr(), ws.data_ptr() if need else None, need)
         ctx.check(fn, rc)
-    finally:
-        ctx.lock.release()
     return out
 
 
@@ -238,7 +258,7 @@ def _ffn_call(fn, x, gate, up, down, activation, group_size, bits):
     if H == 0 or H % group_size or I == 0 or I % group_size:
         raise MlxError(fn, 1, f"hidden={H} and inter={I} must be positive multiples of group_size={group_size}")
     for name, q, rows, cols in (("gate", gate, I, H), ("up", up, I, H), ("down", down, H, I)):
-        check_qweight(fn, name, q, rows, cols, x.dtype, x.device, group_size)
+        check_qweight(fn, name, q, rows, cols, x.dtype, x.get_device(), group_size)
     return ffn_structs(H, I, x.dtype, gate, up, down, activation, group_size, bits)
 
 
@@ -260,21 +280,18 @@ def _ffn_forward(cfg, wts, x, residual, save):
     out = torch.empty_like(x)
     g = u = None
     if save:
-        g = torch.empty(*x.shape[:-1], cfg.inter, dtype=x.dtype, device=x.device)
+        g = torch.empty((*x.shape[:-1], cfg.inter), dtype=x.dtype, device=x.device)
         u = torch.empty_like(g)
-    lib = library()
-    need = C.c_size_t()
-    lib.moe_gated_ffn_workspace(C.byref(cfg), T, 0, C.byref(need))
-    ws = _workspace(need.value, x.device)
-    ctx = _bound(fn, x)
-    try:
-        rc = lib.moe_gated_ffn_forward(ctx.handle, C.byref(cfg), C.byref(wts), x.data_ptr(), T,
-                                       residual.data_ptr() if residual is not None else None,
-                                       g.data_ptr() if save else None, u.data_ptr() if save else None,
-                                       out.data_ptr(), ws.data_ptr() if ws is not None else None, need.value)
+    need = _ffn_workspace(cfg.hidden, cfg.inter, cfg.group_size, cfg.dtype, T, 0)
+    ws = _workspace(need, x.device)
+    ctx = _context(fn, x)
+    with ctx.lock:
+        ctx.bind_stream(_raw_stream(ctx.device))
+        rc = library().moe_gated_ffn_forward(ctx.handle, cfg, wts, x.data_ptr(), T,
+                                             None if residual is None else residual.data_ptr(),
+                                             g.data_ptr() if save else None, u.data_ptr() if save else None,
+                                             out.data_ptr(), ws.data_ptr(), need)
         ctx.check(fn, rc)
-    finally:
-        ctx.lock.release()
     return (out, g, u) if save else out
 
 
@@ -284,18 +301,14 @@ def _ffn_backward(cfg, wts, g, u, dy):
     _like(fn, "gate", g, (*dy.shape[:-1], cfg.inter), dy)
     _like(fn, "up", u, (*dy.shape[:-1], cfg.inter), dy)
     dx, dgate, dup = torch.empty_like(dy), torch.empty_like(g), torch.empty_like(u)
-    lib = library()
-    need = C.c_size_t()
-    lib.moe_gated_ffn_workspace(C.byref(cfg), T, 1, C.byref(need))
-    ws = _workspace(need.value, dy.device)
-    ctx = _bound(fn, dy)
-    try:
-        rc = lib.moe_gated_ffn_backward(ctx.handle, C.byref(cfg), C.byref(wts), g.data_ptr(), u.data_ptr(),
-                                        dy.data_ptr(), T, dgate.data_ptr(), dup.data_ptr(), dx.data_ptr(),
-                                        ws.data_ptr() if ws is not None else None, need.value)
+    need = _ffn_workspace(cfg.hidden, cfg.inter, cfg.group_size, cfg.dtype, T, 1)
+    ws = _workspace(need, dy.device)
+    ctx = _context(fn, dy)
+    with ctx.lock:
+        ctx.bind_stream(_raw_stream(ctx.device))
+        rc = library().moe_gated_ffn_backward(ctx.handle, cfg, wts, g.data_ptr(), u.data_ptr(), dy.data_ptr(), T,
+                                              dgate.data_ptr(), dup.data_ptr(), dx.data_ptr(), ws.data_ptr(), need)
         ctx.check(fn, rc)
-    finally:
-        ctx.lock.release()
     return dx, dgate, dup
 
 
@@ -329,57 +342,48 @@ def fast_rope(x, dims, traditional=False, base=10000.0, scale=1.0, offset=0, fre
     transposed rotation, the gradient with respect to x. out: where to write, x itself
     included (default: a new contiguous tensor). bf16, f16 or f32."""
     fn = "mlx_fast_rope"
-    if x.dtype not in _DTYPES or x.dim() < 2:
+    dt = _DTYPES.get(x.dtype)
+    nd = x.dim()
+    if dt is None or nd < 2:
         raise MlxError(fn, 1, "x must be bf16, f16 or f32 [..., L, D]")
-    xv = x
-    if x.dim() != 4:
-        if isinstance(offset, torch.Tensor) and offset.dim() and x.dim() != 3:
-            raise MlxError(fn, 1, "offsets per batch element need x [B, H, L, D] or [B, L, D]")
-        if x.dim() == 3:
-            xv = x[:, None]
-        else:
-            if not x.is_contiguous():
-                raise MlxError(fn, 1, "x: must be contiguous unless [B, H, L, D] or [B, L, D]")
-            xv = x.reshape(1, -1, *x.shape[-2:])
-    B, H, L, D = xv.shape
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
         raise MlxError(fn, 1, f"out: {x.dtype} {tuple(x.shape)} on {x.device} expected")
-    if out is x or out.data_ptr() == x.data_ptr():
-        if out.stride() != x.stride():
-            raise MlxError(fn, 1, "out shares x's memory with other strides")
-    if x.dim() == 4:
-        ov = out
-    elif x.dim() == 3:
-        ov = out[:, None]
+    elif out.data_ptr() == x.data_ptr() and out.stride() != x.stride():
+        raise MlxError(fn, 1, "out shares x's memory with other strides")
+    xs, os_ = x.stride(), out.stride()
+    if nd == 4:
+        B, H, L, D = x.shape
+    elif nd == 3:
+        (B, L, D), H = x.shape, 1
+        xs, os_ = (xs[0], 0, xs[1], xs[2]), (os_[0], 0, os_[1], os_[2])
     else:
-        if not out.is_contiguous():
-            raise MlxError(fn, 1, "out: must be contiguous unless [B, H, L, D] or [B, L, D]")
-        ov = out.view(1, -1, L, D)
-    xs, os_ = xv.stride(), ov.stride()
+        if not (x.is_contiguous() and out.is_contiguous()):
+            raise MlxError(fn, 1, "x and out: must be contiguous unless [B, H, L, D] or [B, L, D]")
+        L, D = x.shape[-2:]
+        B, H = 1, x.numel() // (L * D) if L * D else 0
+        xs = os_ = (0, L * D, D, 1)
     if D > 1 and (xs[3] != 1 or os_[3] != 1):
         raise MlxError(fn, 1, "the channels of x and out must be contiguous")
     offs, offs_bits, off = None, 0, 0
     if isinstance(offset, torch.Tensor):
-        if offset.dtype not in (torch.int32, torch.int64) or offset.device != x.device or not offset.is_contiguous() \
-                or offset.numel() != B or offset.dim() > 1:
+        if nd not in (3, 4) and offset.dim():
+            raise MlxError(fn, 1, "offsets per batch element need x [B, H, L, D] or [B, L, D]")
+        if offset.dtype not in (torch.int32, torch.int64) or offset.device != x.device or offset.dim() > 1 \
+                or offset.numel() != B or not offset.is_contiguous():
             raise MlxError(fn, 1, f"offset: contiguous int32 or int64 [{B}] on {x.device} expected")
         offs, offs_bits = offset.data_ptr(), 32 if offset.dtype == torch.int32 else 64
     else:
         off = int(offset)
     if freqs is not None and (freqs.dtype != torch.float32 or freqs.device != x.device or
-                              tuple(freqs.shape) != (dims // 2,) or not freqs.is_contiguous()):
+                              freqs.shape != (dims // 2,) or not freqs.is_contiguous()):
         raise MlxError(fn, 1, f"freqs: contiguous float32 [{dims // 2}] on {x.device} expected")
-    cfg = RopeConfig(_DTYPES[x.dtype], dims, int(bool(traditional)), int(bool(inverse)),
-                     float(base) if base is not None else 0.0, scale, mscale)
-    i3 = C.c_int64 * 3
-    ctx = _bound(fn, x)
-    try:
-        rc = library().moe_fast_rope(ctx.handle, C.byref(cfg), x.data_ptr(), i3(*xs[:3]), B, H, L, D, off, offs,
-                                     offs_bits, freqs.data_ptr() if freqs is not None else None, out.data_ptr(),
-                                     i3(*os_[:3]))
+    cfg = RopeConfig(dt, dims, 1 if traditional else 0, 1 if inverse else 0, 0.0 if base is None else base, scale, mscale)
+    ctx = _context(fn, x)
+    with ctx.lock:
+        ctx.bind_stream(_raw_stream(ctx.device))
+        rc = library().moe_fast_rope(ctx.handle, cfg, x.data_ptr(), _I64x3(*xs[:3]), B, H, L, D, off, offs, offs_bits,
+                                     None if freqs is None else freqs.data_ptr(), out.data_ptr(), _I64x3(*os_[:3]))
         ctx.check(fn, rc)
-    finally:
-        ctx.lock.release()
     return out

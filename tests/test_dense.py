@@ -112,7 +112,7 @@ def test_ffn_refusals():
     assert "CUDA" in _refused(call)
     assert "up.w" in _refused(call, u=mk(64, 64))
     assert "down.w" in _refused(call, d=mk(96, 64))
-    assert "scales: dtype" in _refused(call, g=mk(96, 64, torch.float16))
+    assert "gate.scales" in _refused(call, g=mk(96, 64, torch.float16))
     assert "activation" in _refused(call, activation="relu")
     assert "rc=2" in _refused(call, bits=3)
     assert "rc=2" in _refused(call, group_size=16)
