@@ -135,7 +135,7 @@ enum moe_dtype { MOE_DTYPE_BF16 = 0, MOE_DTYPE_F16 = 1, MOE_DTYPE_F32 = 2 };
  *   transpose == 0: out[M, N] = x[M, K] . dequant(w),   w [K, N / 8], scales [K, N / gs]
  * (the second is the gradient of the first with respect to its input). K (N when transpose
  * is 0) must be a multiple of group_size; all pointers 16-byte aligned; out overlaps no
- * input. The workspace (moe_quantized_matmul_workspace bytes, 16-byte aligned, contents
+ * input. The workspace (moe_quantized_matmul_workspace bytes, 32-byte aligned, contents
  * irrelevant) belongs to the call until it has run: calls that may overlap need one each.
  * Array::quantized_matmul, crates/mlx-core/src/ops.rs:592-637.
  */

@@ -99,8 +99,8 @@ int64_t qmm_piece(int64_t N, int64_t K) {
 }
 
 struct QmmWs {
-  uint16_t* w;      // [piece][ld] 16-bit weight rows (columns when !transpose)
-  uint16_t* xpad;   // [M][ld] when K is no multiple of 8
+  uint16_t* w;      // 16-bit weights: [piece][K], or [K][piece] when !transpose
+  uint16_t* xpad;   // [M][K rounded up to 8] when K is no multiple of 8
   float* partial;
   size_t partial_bytes, bytes;
 };
@@ -155,7 +155,7 @@ int check_ffn_weights(moe_ctx* ctx, const char* fn, const moe_ffn_weights* w) {
 }
 
 struct FfnWs {
-  uint16_t *wg, *wu, *wd;  // 16-bit weights, transposed for the backward pass
+  uint16_t *wg, *wu, *wd;  // 16-bit weights
   uint16_t* h;             // [T][I] (forward)
   float* partial;
   size_t partial_bytes, bytes;
@@ -189,7 +189,8 @@ int check_workspace(moe_ctx* ctx, const char* fn, const void* ws, size_t have, s
   if (need == 0) return MOE_OK;
   if (!ws || have < need)
     return fail(ctx, MOE_ERR_INVALID, "%s: workspace of %zu bytes, %zu needed", fn, ws ? have : (size_t)0, need);
-  if (!aligned16(ws)) return fail(ctx, MOE_ERR_INVALID, "%s: workspace must be 16-byte aligned", fn);
+  if (reinterpret_cast<uintptr_t>(ws) & 31)
+    return fail(ctx, MOE_ERR_INVALID, "%s: workspace must be 32-byte aligned", fn);
   return MOE_OK;
 }
 
@@ -243,10 +244,10 @@ int moe_quantized_matmul_ex(moe_ctx* ctx, int dtype, const void* x, int64_t M, i
     DENSE_CUDA(ctx, fn, moe::launch_qmv(a, false, st));
     return MOE_OK;
   }
-  const int64_t ld = up8(K);
+  const int64_t ldx = up8(K);
   const uint16_t* xs = static_cast<const uint16_t*>(x);
   if (ws.xpad) {
-    DENSE_CUDA(ctx, fn, moe::launch_pad_rows(xs, M, K, ws.xpad, ld, st));
+    DENSE_CUDA(ctx, fn, moe::launch_pad_rows(xs, M, K, ws.xpad, ldx, st));
     xs = ws.xpad;
   }
   const int64_t piece = qmm_piece(N, K);
@@ -256,7 +257,6 @@ int moe_quantized_matmul_ex(moe_ctx* ctx, int dtype, const void* x, int64_t M, i
     da.jobs = 1;
     da.group = group_size;
     da.type = dtype;
-    da.transposed = !transpose;
     const int64_t inner = transpose ? K : N;
     moe::PackedMatrix m = packed(q, transpose ? n : K, inner);
     m.w_pitch = (int)(inner / 8);
@@ -272,12 +272,14 @@ int moe_quantized_matmul_ex(moe_ctx* ctx, int dtype, const void* x, int64_t M, i
       if (m.b) m.b += n0 / group_size;
       m.cols = (int)n;
     }
-    da.job[0] = {m, ws.w, ld};
+    da.job[0] = {m, ws.w, transpose ? ldx : piece};
     DENSE_CUDA(ctx, fn, moe::launch_dequant(da, st));
     moe::DenseGemm gm{};
     gm.a[0] = xs;
     gm.b[0] = ws.w;
-    gm.lda[0] = gm.ldb[0] = ld;
+    gm.lda[0] = ldx;
+    gm.ldb[0] = transpose ? ldx : piece;
+    gm.b_rows_k = !transpose;
     gm.pairs = 1;
     gm.M = M;
     gm.N = (int)n;
@@ -424,22 +426,23 @@ int moe_gated_ffn_backward(moe_ctx* ctx, const moe_ffn_config* cfg, const moe_ff
   const cudaStream_t st = static_cast<cudaStream_t>(moe_internal::ctx_stream(ctx));
   const int H = cfg->hidden, I = cfg->inter;
 
-  // the three matrices transposed: the products below sum over the weights' rows
+  // the products below sum over the weights' rows
   moe::DequantArgs da{};
   da.jobs = 3;
   da.group = cfg->group_size;
   da.type = cfg->dtype;
-  da.transposed = 1;
-  da.job[0] = {packed(wts->gate, I, H), ws.wg, I};
-  da.job[1] = {packed(wts->up, I, H), ws.wu, I};
-  da.job[2] = {packed(wts->down, H, I), ws.wd, H};
+  da.job[0] = {packed(wts->gate, I, H), ws.wg, H};
+  da.job[1] = {packed(wts->up, I, H), ws.wu, H};
+  da.job[2] = {packed(wts->down, H, I), ws.wd, I};
   for (auto& j : da.job) j.m.w_pitch = j.m.cols / 8, j.m.s_pitch = j.m.cols / cfg->group_size;
   DENSE_CUDA(ctx, fn, moe::launch_dequant(da, st));
 
   moe::DenseGemm dh{};
   dh.a[0] = static_cast<const uint16_t*>(dy);
   dh.b[0] = ws.wd;
-  dh.lda[0] = dh.ldb[0] = H;
+  dh.lda[0] = H;
+  dh.ldb[0] = I;
+  dh.b_rows_k = 1;
   dh.pairs = 1;
   dh.M = T;
   dh.N = I;
@@ -461,7 +464,9 @@ int moe_gated_ffn_backward(moe_ctx* ctx, const moe_ffn_config* cfg, const moe_ff
   dxg.a[1] = static_cast<const uint16_t*>(dup);
   dxg.b[0] = ws.wg;
   dxg.b[1] = ws.wu;
-  dxg.lda[0] = dxg.lda[1] = dxg.ldb[0] = dxg.ldb[1] = I;
+  dxg.lda[0] = dxg.lda[1] = I;
+  dxg.ldb[0] = dxg.ldb[1] = H;
+  dxg.b_rows_k = 1;
   dxg.pairs = 2;
   dxg.M = T;
   dxg.N = H;

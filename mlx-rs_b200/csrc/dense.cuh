@@ -27,15 +27,15 @@ struct PackedMatrix {
 // ---- dequantisation into 16-bit rows (dense_dequant.cu)
 struct DequantJob {
   PackedMatrix m;
-  uint16_t* out;   // [rows][ld], or [cols][ld] when transposed
+  uint16_t* out;   // [rows][ld], 32-byte aligned rows
   int64_t ld;
 };
 struct DequantArgs {
   DequantJob job[3];
   int jobs;
   int group;
-  int transposed;
   int type;
+  uint32_t rows_cta;  // set by launch_dequant
 };
 cudaError_t launch_dequant(const DequantArgs& a, cudaStream_t st);
 // out[r][0..cols) = x[r][0..cols), rows ld elements apart, the rest of each row zero.
@@ -55,11 +55,13 @@ struct DenseEpi {
 };
 struct DenseGemm {
   // D[M, N] = sum over the operand pairs p of A_p[M, K_p] . B_p[N, K_p]^T (one or two
-  // pairs); in the gated form one A and two B: g = A . B_0^T, u = A . B_1^T.
+  // pairs), or . B_p[K_p, N] with b_rows_k; in the gated form one A and two B:
+  // g = A . B_0^T, u = A . B_1^T.
   const uint16_t* a[2];
   const uint16_t* b[2];
   int64_t lda[2], ldb[2];
   int pairs;
+  int b_rows_k;
   int64_t M;
   int N, K;
   int type;      // kBf16 / kF16
@@ -133,6 +135,55 @@ struct Elem<kF16> {
   static MOE_DEV float lo(uint32_t v) { return to_f((uint16_t)(v & 0xffffu)); }
   static MOE_DEV float hi(uint32_t v) { return to_f((uint16_t)(v >> 16)); }
 };
+
+// Two 4-bit fields of a word as 16 + q, exact in either type: the field becomes the top
+// mantissa bits under the exponent of 16 (one shift and one LOP3).
+template <int TYPE>
+struct Nib;
+template <>
+struct Nib<kBf16> {
+  static constexpr uint32_t kMask = 0x00780078u, kBase = 0x41804180u, kOne = 0x3f803f80u;
+  static constexpr int kBit = 3;  // lowest mantissa bit of the field
+};
+template <>
+struct Nib<kF16> {
+  static constexpr uint32_t kMask = 0x03c003c0u, kBase = 0x4c004c00u, kOne = 0x3c003c00u;
+  static constexpr int kBit = 6;
+};
+// fields j and j + 4 of w
+template <int TYPE, int J>
+MOE_DEV uint32_t fields(uint32_t w) {
+  constexpr int sh = Nib<TYPE>::kBit - 4 * J;
+  const uint32_t v = sh >= 0 ? w << (sh >= 0 ? sh : 0) : w >> (sh >= 0 ? 0 : -sh);
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;\n" : "=r"(r) : "r"(v), "n"(Nib<TYPE>::kMask), "n"(Nib<TYPE>::kBase));
+  return r;
+}
+// RN(s * q + b) of a pair of fields: the subtraction of 16 is exact, the fused multiply-add
+// rounds once. s2 / b2: the scale / bias in both halves.
+template <int TYPE>
+MOE_DEV uint32_t scale2(uint32_t f, uint32_t s2, uint32_t b2) {
+  uint32_t q, r;
+  if constexpr (TYPE == kBf16) {
+    asm("sub.rn.bf16x2 %0, %1, %2;\n" : "=r"(q) : "r"(f), "r"(Nib<TYPE>::kBase));
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;\n" : "=r"(r) : "r"(q), "r"(s2), "r"(b2));
+  } else {
+    asm("sub.rn.f16x2 %0, %1, %2;\n" : "=r"(q) : "r"(f), "r"(Nib<TYPE>::kBase));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(r) : "r"(q), "r"(s2), "r"(b2));
+  }
+  return r;
+}
+// A word's eight weights in element order.
+template <int TYPE>
+MOE_DEV uint4 dequant8(uint32_t w, uint32_t s2, uint32_t b2) {
+  const uint32_t f0 = fields<TYPE, 0>(w), f1 = fields<TYPE, 1>(w), f2 = fields<TYPE, 2>(w), f3 = fields<TYPE, 3>(w);
+  uint4 o;
+  o.x = scale2<TYPE>(__byte_perm(f0, f1, 0x5410), s2, b2);
+  o.y = scale2<TYPE>(__byte_perm(f2, f3, 0x5410), s2, b2);
+  o.z = scale2<TYPE>(__byte_perm(f0, f1, 0x7632), s2, b2);
+  o.w = scale2<TYPE>(__byte_perm(f2, f3, 0x7632), s2, b2);
+  return o;
+}
 
 // 1 / (1 + exp(-x)) from the hardware base-2 exponential and reciprocal (relative error a
 // few fp32 ulps, far below the 16-bit rounding that follows).

@@ -10,83 +10,52 @@ namespace moe {
 
 namespace {
 
-template <int TYPE>
-MOE_DEV uint4 dequant_word(uint32_t w, float s, float b) {
-  float v[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = __fmaf_rn(s, (float)((w >> (4 * e)) & 15u), b);
-  return make_uint4(Elem<TYPE>::pack(v[0], v[1]), Elem<TYPE>::pack(v[2], v[3]), Elem<TYPE>::pack(v[4], v[5]),
-                    Elem<TYPE>::pack(v[6], v[7]));
-}
+constexpr int kSteps = 4;  // pairs of words in flight per thread
 
-constexpr int kWordsPerThread = 4;
-
-// Row-major: thread = words wi, wi + 256, ... of the flattened matrix, so that a warp reads
-// 128 and writes 512 contiguous bytes per step.
+// Thread = two words (16 weights of one group) at a time, kSteps of them 256 pairs apart, so
+// that a warp reads 256 and writes 1024 contiguous bytes per step. The row and column of a
+// thread's first pair take one division; the next ones follow by addition.
 template <int TYPE>
-__global__ void __launch_bounds__(256) dequant_rows_kernel(const __grid_constant__ DequantArgs a) {
-  pdl_wait();
+__global__ void __launch_bounds__(256) dequant_kernel(const __grid_constant__ DequantArgs a) {
   const DequantJob& j = a.job[blockIdx.y];
-  const int wpr = j.m.cols >> 3, wpg = a.group >> 3;
-  const int64_t total = j.m.rows * wpr;
-  const int64_t base = (int64_t)blockIdx.x * (256 * kWordsPerThread) + threadIdx.x;
-#pragma unroll
-  for (int i = 0; i < kWordsPerThread; ++i) {
-    const int64_t wi = base + i * 256;
-    if (wi >= total) break;
-    const int64_t row = wi / wpr;
-    const int c = (int)(wi - row * wpr);
-    const int64_t g = row * j.m.s_pitch + c / wpg;
-    const float s = Elem<TYPE>::to_f(j.m.s[g]);
-    const float b = j.m.b ? Elem<TYPE>::to_f(j.m.b[g]) : 0.0f;
-    *reinterpret_cast<uint4*>(j.out + row * j.ld + c * 8) = dequant_word<TYPE>(__ldg(j.m.w + row * j.m.w_pitch + c), s, b);
-  }
-}
-
-// Transposed: a CTA turns 64 rows x 64 columns. Lane = a pair of rows, warp = a word of 8
-// columns: the pair's elements leave as one 32-bit shared store per column (conflict-free),
-// then each column's 64 rows leave as 128 contiguous bytes.
-template <int TYPE>
-__global__ void __launch_bounds__(256) dequant_cols_kernel(const __grid_constant__ DequantArgs a) {
-  __shared__ __align__(16) uint32_t tile[64][36];  // [column][pair of rows], 144-byte rows
+  const uint32_t ppr = (uint32_t)j.m.cols >> 4, ppg = (uint32_t)a.group >> 4;  // pairs per row, per group
+  const uint32_t rows_cta = a.rows_cta;
+  const int64_t row0 = (int64_t)blockIdx.x * rows_cta;
+  if (row0 >= j.m.rows) return;
+  const uint32_t rows = (uint32_t)(j.m.rows - row0 < rows_cta ? j.m.rows - row0 : rows_cta);
+  const uint32_t* w = j.m.w + row0 * j.m.w_pitch;
+  const uint16_t* s = j.m.s + row0 * j.m.s_pitch;
+  const uint16_t* b = j.m.b ? j.m.b + row0 * j.m.s_pitch : nullptr;
+  uint16_t* out = j.out + row0 * j.ld;
+  uint32_t r = threadIdx.x / ppr, c = threadIdx.x - r * ppr;
+  const uint32_t dr = 256 / ppr, dc = 256 - dr * ppr;
   pdl_wait();
-  const DequantJob& j = a.job[blockIdx.z];
-  const int wpr = j.m.cols >> 3, wpg = a.group >> 3;
-  const int64_t n0 = (int64_t)blockIdx.x * 64;
-  const int c0 = blockIdx.y * 8;
-  if (n0 >= j.m.rows || c0 >= wpr) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = c0 + warp;
-  if (c < wpr) {
-    uint32_t v[2][4];
+  pdl_trigger();
+  while (r < rows) {
+    uint2 q[kSteps];
+    uint32_t sc[kSteps], bi[kSteps], rr[kSteps], cc[kSteps];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int64_t row = n0 + 2 * lane + h;
-      uint4 d = make_uint4(0, 0, 0, 0);
-      if (row < j.m.rows) {
-        const int64_t g = row * j.m.s_pitch + c / wpg;
-        const float s = Elem<TYPE>::to_f(j.m.s[g]);
-        const float b = j.m.b ? Elem<TYPE>::to_f(j.m.b[g]) : 0.0f;
-        d = dequant_word<TYPE>(__ldg(j.m.w + row * j.m.w_pitch + c), s, b);
+    for (int i = 0; i < kSteps; ++i) {
+      rr[i] = r, cc[i] = c;
+      if (r < rows) {
+        q[i] = __ldg(reinterpret_cast<const uint2*>(w + (size_t)r * j.m.w_pitch) + c);
+        const size_t g = (size_t)r * j.m.s_pitch + c / ppg;
+        sc[i] = __ldg(s + g);
+        bi[i] = b ? __ldg(b + g) : 0u;
       }
-      v[h][0] = d.x, v[h][1] = d.y, v[h][2] = d.z, v[h][3] = d.w;
+      r += dr, c += dc;
+      if (c >= ppr) c -= ppr, ++r;
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      tile[warp * 8 + 2 * e][lane] = __byte_perm(v[0][e], v[1][e], 0x5410);
-      tile[warp * 8 + 2 * e + 1][lane] = __byte_perm(v[0][e], v[1][e], 0x7632);
+    for (int i = 0; i < kSteps; ++i) {
+      if (rr[i] >= rows) break;
+      const uint32_t s2 = __byte_perm(sc[i], 0, 0x1010), b2 = __byte_perm(bi[i], 0, 0x1010);
+      const uint4 lo = dequant8<TYPE>(q[i].x, s2, b2), hi = dequant8<TYPE>(q[i].y, s2, b2);
+      uint16_t* o = out + (size_t)rr[i] * j.ld + cc[i] * 16;
+      asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"l"(o), "r"(lo.x), "r"(lo.y), "r"(lo.z),
+                   "r"(lo.w), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w)
+                   : "memory");
     }
-  }
-  __syncthreads();
-  // 64 columns x 8 pieces of 16 bytes; ld is a multiple of 8 and covers the rows rounded
-  // up to 8, so a piece that starts inside the rows lies inside the output row
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int p = threadIdx.x + 256 * i;
-    const int col = p >> 3, piece = p & 7;
-    if (c0 * 8 + col < j.m.cols && n0 + piece * 8 < j.m.rows)
-      *reinterpret_cast<uint4*>(j.out + (int64_t)(c0 * 8 + col) * j.ld + n0 + piece * 8) =
-          *reinterpret_cast<const uint4*>(&tile[col][piece * 4]);
   }
 }
 
@@ -101,24 +70,20 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* __restric
 
 }  // namespace
 
-cudaError_t launch_dequant(const DequantArgs& a, cudaStream_t st) {
-  int64_t rows = 0, words = 0;
+cudaError_t launch_dequant(const DequantArgs& args, cudaStream_t st) {
+  DequantArgs a = args;
+  int64_t rows = 0;
   int cols = 0;
   for (int i = 0; i < a.jobs; ++i) {
     rows = rows > a.job[i].m.rows ? rows : a.job[i].m.rows;
     cols = cols > a.job[i].m.cols ? cols : a.job[i].m.cols;
-    const int64_t n = a.job[i].m.rows * (a.job[i].m.cols / 8);
-    words = words > n ? words : n;
   }
-  if (!a.transposed) {
-    const int64_t per = 256 * kWordsPerThread;
-    const dim3 grid((unsigned)((words + per - 1) / per), a.jobs);
-    return a.type == kF16 ? launch_k(dequant_rows_kernel<kF16>, grid, dim3(256), 0, st, a)
-                          : launch_k(dequant_rows_kernel<kBf16>, grid, dim3(256), 0, st, a);
-  }
-  const dim3 grid((unsigned)((rows + 63) / 64), (unsigned)((cols + 63) / 64), a.jobs);
-  return a.type == kF16 ? launch_k(dequant_cols_kernel<kF16>, grid, dim3(256), 0, st, a)
-                        : launch_k(dequant_cols_kernel<kBf16>, grid, dim3(256), 0, st, a);
+  // rows per CTA: about two rounds of a thread's steps in the widest matrix
+  a.rows_cta = 256 * 2 * kSteps / (cols / 16);
+  if (a.rows_cta < 1) a.rows_cta = 1;
+  const dim3 grid((unsigned)((rows + a.rows_cta - 1) / a.rows_cta), a.jobs);
+  return a.type == kF16 ? launch_k(dequant_kernel<kF16>, grid, dim3(256), 0, st, a)
+                        : launch_k(dequant_kernel<kBf16>, grid, dim3(256), 0, st, a);
 }
 
 cudaError_t launch_pad_rows(const uint16_t* x, int64_t rows, int64_t cols, uint16_t* out, int64_t ld, cudaStream_t st) {

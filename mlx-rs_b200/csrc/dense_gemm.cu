@@ -18,6 +18,11 @@
 // K can be split over several CTAs when there are fewer tiles than SMs: fp32 partial sums,
 // then one launch that adds them in split order and applies the epilogue (no atomics, the
 // same bits on every run).
+// B may lie with its N contiguous (BN_MAJOR: the weights' rows are the summed index, in the
+// backward pass): boxes of 64 columns x 64 rows, read through the MN-major descriptor, so
+// that both directions use the weights as they are stored.
+// The epilogue moves global memory through a 2 KB buffer per warp: a thread owns a row of the
+// accumulator, but a warp's accesses cover 64 contiguous bytes of eight rows each.
 // Every wait is bounded (2 s): on expiry the CTA records a code in the device's status word,
 // stops working and leaves through the same barriers as the rest of its pair.
 #include <cudaTypedefs.h>
@@ -34,6 +39,7 @@ constexpr int kBHalf = 128 * kBK * 2;        // 16 KB: 128 weight rows
 constexpr int kEpiWarps = 8;
 constexpr int kTmaWarp = 8, kMmaWarp = 9;
 constexpr int kThreads = 320;
+constexpr int kStage2K = 2048;               // 32 rows x 32 columns of 16 bits
 constexpr uint64_t kWaitLimitNs = 2000ull * 1000 * 1000;
 
 __device__ int32_t g_dense_status;
@@ -42,8 +48,9 @@ template <int CG>
 struct Cfg {
   static constexpr int kStages = CG == 2 ? 6 : 4;
   static constexpr int kStageBytes = kATile + (CG == 2 ? 1 : 2) * kBHalf;
-  static constexpr int kBars = kStages * kStageBytes;
   // full[S] empty[S] acc_full[2] acc_empty[2] | tmem base
+  static constexpr int kStaging = kStages * kStageBytes;  // [epilogue warps][2 KB]
+  static constexpr int kBars = kStaging + kEpiWarps * kStage2K;
   static constexpr int kSmem = kBars + 8 * (2 * kStages + 4) + 16 + 1024;
 };
 
@@ -147,6 +154,12 @@ MOE_DEV uint64_t sw128_desc(uint32_t saddr) {
   return (uint64_t)((saddr >> 4) & 0x3fffu) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
          (uint64_t)2 << 61;
 }
+// N-contiguous operand: 64-column blocks of 64 rows x 128 bytes (8 KB apart, the leading
+// offset), 8-row groups 1024 bytes apart.
+MOE_DEV uint64_t sw128_mn_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3fffu) | (uint64_t)(8192 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
 MOE_DEV void tmem_ld32(uint32_t taddr, float (&r)[32]) {
   uint32_t* u = reinterpret_cast<uint32_t*>(r);
   asm volatile(
@@ -228,7 +241,65 @@ MOE_DEV void epilogue8(const DenseEpi& e, int64_t m, int c, int n, bool vec, flo
   }
 }
 
-template <int CG, int EPI, int TYPE>
+// ---- a warp's 32 rows x 32 columns through its staging buffer. 16-byte piece j of row r lies
+// at piece j ^ ((r >> 1) & 3): conflict-free both by row (one lane each) and by four lanes
+// of a row. cols: valid columns (a multiple of 8), rows: valid rows.
+MOE_DEV uint32_t stage_off(int r, int j) { return (uint32_t)(r * 64 + ((j ^ ((r >> 1) & 3)) << 4)); }
+MOE_DEV void sts16(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+MOE_DEV uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+template <int TYPE>
+MOE_DEV void store_tile(uint32_t stage, const float (&v)[32], uint16_t* base, int64_t ld, int rows, int cols, int lane) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    sts16(stage + stage_off(lane, j),
+          make_uint4(Elem<TYPE>::pack(v[8 * j], v[8 * j + 1]), Elem<TYPE>::pack(v[8 * j + 2], v[8 * j + 3]),
+                     Elem<TYPE>::pack(v[8 * j + 4], v[8 * j + 5]), Elem<TYPE>::pack(v[8 * j + 6], v[8 * j + 7])));
+  __syncwarp();
+  const int j = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 8 * i + (lane >> 2);
+    const uint4 q = lds16(stage + stage_off(r, j));
+    if (r < rows && 8 * j < cols) *reinterpret_cast<uint4*>(base + (int64_t)r * ld + 8 * j) = q;
+  }
+  __syncwarp();
+}
+struct Tile32 {
+  uint4 q[4];
+};
+MOE_DEV void fetch_tile(Tile32& t, const uint16_t* base, int64_t ld, int rows, int cols, int lane) {
+  const int j = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 8 * i + (lane >> 2);
+    t.q[i] = r < rows && 8 * j < cols ? *reinterpret_cast<const uint4*>(base + (int64_t)r * ld + 8 * j)
+                                      : make_uint4(0, 0, 0, 0);
+  }
+}
+// The fetched tile, turned: this lane's row.
+template <int TYPE>
+MOE_DEV void turn_tile(uint32_t stage, const Tile32& t, float (&v)[32], int lane) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sts16(stage + stage_off(8 * i + (lane >> 2), lane & 3), t.q[i]);
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint4 q = lds16(stage + stage_off(lane, j));
+    v[8 * j] = Elem<TYPE>::lo(q.x), v[8 * j + 1] = Elem<TYPE>::hi(q.x);
+    v[8 * j + 2] = Elem<TYPE>::lo(q.y), v[8 * j + 3] = Elem<TYPE>::hi(q.y);
+    v[8 * j + 4] = Elem<TYPE>::lo(q.z), v[8 * j + 5] = Elem<TYPE>::hi(q.z);
+    v[8 * j + 6] = Elem<TYPE>::lo(q.w), v[8 * j + 7] = Elem<TYPE>::hi(q.w);
+  }
+  __syncwarp();
+}
+
+template <int CG, int EPI, int TYPE, bool BN_MAJOR>
 __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
   using C = Cfg<CG>;
   extern __shared__ unsigned char smem_raw[];
@@ -319,9 +390,15 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
 #pragma unroll
           for (int h = 0; h < (CG == 2 ? 1 : 2); ++h) {
             const int half = CG == 2 ? (int)rank : h;
-            const CUtensorMap* bm = p.gated ? &p.b[half] : &p.b[pr];
-            const int y = p.gated ? nt * 128 : nt * kBN + half * 128;
-            tma_2d<CG>(st + kATile + h * kBHalf, bm, x, y, bar);
+            if constexpr (BN_MAJOR) {
+              const int n = nt * kBN + half * 128;
+              tma_2d<CG>(st + kATile + h * kBHalf, &p.b[pr], n, x, bar);
+              tma_2d<CG>(st + kATile + h * kBHalf + kBHalf / 2, &p.b[pr], n + 64, x, bar);
+            } else {
+              const CUtensorMap* bm = p.gated ? &p.b[half] : &p.b[pr];
+              const int y = p.gated ? nt * 128 : nt * kBN + half * 128;
+              tma_2d<CG>(st + kATile + h * kBHalf, bm, x, y, bar);
+            }
           }
         }
       }
@@ -341,8 +418,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     }
   } else if (warp == kMmaWarp) {
     if (lane == 0 && rank == 0) {
-      const uint32_t idesc = (1u << 4) | (TYPE == kBf16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(kBN >> 3) << 17) |
-                             ((uint32_t)(CG * kBM >> 4) << 24);
+      const uint32_t idesc = (1u << 4) | (TYPE == kBf16 ? (1u << 7) | (1u << 10) : 0u) | (BN_MAJOR ? 1u << 16 : 0u) |
+                             ((uint32_t)(kBN >> 3) << 17) | ((uint32_t)(CG * kBM >> 4) << 24);
       int it = 0, tile = 0;
       bool ok = true;
       for (int64_t unit = first; ok && unit < p.units; unit += stride, ++tile) {
@@ -366,10 +443,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
           }
           tc_after();
           const uint64_t ad = sw128_desc(sbase + s * C::kStageBytes);
-          const uint64_t bd = sw128_desc(sbase + s * C::kStageBytes + kATile);
+          const uint32_t bs = sbase + s * C::kStageBytes + kATile;
+          const uint64_t bd = BN_MAJOR ? sw128_mn_desc(bs) : sw128_desc(bs);
+          constexpr int kBStep = BN_MAJOR ? (16 * 128) >> 4 : 32 >> 4;  // 16 rows, or 32 bytes of each row
 #pragma unroll
           for (int j = 0; j < kBK / 16; ++j)
-            tc_mma<CG>(tmem + buf * kBN, ad + 2 * j, bd + 2 * j, idesc, (k > k0 || j > 0) ? 1u : 0u);
+            tc_mma<CG>(tmem + buf * kBN, ad + 2 * j, bd + kBStep * j, idesc, (k > k0 || j > 0) ? 1u : 0u);
           tc_commit<CG>(bar_empty + 8 * s);
         }
         tc_commit<CG>(bar_accf + 8 * buf);
@@ -380,6 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     const int quad = warp & 3, half = warp >> 2;
     const bool vec = ((p.N | p.e.ldo) & 7) == 0;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    const uint32_t stage = sbase + C::kStaging + warp * kStage2K;
     int tile = 0;
     for (int64_t unit = first; unit < p.units; unit += stride, ++tile) {
       int mt, sp, nt;
@@ -407,38 +487,77 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             for (int i = 0; i < 8; ++i) dst[i] = make_float4(d[4 * i], d[4 * i + 1], d[4 * i + 2], d[4 * i + 3]);
           }
         }
-      } else if constexpr (EPI == kEpiGated) {
+      } else {
+        constexpr int kChunks = EPI == kEpiGated ? 2 : 4;  // of 32 output columns, this warp's half
+        const int64_t mrow = m - lane;  // the warp's first row
+        const int rows = p.M - mrow < 32 ? (int)(p.M - mrow) : 32;  // may be <= 0
+        const int64_t ld = p.e.ldo;
+        auto column = [&](int q) {
+          return EPI == kEpiGated ? nt * 128 + half * 64 + q * 32 : nt * kBN + half * 128 + q * 32;
+        };
+        Tile32 tg, tu;
+        auto fetch = [&](int q) {
+          const int n = column(q);
+          const int64_t at = mrow * ld + n;
+          if constexpr (EPI == kEpiGatedBackward) {
+            fetch_tile(tg, p.e.gate + at, ld, rows, p.N - n, lane);
+            fetch_tile(tu, p.e.up + at, ld, rows, p.N - n, lane);
+          } else if constexpr (EPI == kEpiPlain) {
+            if (p.e.residual) fetch_tile(tg, p.e.residual + at, ld, rows, p.N - n, lane);
+          }
+        };
+        if (vec) fetch(0);
 #pragma unroll 1
-        for (int q = 0; q < 2; ++q) {
-          const int c = half * 64 + q * 32;
+        for (int q = 0; q < kChunks; ++q) {
+          const int c = EPI == kEpiGated ? half * 64 + q * 32 : half * 128 + q * 32;
+          const int n = column(q);
           float d[32], u[32];
           tmem_ld32(acc + c, d);
-          tmem_ld32(acc + 128 + c, u);
+          if constexpr (EPI == kEpiGated) tmem_ld32(acc + 128 + c, u);
           tmem_wait_ld();
-          if (m < p.M) {
+          if (!vec) {  // rows of any length: element by element
+            if (m < p.M) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int n = nt * 128 + c + 8 * i;
-              if (n < p.N)
-                epilogue8<EPI, TYPE>(p.e, m, n, p.N, vec, *reinterpret_cast<float(*)[8]>(d + 8 * i),
-                                     *reinterpret_cast<float(*)[8]>(u + 8 * i));
+              for (int i = 0; i < 4; ++i) {
+                float(&d8)[8] = *reinterpret_cast<float(*)[8]>(d + 8 * i);
+                const float(&u8)[8] = *reinterpret_cast<float(*)[8]>((EPI == kEpiGated ? u : d) + 8 * i);
+                if (n + 8 * i < p.N) epilogue8<EPI, TYPE>(p.e, m, n + 8 * i, p.N, false, d8, u8);
+              }
             }
+            continue;
           }
-        }
-      } else {
-#pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          const int c = half * 128 + q * 32;
-          float d[32];
-          tmem_ld32(acc + c, d);
-          tmem_wait_ld();
-          if (m < p.M) {
+          const int64_t at = mrow * ld + n;
+          const int cols = p.N - n;
+          if constexpr (EPI == kEpiPlain) {
+            if (p.e.residual) {
+              turn_tile<TYPE>(stage, tg, u, lane);
+              if (q + 1 < kChunks) fetch(q + 1);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int n = nt * kBN + c + 8 * i;
-              float(&d8)[8] = *reinterpret_cast<float(*)[8]>(d + 8 * i);
-              if (n < p.N) epilogue8<EPI, TYPE>(p.e, m, n, p.N, vec, d8, d8);
+              for (int i = 0; i < 32; ++i) d[i] += u[i];
             }
+            store_tile<TYPE>(stage, d, p.e.out + at, ld, rows, cols, lane);
+          } else if constexpr (EPI == kEpiGated) {
+            if (p.e.gate) {
+              store_tile<TYPE>(stage, d, p.e.gate + at, ld, rows, cols, lane);
+              store_tile<TYPE>(stage, u, p.e.up + at, ld, rows, cols, lane);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) d[i] = act_val(d[i], p.e.act) * u[i];
+            store_tile<TYPE>(stage, d, p.e.out + at, ld, rows, cols, lane);
+          } else {
+            float g[32];
+            turn_tile<TYPE>(stage, tg, g, lane);
+            turn_tile<TYPE>(stage, tu, u, lane);
+            if (q + 1 < kChunks) fetch(q + 1);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              float val, grad;
+              act_grad(g[i], p.e.act, val, grad);
+              g[i] = d[i] * u[i] * grad;
+              d[i] *= val;
+            }
+            store_tile<TYPE>(stage, g, p.e.dgate + at, ld, rows, cols, lane);
+            store_tile<TYPE>(stage, d, p.e.dup + at, ld, rows, cols, lane);
           }
         }
       }
@@ -502,13 +621,13 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   return fn;
 }
 
-// [rows][cols] 16-bit elements, rows ld apart, boxes of 128 rows x 64 elements.
-cudaError_t encode(CUtensorMap* map, const uint16_t* ptr, int64_t rows, int cols, int64_t ld, int type) {
+// [rows][cols] 16-bit elements, rows ld apart, boxes of box_rows rows x 64 elements.
+cudaError_t encode(CUtensorMap* map, const uint16_t* ptr, int64_t rows, int cols, int64_t ld, int box_rows, int type) {
   auto enc = encoder();
   if (!enc) return cudaErrorNotSupported;
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-  const cuuint32_t box[2] = {kBK, 128};
+  const cuuint32_t box[2] = {kBK, (cuuint32_t)box_rows};
   const cuuint32_t one[2] = {1, 1};
   const CUresult r =
       enc(map, type == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
@@ -540,10 +659,10 @@ Plan plan(int64_t M, int N, int K, int pairs, bool gated) {
   return q;
 }
 
-template <int CG, int EPI, int TYPE>
+template <int CG, int EPI, int TYPE, bool BN_MAJOR>
 cudaError_t launch_t(const GemmParams& p, cudaStream_t st) {
   using C = Cfg<CG>;
-  auto kern = gemm_kernel<CG, EPI, TYPE>;
+  auto kern = gemm_kernel<CG, EPI, TYPE, BN_MAJOR>;
   cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (err != cudaSuccess) return err;
   const int64_t most = kSms / CG;
@@ -574,10 +693,10 @@ cudaError_t launch_t(const GemmParams& p, cudaStream_t st) {
 }
 
 template <int CG, int TYPE>
-cudaError_t launch_e(const GemmParams& p, int epi, cudaStream_t st) {
-  if (epi == kEpiGated) return launch_t<CG, kEpiGated, TYPE>(p, st);
-  if (epi == kEpiGatedBackward) return launch_t<CG, kEpiGatedBackward, TYPE>(p, st);
-  return launch_t<CG, kEpiPlain, TYPE>(p, st);
+cudaError_t launch_e(const GemmParams& p, int epi, bool n_major, cudaStream_t st) {
+  if (epi == kEpiGated) return launch_t<CG, kEpiGated, TYPE, false>(p, st);
+  if (epi == kEpiGatedBackward) return launch_t<CG, kEpiGatedBackward, TYPE, true>(p, st);
+  return n_major ? launch_t<CG, kEpiPlain, TYPE, true>(p, st) : launch_t<CG, kEpiPlain, TYPE, false>(p, st);
 }
 
 }  // namespace
@@ -589,6 +708,7 @@ size_t dense_partial_bytes(int64_t M, int N, int K, int pairs, bool gated) {
 
 cudaError_t launch_dense_gemm(const DenseGemm& g, cudaStream_t st) {
   const bool gated = g.epilogue == kEpiGated;
+  if (g.b_rows_k ? gated : g.epilogue == kEpiGatedBackward) return cudaErrorInvalidValue;
   const Plan q = plan(g.M, g.N, g.K, g.pairs, gated);
   GemmParams p;
   p.M = g.M;
@@ -607,12 +727,14 @@ cudaError_t launch_dense_gemm(const DenseGemm& g, cudaStream_t st) {
     return cudaErrorInvalidValue;
   for (int i = 0; i < 2; ++i) {
     const int ai = g.pairs > 1 ? i : 0, bi = (g.pairs > 1 || gated) ? i : 0;
-    cudaError_t err = encode(&p.a[i], g.a[ai], g.M, g.K, g.lda[ai], g.type);
-    if (err == cudaSuccess) err = encode(&p.b[i], g.b[bi], g.N, g.K, g.ldb[bi], g.type);
+    cudaError_t err = encode(&p.a[i], g.a[ai], g.M, g.K, g.lda[ai], kBM, g.type);
+    if (err == cudaSuccess)
+      err = g.b_rows_k ? encode(&p.b[i], g.b[bi], g.K, g.N, g.ldb[bi], kBK, g.type)
+                       : encode(&p.b[i], g.b[bi], g.N, g.K, g.ldb[bi], 128, g.type);
     if (err != cudaSuccess) return err;
   }
-  if (g.type == kF16) return q.cg == 2 ? launch_e<2, kF16>(p, g.epilogue, st) : launch_e<1, kF16>(p, g.epilogue, st);
-  return q.cg == 2 ? launch_e<2, kBf16>(p, g.epilogue, st) : launch_e<1, kBf16>(p, g.epilogue, st);
+  if (g.type == kF16) return q.cg == 2 ? launch_e<2, kF16>(p, g.epilogue, g.b_rows_k, st) : launch_e<1, kF16>(p, g.epilogue, g.b_rows_k, st);
+  return q.cg == 2 ? launch_e<2, kBf16>(p, g.epilogue, g.b_rows_k, st) : launch_e<1, kBf16>(p, g.epilogue, g.b_rows_k, st);
 }
 
 cudaError_t dense_status(int32_t* status, cudaStream_t st) {

@@ -25,29 +25,6 @@ namespace moe {
 namespace {
 
 template <int TYPE>
-struct Nib;  // two fields of a word as 16 + q, and ones
-template <>
-struct Nib<kBf16> {
-  static constexpr uint32_t kMask = 0x00780078u, kBase = 0x41804180u, kOne = 0x3f803f80u;
-  static constexpr int kBit = 3;  // lowest mantissa bit of the field
-};
-template <>
-struct Nib<kF16> {
-  static constexpr uint32_t kMask = 0x03c003c0u, kBase = 0x4c004c00u, kOne = 0x3c003c00u;
-  static constexpr int kBit = 6;
-};
-
-// fields j and j + 4 of w
-template <int TYPE, int J>
-MOE_DEV uint32_t fields(uint32_t w) {
-  constexpr int sh = Nib<TYPE>::kBit - 4 * J;
-  const uint32_t v = sh >= 0 ? w << (sh >= 0 ? sh : 0) : w >> (sh >= 0 ? 0 : -sh);
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;\n" : "=r"(r) : "r"(v), "n"(Nib<TYPE>::kMask), "n"(Nib<TYPE>::kBase));
-  return r;
-}
-
-template <int TYPE>
 MOE_DEV void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (TYPE == kBf16)
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"

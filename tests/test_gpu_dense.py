@@ -287,6 +287,7 @@ def test_c_entry_refusals_launch_nothing():
     assert q(ctx.handle, 0, p, 200, 64, p, p, p, 64, 1, 32, 4, p, p, need.value - 1) == 1
     assert b"workspace" in lib.moe_last_error(ctx.handle)
     assert q(ctx.handle, 0, p, 200, 64, p, p, p, 64, 1, 32, 4, p, None, 0) == 1
+    assert q(ctx.handle, 0, p, 200, 64, p, p, p, 64, 1, 32, 4, p, p + 16, need.value) == 1
     assert q(ctx.handle, 0, p + 2, 1, 64, p, p, p, 64, 1, 32, 4, p, p, 1 << 16) == 1
     assert q(ctx.handle, 0, p, 1, 64, p, p + 2, p, 64, 1, 32, 4, p, p, 1 << 16) == 1
     assert q(ctx.handle, 0, p, 1, 64, None, p, p, 64, 1, 32, 4, p, p, 1 << 16) == 1
