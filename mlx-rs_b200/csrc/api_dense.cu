@@ -53,18 +53,6 @@ struct DeviceGuard {
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 int64_t up8(int64_t v) { return (v + 7) & ~int64_t(7); }
 
-struct Carve {
-  char* base;
-  size_t off = 0;
-  template <class T>
-  T* take(size_t count) {
-    off = (off + 255) & ~size_t(255);
-    T* p = reinterpret_cast<T*>(base ? base + off : nullptr);
-    off += count * sizeof(T);
-    return p;
-  }
-};
-
 int check_format(moe_ctx* ctx, const char* fn, int dtype, int group_size, int bits) {
   if (!(bits == 2 || bits == 3 || bits == 4 || bits == 5 || bits == 6 || bits == 8))
     return fail(ctx, MOE_ERR_INVALID, "%s: bits=%d is not a valid MLX affine width", fn, bits);
@@ -88,34 +76,29 @@ moe::PackedMatrix packed(const moe_qweight& q, int64_t rows, int64_t cols) {
   return {q.w, static_cast<const uint16_t*>(q.scales), static_cast<const uint16_t*>(q.biases), rows, (int)cols};
 }
 
-// ---- 4-bit matrix product. Weight rows are dequantised in pieces of at most this many
-// elements (64 MB of 16-bit values, which stay in the 126 MB L2 for the product).
-constexpr int64_t kPieceElems = int64_t(32) << 20;
+// ---- workspaces, in 256-byte steps
+size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 
-// Output columns per piece.
+// Output columns per piece of a product over 16-bit weights: at most 32 M weights at a time
+// (64 MB, which stay in the 126 MB L2 between the dequantisation and the product).
 int64_t qmm_piece(int64_t N, int64_t K) {
-  const int64_t n = std::max<int64_t>(256, kPieceElems / up8(K) / 256 * 256);
-  return std::min(N, n);
+  const int64_t n = (int64_t(32) << 20) / K / 256 * 256;
+  return std::min(N, std::max<int64_t>(256, n));
 }
-
+// The 4-bit matrix product: a copy of x with rows of 16-byte pitch when K is no multiple of 8
+// (possible in the direction that sums over the weights' rows); for many tokens one piece of
+// 16-bit weights. A piece of weight columns would not be contiguous, so that direction takes
+// 16-bit weights only where one piece holds them all.
 struct QmmWs {
-  uint16_t* w;      // 16-bit weights: [piece][K], or [K][piece] when !transpose
-  uint16_t* xpad;   // [M][K rounded up to 8] when K is no multiple of 8
-  float* partial;
-  size_t partial_bytes, bytes;
+  bool wide;
+  size_t xpad, total;
 };
-QmmWs carve_qmm(void* base, int64_t M, int64_t N, int64_t K, int transpose) {
-  Carve cv{static_cast<char*>(base)};
+QmmWs qmm_workspace(int64_t M, int64_t N, int64_t K, int transpose) {
   QmmWs w{};
-  if (transpose && M <= moe::kQmvMaxM) return w;  // straight from the packed weights
+  w.xpad = K % 8 ? up256((size_t)M * up8(K) * sizeof(uint16_t)) : 0;
   const int64_t piece = qmm_piece(N, K);
-  w.w = cv.take<uint16_t>(piece * up8(K));
-  if (K % 8) w.xpad = cv.take<uint16_t>(M * up8(K));
-  // the last piece may split where the full ones do not
-  w.partial_bytes = moe::dense_partial_bytes(M, (int)piece, (int)K, 1, false);
-  if (N % piece) w.partial_bytes = std::max(w.partial_bytes, moe::dense_partial_bytes(M, (int)(N % piece), (int)K, 1, false));
-  w.partial = w.partial_bytes ? cv.take<float>(w.partial_bytes / sizeof(float)) : nullptr;
-  w.bytes = cv.off;
+  w.wide = M >= moe::kWideMinM && (transpose || piece == N);
+  w.total = w.xpad + (w.wide ? (size_t)piece * K * sizeof(uint16_t) : 0);
   return w;
 }
 
@@ -154,35 +137,40 @@ int check_ffn_weights(moe_ctx* ctx, const char* fn, const moe_ffn_weights* w) {
   return rc;
 }
 
+// The forward pass keeps h [T][I] between its two products; for many tokens both passes keep
+// the three matrices in 16 bits.
 struct FfnWs {
-  uint16_t *wg, *wu, *wd;  // 16-bit weights
-  uint16_t* h;             // [T][I] (forward)
-  float* partial;
-  size_t partial_bytes, bytes;
+  bool wide;
+  size_t h, each, total;  // bytes of h, of one matrix, of all
 };
-FfnWs carve_ffn(void* base, const moe_ffn_config* c, int64_t T, bool backward) {
-  Carve cv{static_cast<char*>(base)};
+FfnWs ffn_workspace(const moe_ffn_config* c, int64_t T, bool backward) {
   FfnWs w{};
-  const size_t n = (size_t)c->hidden * c->inter;
-  const int H = c->hidden, I = c->inter;
-  if (!backward && T <= moe::kQmvMaxM) {  // straight from the packed weights
-    w.h = cv.take<uint16_t>((size_t)T * I);
-    w.bytes = cv.off;
-    return w;
-  }
-  w.wg = cv.take<uint16_t>(n);
-  w.wu = cv.take<uint16_t>(n);
-  w.wd = cv.take<uint16_t>(n);
-  if (!backward) {
-    w.h = cv.take<uint16_t>((size_t)T * I);
-    w.partial_bytes = std::max(moe::dense_partial_bytes(T, I, H, 1, true), moe::dense_partial_bytes(T, H, I, 1, false));
-  } else {
-    w.partial_bytes =
-        std::max(moe::dense_partial_bytes(T, I, H, 1, false), moe::dense_partial_bytes(T, H, I, 2, false));
-  }
-  w.partial = w.partial_bytes ? cv.take<float>(w.partial_bytes / sizeof(float)) : nullptr;
-  w.bytes = cv.off;
+  w.wide = T >= moe::kWideMinM;
+  w.h = backward ? 0 : up256((size_t)T * c->inter * sizeof(uint16_t));
+  w.each = w.wide ? up256((size_t)c->hidden * c->inter * sizeof(uint16_t)) : 0;
+  w.total = w.h + 3 * w.each;
   return w;
+}
+
+// The three matrices in 16 bits, behind h in the workspace.
+struct Wide {
+  uint16_t *gate = nullptr, *up = nullptr, *down = nullptr;
+};
+cudaError_t widen(const moe_ffn_config* c, const moe_ffn_weights* w, const FfnWs& ws, void* workspace, Wide& out,
+                  cudaStream_t st) {
+  if (!ws.wide) return cudaSuccess;
+  char* base = static_cast<char*>(workspace) + ws.h;
+  out.gate = reinterpret_cast<uint16_t*>(base);
+  out.up = reinterpret_cast<uint16_t*>(base + ws.each);
+  out.down = reinterpret_cast<uint16_t*>(base + 2 * ws.each);
+  moe::DequantArgs da{};
+  da.jobs = 3;
+  da.group = c->group_size;
+  da.type = c->dtype;
+  da.job[0] = {packed(w->gate, c->inter, c->hidden), out.gate};
+  da.job[1] = {packed(w->up, c->inter, c->hidden), out.up};
+  da.job[2] = {packed(w->down, c->hidden, c->inter), out.down};
+  return moe::launch_dequant(da, st);
 }
 
 int check_workspace(moe_ctx* ctx, const char* fn, const void* ws, size_t have, size_t need) {
@@ -205,7 +193,7 @@ int moe_quantized_matmul_workspace(int dtype, int64_t M, int64_t K, int64_t N, i
   int rc = check_format(nullptr, "", dtype, group_size, bits);
   if (!rc) rc = check_qmm_sizes(nullptr, "", M, K, N, transpose, group_size);
   if (rc || M == 0) return rc;
-  *bytes = carve_qmm(nullptr, M, N, K, transpose).bytes;
+  *bytes = qmm_workspace(M, N, K, transpose).total;
   return MOE_OK;
 }
 
@@ -223,10 +211,9 @@ int moe_quantized_matmul_ex(moe_ctx* ctx, int dtype, const void* x, int64_t M, i
   rc = check_weight(ctx, fn, "w", q);
   if (rc) return rc;
   if (!aligned16(x) || !aligned16(out)) return fail(ctx, MOE_ERR_INVALID, "%s: x and out must be 16-byte aligned", fn);
-  const QmmWs need = carve_qmm(nullptr, M, N, K, transpose);
-  rc = check_workspace(ctx, fn, workspace, workspace_bytes, need.bytes);
+  const QmmWs ws = qmm_workspace(M, N, K, transpose);
+  rc = check_workspace(ctx, fn, workspace, workspace_bytes, ws.total);
   if (rc) return rc;
-  const QmmWs ws = carve_qmm(workspace, M, N, K, transpose);
   DeviceGuard g(moe_internal::ctx_device(ctx));
   if (!g.ok) return fail(ctx, MOE_ERR_CUDA, "%s: cudaSetDevice failed", fn);
   const cudaStream_t st = static_cast<cudaStream_t>(moe_internal::ctx_stream(ctx));
@@ -244,52 +231,47 @@ int moe_quantized_matmul_ex(moe_ctx* ctx, int dtype, const void* x, int64_t M, i
     DENSE_CUDA(ctx, fn, moe::launch_qmv(a, false, st));
     return MOE_OK;
   }
-  const int64_t ldx = up8(K);
-  const uint16_t* xs = static_cast<const uint16_t*>(x);
-  if (ws.xpad) {
-    DENSE_CUDA(ctx, fn, moe::launch_pad_rows(xs, M, K, ws.xpad, ldx, st));
-    xs = ws.xpad;
+  moe::DenseGemm gm{};
+  gm.a[0] = static_cast<const uint16_t*>(x);
+  gm.lda = up8(K);
+  if (gm.lda != K) {
+    uint16_t* padded = static_cast<uint16_t*>(workspace);
+    DENSE_CUDA(ctx, fn, moe::launch_pad_rows(gm.a[0], M, K, padded, gm.lda, st));
+    gm.a[0] = padded;
   }
+  gm.w[0] = packed(q, transpose ? N : K, transpose ? K : N);
+  gm.pairs = 1;
+  gm.rows_k = !transpose;
+  gm.M = M;
+  gm.N = (int)N;
+  gm.K = (int)K;
+  gm.group = group_size;
+  gm.type = dtype;
+  gm.epilogue = moe::kEpiPlain;
+  gm.e.out = static_cast<uint16_t*>(out);
+  gm.e.ldo = N;
+  if (!ws.wide) {
+    DENSE_CUDA(ctx, fn, moe::launch_dense_gemm(gm, st));
+    return MOE_OK;
+  }
+  uint16_t* w16 = reinterpret_cast<uint16_t*>(static_cast<char*>(workspace) + ws.xpad);
   const int64_t piece = qmm_piece(N, K);
   for (int64_t n0 = 0; n0 < N; n0 += piece) {
-    const int64_t n = std::min(piece, N - n0);
     moe::DequantArgs da{};
     da.jobs = 1;
     da.group = group_size;
     da.type = dtype;
-    const int64_t inner = transpose ? K : N;
-    moe::PackedMatrix m = packed(q, transpose ? n : K, inner);
-    m.w_pitch = (int)(inner / 8);
-    m.s_pitch = (int)(inner / group_size);
-    if (transpose) {
+    moe::PackedMatrix m = gm.w[0];
+    if (transpose) {  // rows n0.. of the weights
+      m.rows = gm.N = (int)std::min(piece, N - n0);
       m.w += n0 * (K / 8);
       m.s += n0 * (K / group_size);
       if (m.b) m.b += n0 * (K / group_size);
-    } else {
-      // a piece of columns: whole words and groups (the piece is a multiple of 256)
-      m.w += n0 / 8;
-      m.s += n0 / group_size;
-      if (m.b) m.b += n0 / group_size;
-      m.cols = (int)n;
     }
-    da.job[0] = {m, ws.w, transpose ? ldx : piece};
+    da.job[0] = {m, w16};
     DENSE_CUDA(ctx, fn, moe::launch_dequant(da, st));
-    moe::DenseGemm gm{};
-    gm.a[0] = xs;
-    gm.b[0] = ws.w;
-    gm.lda[0] = ldx;
-    gm.ldb[0] = transpose ? ldx : piece;
-    gm.b_rows_k = !transpose;
-    gm.pairs = 1;
-    gm.M = M;
-    gm.N = (int)n;
-    gm.K = (int)K;
-    gm.type = dtype;
-    gm.epilogue = moe::kEpiPlain;
+    gm.wide[0] = w16;
     gm.e.out = static_cast<uint16_t*>(out) + n0;
-    gm.e.ldo = N;
-    gm.partial = ws.partial;
-    gm.partial_bytes = ws.partial_bytes;
     DENSE_CUDA(ctx, fn, moe::launch_dense_gemm(gm, st));
   }
   return MOE_OK;
@@ -300,7 +282,7 @@ int moe_gated_ffn_workspace(const moe_ffn_config* cfg, int64_t T, int backward, 
   *bytes = 0;
   int rc = check_ffn(nullptr, "", cfg, T);
   if (rc || T == 0) return rc;
-  *bytes = carve_ffn(nullptr, cfg, T, backward != 0).bytes;
+  *bytes = ffn_workspace(cfg, T, backward != 0).total;
   return MOE_OK;
 }
 
@@ -317,10 +299,10 @@ int moe_gated_ffn_forward(moe_ctx* ctx, const moe_ffn_config* cfg, const moe_ffn
   if (!gate != !up) return fail(ctx, MOE_ERR_INVALID, "%s: gate and up are saved together or not at all", fn);
   for (const void* p : {x, residual, (const void*)gate, (const void*)up, (const void*)out})
     if (!aligned16(p)) return fail(ctx, MOE_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
-  const FfnWs need = carve_ffn(nullptr, cfg, T, false);
-  rc = check_workspace(ctx, fn, workspace, workspace_bytes, need.bytes);
+  const FfnWs ws = ffn_workspace(cfg, T, false);
+  rc = check_workspace(ctx, fn, workspace, workspace_bytes, ws.total);
   if (rc) return rc;
-  const FfnWs ws = carve_ffn(workspace, cfg, T, false);
+  uint16_t* h = static_cast<uint16_t*>(workspace);
   DeviceGuard g(moe_internal::ctx_device(ctx));
   if (!g.ok) return fail(ctx, MOE_ERR_CUDA, "%s: cudaSetDevice failed", fn);
   const cudaStream_t st = static_cast<cudaStream_t>(moe_internal::ctx_stream(ctx));
@@ -336,13 +318,13 @@ int moe_gated_ffn_forward(moe_ctx* ctx, const moe_ffn_config* cfg, const moe_ffn
     a.K = H;
     a.group = cfg->group_size;
     a.type = cfg->dtype;
-    a.out = ws.h;
+    a.out = h;
     a.gate = static_cast<uint16_t*>(gate);
     a.up = static_cast<uint16_t*>(up);
     a.act = cfg->activation;
     DENSE_CUDA(ctx, fn, moe::launch_qmv(a, true, st));
     moe::QmvArgs d{};
-    d.x = ws.h;
+    d.x = h;
     d.m[0] = packed(wts->down, H, I);
     d.M = (int)T;
     d.N = H;
@@ -355,51 +337,45 @@ int moe_gated_ffn_forward(moe_ctx* ctx, const moe_ffn_config* cfg, const moe_ffn
     DENSE_CUDA(ctx, fn, moe::launch_qmv(d, false, st));
     return MOE_OK;
   }
-  moe::DequantArgs da{};
-  da.jobs = 3;
-  da.group = cfg->group_size;
-  da.type = cfg->dtype;
-  da.job[0] = {packed(wts->gate, I, H), ws.wg, H};
-  da.job[1] = {packed(wts->up, I, H), ws.wu, H};
-  da.job[2] = {packed(wts->down, H, I), ws.wd, I};
-  for (auto& j : da.job) j.m.w_pitch = j.m.cols / 8, j.m.s_pitch = j.m.cols / cfg->group_size;
-  DENSE_CUDA(ctx, fn, moe::launch_dequant(da, st));
-
+  Wide wide;
+  DENSE_CUDA(ctx, fn, widen(cfg, wts, ws, workspace, wide, st));
   moe::DenseGemm gu{};
   gu.a[0] = static_cast<const uint16_t*>(x);
-  gu.b[0] = ws.wg;
-  gu.b[1] = ws.wu;
-  gu.lda[0] = gu.ldb[0] = gu.ldb[1] = H;
+  gu.w[0] = packed(wts->gate, I, H);
+  gu.w[1] = packed(wts->up, I, H);
+  gu.wide[0] = wide.gate;
+  gu.wide[1] = wide.up;
+  gu.lda = H;
   gu.pairs = 1;
   gu.M = T;
   gu.N = I;
   gu.K = H;
+  gu.group = cfg->group_size;
   gu.type = cfg->dtype;
   gu.epilogue = moe::kEpiGated;
-  gu.e.out = ws.h;
+  gu.e.out = h;
   gu.e.ldo = I;
   gu.e.gate = static_cast<uint16_t*>(gate);
   gu.e.up = static_cast<uint16_t*>(up);
   gu.e.act = cfg->activation;
-  gu.partial = ws.partial;
-  gu.partial_bytes = ws.partial_bytes;
   DENSE_CUDA(ctx, fn, moe::launch_dense_gemm(gu, st));
 
   moe::DenseGemm dn{};
-  dn.a[0] = ws.h;
-  dn.b[0] = ws.wd;
-  dn.lda[0] = dn.ldb[0] = I;
+  dn.a[0] = h;
+  dn.w[0] = packed(wts->down, H, I);
+  dn.wide[0] = wide.down;
+  dn.lda = I;
   dn.pairs = 1;
   dn.M = T;
   dn.N = H;
   dn.K = I;
+  dn.group = cfg->group_size;
   dn.type = cfg->dtype;
+  dn.early = 1;
   dn.epilogue = moe::kEpiPlain;
   dn.e.out = static_cast<uint16_t*>(out);
   dn.e.ldo = H;
   dn.e.residual = static_cast<const uint16_t*>(residual);
-  dn.partial = ws.partial;
-  dn.partial_bytes = ws.partial_bytes;
   DENSE_CUDA(ctx, fn, moe::launch_dense_gemm(dn, st));
   return MOE_OK;
 }
@@ -417,36 +393,28 @@ int moe_gated_ffn_backward(moe_ctx* ctx, const moe_ffn_config* cfg, const moe_ff
     if (!p) return fail(ctx, MOE_ERR_INVALID, "%s: null pointer", fn);
     if (!aligned16(p)) return fail(ctx, MOE_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
   }
-  const FfnWs need = carve_ffn(nullptr, cfg, T, true);
-  rc = check_workspace(ctx, fn, workspace, workspace_bytes, need.bytes);
+  const FfnWs ws = ffn_workspace(cfg, T, true);
+  rc = check_workspace(ctx, fn, workspace, workspace_bytes, ws.total);
   if (rc) return rc;
-  const FfnWs ws = carve_ffn(workspace, cfg, T, true);
   DeviceGuard g(moe_internal::ctx_device(ctx));
   if (!g.ok) return fail(ctx, MOE_ERR_CUDA, "%s: cudaSetDevice failed", fn);
   const cudaStream_t st = static_cast<cudaStream_t>(moe_internal::ctx_stream(ctx));
   const int H = cfg->hidden, I = cfg->inter;
 
-  // the products below sum over the weights' rows
-  moe::DequantArgs da{};
-  da.jobs = 3;
-  da.group = cfg->group_size;
-  da.type = cfg->dtype;
-  da.job[0] = {packed(wts->gate, I, H), ws.wg, H};
-  da.job[1] = {packed(wts->up, I, H), ws.wu, H};
-  da.job[2] = {packed(wts->down, H, I), ws.wd, I};
-  for (auto& j : da.job) j.m.w_pitch = j.m.cols / 8, j.m.s_pitch = j.m.cols / cfg->group_size;
-  DENSE_CUDA(ctx, fn, moe::launch_dequant(da, st));
-
+  Wide wide;
+  DENSE_CUDA(ctx, fn, widen(cfg, wts, ws, workspace, wide, st));
+  // both products sum over the weights' rows
   moe::DenseGemm dh{};
   dh.a[0] = static_cast<const uint16_t*>(dy);
-  dh.b[0] = ws.wd;
-  dh.lda[0] = H;
-  dh.ldb[0] = I;
-  dh.b_rows_k = 1;
+  dh.w[0] = packed(wts->down, H, I);
+  dh.wide[0] = wide.down;
+  dh.lda = H;
   dh.pairs = 1;
+  dh.rows_k = 1;
   dh.M = T;
   dh.N = I;
   dh.K = H;
+  dh.group = cfg->group_size;
   dh.type = cfg->dtype;
   dh.epilogue = moe::kEpiGatedBackward;
   dh.e.ldo = I;
@@ -455,29 +423,28 @@ int moe_gated_ffn_backward(moe_ctx* ctx, const moe_ffn_config* cfg, const moe_ff
   dh.e.dgate = static_cast<uint16_t*>(dgate);
   dh.e.dup = static_cast<uint16_t*>(dup);
   dh.e.act = cfg->activation;
-  dh.partial = ws.partial;
-  dh.partial_bytes = ws.partial_bytes;
   DENSE_CUDA(ctx, fn, moe::launch_dense_gemm(dh, st));
 
-  moe::DenseGemm dxg{};
-  dxg.a[0] = static_cast<const uint16_t*>(dgate);
-  dxg.a[1] = static_cast<const uint16_t*>(dup);
-  dxg.b[0] = ws.wg;
-  dxg.b[1] = ws.wu;
-  dxg.lda[0] = dxg.lda[1] = I;
-  dxg.ldb[0] = dxg.ldb[1] = H;
-  dxg.b_rows_k = 1;
-  dxg.pairs = 2;
-  dxg.M = T;
-  dxg.N = H;
-  dxg.K = I;
-  dxg.type = cfg->dtype;
-  dxg.epilogue = moe::kEpiPlain;
-  dxg.e.out = static_cast<uint16_t*>(dx);
-  dxg.e.ldo = H;
-  dxg.partial = ws.partial;
-  dxg.partial_bytes = ws.partial_bytes;
-  DENSE_CUDA(ctx, fn, moe::launch_dense_gemm(dxg, st));
+  moe::DenseGemm in{};  // dx = dgate . gate + dup . up: one sum over both
+  in.a[0] = static_cast<const uint16_t*>(dgate);
+  in.a[1] = static_cast<const uint16_t*>(dup);
+  in.w[0] = packed(wts->gate, I, H);
+  in.w[1] = packed(wts->up, I, H);
+  in.wide[0] = wide.gate;
+  in.wide[1] = wide.up;
+  in.lda = I;
+  in.pairs = 2;
+  in.rows_k = 1;
+  in.M = T;
+  in.N = H;
+  in.K = I;
+  in.group = cfg->group_size;
+  in.type = cfg->dtype;
+  in.early = 1;
+  in.epilogue = moe::kEpiPlain;
+  in.e.out = static_cast<uint16_t*>(dx);
+  in.e.ldo = H;
+  DENSE_CUDA(ctx, fn, moe::launch_dense_gemm(in, st));
   return MOE_OK;
 }
 

@@ -21,14 +21,12 @@ struct PackedMatrix {
   const uint16_t* b;  // may be null
   int64_t rows;
   int cols;
-  int w_pitch, s_pitch;  // words and scales from one row to the next (cols may be a part)
 };
 
-// ---- dequantisation into 16-bit rows (dense_dequant.cu)
+// ---- 4-bit weights to 16-bit rows [rows][cols], 32-byte aligned (dense_dequant.cu)
 struct DequantJob {
   PackedMatrix m;
-  uint16_t* out;   // [rows][ld], 32-byte aligned rows
-  int64_t ld;
+  uint16_t* out;
 };
 struct DequantArgs {
   DequantJob job[3];
@@ -38,10 +36,15 @@ struct DequantArgs {
   uint32_t rows_cta;  // set by launch_dequant
 };
 cudaError_t launch_dequant(const DequantArgs& a, cudaStream_t st);
-// out[r][0..cols) = x[r][0..cols), rows ld elements apart, the rest of each row zero.
+// Tokens from which the products take weights dequantised once by launch_dequant; below, the
+// product's own warps dequantise each tile (twice at 512 tokens, 16 times at 4096).
+constexpr int64_t kWideMinM = 1024;
+
+// out[r][0..cols) = x[r][0..cols), rows ld elements apart, the rest of each row zero
+// (dense_pad.cu).
 cudaError_t launch_pad_rows(const uint16_t* x, int64_t rows, int64_t cols, uint16_t* out, int64_t ld, cudaStream_t st);
 
-// ---- 16-bit matrix product with fused epilogues (dense_gemm.cu)
+// ---- 4-bit matrix product on tcgen05 with fused epilogues (dense_gemm.cu)
 enum DenseEpilogue { kEpiPlain = 0, kEpiGated = 1, kEpiGatedBackward = 2 };
 struct DenseEpi {
   int64_t ldo;               // row pitch of every tensor below
@@ -54,23 +57,21 @@ struct DenseEpi {
   int act;                   // 0 SiLU, 1 GELU (tanh form)
 };
 struct DenseGemm {
-  // D[M, N] = sum over the operand pairs p of A_p[M, K_p] . B_p[N, K_p]^T (one or two
-  // pairs), or . B_p[K_p, N] with b_rows_k; in the gated form one A and two B:
-  // g = A . B_0^T, u = A . B_1^T.
+  // D[M, N] = sum over the operand pairs p of A_p[M, K] . W_p[N, K]^T (one or two pairs), or
+  // . W_p[K, N] with rows_k; in the gated form one A and two W: g = A . W_0^T, u = A . W_1^T.
   const uint16_t* a[2];
-  const uint16_t* b[2];
-  int64_t lda[2], ldb[2];
+  int64_t lda;   // elements, a multiple of 8
+  PackedMatrix w[2];
+  const uint16_t* wide[2];  // the same weights in 16 bits (M > 128), or null
   int pairs;
-  int b_rows_k;
+  int rows_k;
   int64_t M;
   int N, K;
-  int type;      // kBf16 / kF16
-  int epilogue;  // DenseEpilogue
+  int group, type;  // type: kBf16 / kF16
+  int early;        // the weights may be read before the launch before has completed
+  int epilogue;     // DenseEpilogue
   DenseEpi e;
-  float* partial;        // split-K partial sums (dense_partial_bytes), or null: never split
-  size_t partial_bytes;
 };
-size_t dense_partial_bytes(int64_t M, int N, int K, int pairs, bool gated);
 cudaError_t launch_dense_gemm(const DenseGemm& g, cudaStream_t st);
 // Device status word of the dense kernels on the current device (bounded waits).
 cudaError_t dense_status(int32_t* status, cudaStream_t st);

@@ -20,13 +20,14 @@ __global__ void __launch_bounds__(256) dequant_kernel(const __grid_constant__ De
   const DequantJob& j = a.job[blockIdx.y];
   const uint32_t ppr = (uint32_t)j.m.cols >> 4, ppg = (uint32_t)a.group >> 4;  // pairs per row, per group
   const uint32_t rows_cta = a.rows_cta;
+  const uint32_t wpr = (uint32_t)j.m.cols >> 3, gpr = (uint32_t)(j.m.cols / a.group);
   const int64_t row0 = (int64_t)blockIdx.x * rows_cta;
   if (row0 >= j.m.rows) return;
   const uint32_t rows = (uint32_t)(j.m.rows - row0 < rows_cta ? j.m.rows - row0 : rows_cta);
-  const uint32_t* w = j.m.w + row0 * j.m.w_pitch;
-  const uint16_t* s = j.m.s + row0 * j.m.s_pitch;
-  const uint16_t* b = j.m.b ? j.m.b + row0 * j.m.s_pitch : nullptr;
-  uint16_t* out = j.out + row0 * j.ld;
+  const uint32_t* w = j.m.w + row0 * wpr;
+  const uint16_t* s = j.m.s + row0 * gpr;
+  const uint16_t* b = j.m.b ? j.m.b + row0 * gpr : nullptr;
+  uint16_t* out = j.out + row0 * j.m.cols;
   uint32_t r = threadIdx.x / ppr, c = threadIdx.x - r * ppr;
   const uint32_t dr = 256 / ppr, dc = 256 - dr * ppr;
   pdl_wait();
@@ -38,8 +39,8 @@ __global__ void __launch_bounds__(256) dequant_kernel(const __grid_constant__ De
     for (int i = 0; i < kSteps; ++i) {
       rr[i] = r, cc[i] = c;
       if (r < rows) {
-        q[i] = __ldg(reinterpret_cast<const uint2*>(w + (size_t)r * j.m.w_pitch) + c);
-        const size_t g = (size_t)r * j.m.s_pitch + c / ppg;
+        q[i] = __ldg(reinterpret_cast<const uint2*>(w + (size_t)r * wpr) + c);
+        const size_t g = (size_t)r * gpr + c / ppg;
         sc[i] = __ldg(s + g);
         bi[i] = b ? __ldg(b + g) : 0u;
       }
@@ -51,21 +52,12 @@ __global__ void __launch_bounds__(256) dequant_kernel(const __grid_constant__ De
       if (rr[i] >= rows) break;
       const uint32_t s2 = __byte_perm(sc[i], 0, 0x1010), b2 = __byte_perm(bi[i], 0, 0x1010);
       const uint4 lo = dequant8<TYPE>(q[i].x, s2, b2), hi = dequant8<TYPE>(q[i].y, s2, b2);
-      uint16_t* o = out + (size_t)rr[i] * j.ld + cc[i] * 16;
+      uint16_t* o = out + (size_t)rr[i] * j.m.cols + cc[i] * 16;
       asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"l"(o), "r"(lo.x), "r"(lo.y), "r"(lo.z),
                    "r"(lo.w), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w)
                    : "memory");
     }
   }
-}
-
-__global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* __restrict__ x, int64_t rows, int64_t cols,
-                                                       uint16_t* __restrict__ out, int64_t ld) {
-  pdl_wait();
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * ld) return;
-  const int64_t r = i / ld, c = i - r * ld;
-  out[i] = c < cols ? x[r * cols + c] : (uint16_t)0;
 }
 
 }  // namespace
@@ -84,10 +76,6 @@ cudaError_t launch_dequant(const DequantArgs& args, cudaStream_t st) {
   const dim3 grid((unsigned)((rows + a.rows_cta - 1) / a.rows_cta), a.jobs);
   return a.type == kF16 ? launch_k(dequant_kernel<kF16>, grid, dim3(256), 0, st, a)
                         : launch_k(dequant_kernel<kBf16>, grid, dim3(256), 0, st, a);
-}
-
-cudaError_t launch_pad_rows(const uint16_t* x, int64_t rows, int64_t cols, uint16_t* out, int64_t ld, cudaStream_t st) {
-  return launch_k(pad_rows_kernel, dim3((unsigned)((rows * ld + 255) / 256)), dim3(256), 0, st, x, rows, cols, out, ld);
 }
 
 }  // namespace moe

@@ -1,31 +1,38 @@
-// dense_gemm.cu — 16-bit matrix products on tcgen05 with the feed-forward block's epilogues.
+// dense_gemm.cu — 4-bit matrix products on tcgen05 with the feed-forward block's epilogues.
 //
-// D[m, n] = sum_p A_p[m, :] . B_p[n, :]^T with fp32 accumulators in tensor memory. Tokens are
-// the MMA's rows (an epilogue thread owns one token and walks its columns), weight rows its
-// columns. Persistent CTAs (CG = 1) or CTA pairs (CG = 2): 128 tokens per CTA x 256 weight
-// rows per tile, K in steps of 64 elements (one 128-byte swizzled row per operand row).
-//   warp 8    one lane streams both operands with TMA into a ring of mbarrier stages;
-//   warp 9    allocates all 512 tensor-memory columns (two accumulators) and issues
-//             tcgen05.mma from one lane: M = 128 (or 256 over the pair), N = 256, K = 16;
-//   warps 0-7 read the finished accumulator back (warp w: TMEM lanes 32 (w % 4).., column
-//             half w / 4) and apply the epilogue while the next tile accumulates in the
-//             other buffer.
-// In the pair form each CTA loads its own 128 tokens and half of the 256 weight rows, so a
-// weight row crosses L2 -> SM once per 256 tokens; the leader (rank 0) owns the full and
-// accumulator-empty barriers and issues the MMAs of both. In the gated form the first 128
-// columns of a tile are gate rows and the second 128 the same rows of up, so that one thread
-// holds g and u of the same element.
-// K can be split over several CTAs when there are fewer tiles than SMs: fp32 partial sums,
-// then one launch that adds them in split order and applies the epilogue (no atomics, the
-// same bits on every run).
-// B may lie with its N contiguous (BN_MAJOR: the weights' rows are the summed index, in the
-// backward pass): boxes of 64 columns x 64 rows, read through the MN-major descriptor, so
-// that both directions use the weights as they are stored.
-// The epilogue moves global memory through a 2 KB buffer per warp: a thread owns a row of the
-// accumulator, but a warp's accesses cover 64 contiguous bytes of eight rows each.
+// D[m, n] = sum_p A_p[m, :] . W_p[n, :]^T, or A_p . W_p with the weights' rows as the summed
+// index (the gradient's direction), fp32 accumulators in tensor memory. The weights go from
+// their packed form straight into the operand tile: no 16-bit copy of them exists in global
+// memory. Tokens are the MMA's rows (an epilogue thread owns one token and walks its
+// columns), weights its columns; K runs in steps of 64.
+//   warp 20     streams the token tile with TMA (128 rows x 128 bytes, swizzled);
+//   warp 22     streams the packed tiles with TMA into a ring of their own;
+//   warps 4-19  four groups, taking the K steps in turn: 16 bytes of packed weights (32 weights,
+//               within one quantization group) per thread and item become four 16-byte
+//               pieces of the B tile, w = RN16(s q + b) (one rounding: a tcgen05 product
+//               takes both operands in one 16-bit type). With the rows summed, a word's eight
+//               weights are neighbours along N and the tile is MN-major; the addresses are
+//               the same in both layouts, only the meaning of a row differs;
+//   warp 21     allocates the tensor memory (two accumulators) and issues tcgen05.mma from one
+//               lane: M = 128 (256 over a pair of CTAs), K = 16;
+//   warps 0-3   read the finished accumulator back and apply the epilogue, while the next
+//               tile accumulates in the other buffer. A warp's global accesses go through a
+//               1 KB buffer, so that they cover 32 contiguous bytes of 16 rows each.
+// CTA pairs (CG = 2, more than 128 tokens): each CTA loads its own 128 tokens and dequantises
+// its half of the weight rows, once per 256 tokens; the leader (even rank) owns the full and
+// accumulator-empty barriers and issues the MMAs of both. In the gated form the two halves of
+// a tile's columns are gate rows and the same rows of up, so that one thread holds g and u of
+// the same element.
+// Few tiles: K is split over the CTAs of a cluster (up to 8). Each leaves its fp32 sums in its
+// own shared memory, and after a cluster barrier every CTA adds one slice of the tokens over
+// the cluster in split order (distributed shared memory; no atomics, the same bits on every
+// run) and applies the epilogue to it.
 // Every wait is bounded (2 s): on expiry the CTA records a code in the device's status word,
-// stops working and leaves through the same barriers as the rest of its pair.
+// stops working and leaves through the same barriers as the rest of its cluster.
 #include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <atomic>
 
 #include "dense.cuh"
 
@@ -33,36 +40,63 @@ namespace moe {
 
 namespace {
 
-constexpr int kBM = 128, kBN = 256, kBK = 64;
-constexpr int kATile = kBM * kBK * 2;        // 16 KB
-constexpr int kBHalf = 128 * kBK * 2;        // 16 KB: 128 weight rows
-constexpr int kEpiWarps = 8;
-constexpr int kTmaWarp = 8, kMmaWarp = 9;
-constexpr int kThreads = 320;
-constexpr int kStage2K = 2048;               // 32 rows x 32 columns of 16 bits
+constexpr int kBM = 128, kBK = 64;
+constexpr int kATile = kBM * kBK * 2;      // 16 KB
+constexpr int kBTile = 128 * kBK * 2;      // 16 KB: this CTA's weight rows of a tile, at most 128
+constexpr int kPackBytes = 128 * 32;       // 4 KB: their packed K step
+constexpr int kStageBuf = 1024;            // 32 rows x 16 columns of 16 bits, per epilogue warp
 constexpr uint64_t kWaitLimitNs = 2000ull * 1000 * 1000;
+constexpr int kSms = 148;
 
 __device__ int32_t g_dense_status;
 
-template <int CG>
+constexpr int kStageBytes = kATile + kBTile;
+constexpr int kSumPitch = 260;
+// The two sources of the weight tile. PACKED: dequantised by this kernel's warps; otherwise
+// 16-bit weights (dense_dequant.cu wrote them) that TMA copies like the tokens.
+// Shared memory: [stages][token tile, weight tile] | [slots][packed step] | [epilogue warps][1 KB]
+// | full[S] empty[S] acc_full[2] acc_empty[2] pfull[P] pempty[P] | tensor-memory base.
+template <bool PACKED>
 struct Cfg {
-  static constexpr int kStages = CG == 2 ? 6 : 4;
-  static constexpr int kStageBytes = kATile + (CG == 2 ? 1 : 2) * kBHalf;
-  // full[S] empty[S] acc_full[2] acc_empty[2] | tmem base
-  static constexpr int kStaging = kStages * kStageBytes;  // [epilogue warps][2 KB]
-  static constexpr int kBars = kStaging + kEpiWarps * kStage2K;
-  static constexpr int kSmem = kBars + 8 * (2 * kStages + 4) + 16 + 1024;
+  static constexpr int kEpiWarps = PACKED ? 4 : 8;
+  static constexpr int kGroups = PACKED ? 4 : 0;  // of 4 dequantising warps
+  static constexpr int kDeqWarp = kEpiWarps;
+  static constexpr int kTmaWarp = kDeqWarp + 4 * kGroups, kMmaWarp = kTmaWarp + 1, kPackWarp = kTmaWarp + 2;
+  static constexpr int kThreads = (kMmaWarp + 1 + (PACKED ? 1 : 0)) * 32;
+  static constexpr int kStages = PACKED ? 5 : 6, kSlots = PACKED ? 8 : 0;
+  static constexpr int kPackAt = kStages * kStageBytes;
+  static constexpr int kStagingAt = kPackAt + kSlots * kPackBytes;
+  static constexpr int kBarsAt = kStagingAt + kEpiWarps * kStageBuf;
+  static constexpr int kNumBars = 2 * kStages + 4 + 2 * kSlots;
+  static constexpr int kSmem = kBarsAt + 8 * kNumBars + 16 + 1024;
+  // A group that waits for a stage has written its step kGroups before, so the stage's
+  // previous use but one is over when kGroups <= kStages, and one parity bit tells the phases
+  // apart; a slot belongs to one group.
+  static_assert(kGroups <= kStages && (!PACKED || kSlots % (PACKED ? kGroups : 1) == 0), "phases told apart by parity");
+  // the split form leaves its sums, rows of 256 floats and one 16-byte piece (so that a column
+  // of rows spreads over the banks), over the operand stages
+  static_assert(kBM * kSumPitch * 4 <= kPackAt, "sums over the stages");
 };
 
+struct WeightSide {  // scales and biases of one operand pair's weights
+  const uint16_t* s;
+  const uint16_t* b;
+};
 struct GemmParams {
-  CUtensorMap a[2], b[2];
+  CUtensorMap a[2], w[2];
+  WeightSide q[2];
   int64_t M;
   int N;
+  int rows;             // weight rows of each matrix (N, or the summed K when ROWS_K)
+  int s_pitch;          // scales per weight row
+  int lg;               // log2 of the group size
   int gated;
+  int hb;               // weight rows (columns of D) per half of a tile
   int ks0, ks;          // K steps of the first operand pair, of all
-  int tiles_m, tiles_n, splits, spk;
-  int64_t units;
-  float* partial;       // [splits][M][tiles_n * kBN]
+  int tiles_m, splits, spk;
+  int units;            // tiles
+  int wide;             // the weights are 16-bit (w maps them), not packed
+  int early;            // the weights may be read before the launch before has completed
   DenseEpi e;
 };
 
@@ -77,10 +111,22 @@ MOE_DEV bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
       "selp.b32 %0, 1, 0, p;\n\t}\n"
       : "=r"(ok)
       : "r"(bar), "r"(parity), "r"(1000u)
+      : "memory");
+  return ok != 0;
+}
+// Non-blocking (a try_wait may hold the thread until the phase completes).
+MOE_DEV bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
       : "memory");
   return ok != 0;
 }
@@ -98,14 +144,20 @@ MOE_DEV bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* gone) {
     if (*gone || now_ns() - t0 > kWaitLimitNs) return false;
   return true;
 }
+MOE_DEV void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
 // The address of `a` in CTA `rank` of the cluster.
 MOE_DEV uint32_t map_rank(uint32_t a, uint32_t rank) {
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(rank));
   return r;
 }
+// Arrival on a barrier of this CTA, or of the pair's leader (an address from map_rank). CTA
+// scope on purpose: what it publishes is this SM's shared memory (after fence_proxy) or tensor
+// memory (after tc_before); cluster scope costs a fence over global memory in every step.
 MOE_DEV void mbar_arrive_cluster(uint32_t cluster_bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_bar) : "memory");
 }
 template <int CG>
 MOE_DEV void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -124,6 +176,14 @@ MOE_DEV void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t
 }
 MOE_DEV void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 MOE_DEV void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+MOE_DEV void fence_proxy() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+// 1 in one lane of the (converged) warp.
+MOE_DEV uint32_t elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
+  return r;
+}
 template <int CG>
 MOE_DEV void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   if constexpr (CG == 2)
@@ -137,14 +197,14 @@ MOE_DEV void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(acc));
 }
-// Arrives on `bar` of every CTA of the group when the MMAs issued so far have completed.
+// Arrives on `bar` of every CTA in `mask` when the MMAs issued so far have completed.
 template <int CG>
-MOE_DEV void tc_commit(uint32_t bar) {
+MOE_DEV void tc_commit(uint32_t bar, uint32_t mask) {
   if constexpr (CG == 2)
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(
             bar),
-        "h"((uint16_t)3)
+        "h"((uint16_t)mask)
         : "memory");
   else
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
@@ -160,16 +220,13 @@ MOE_DEV uint64_t sw128_mn_desc(uint32_t saddr) {
   return (uint64_t)((saddr >> 4) & 0x3fffu) | (uint64_t)(8192 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
          (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
-MOE_DEV void tmem_ld32(uint32_t taddr, float (&r)[32]) {
+MOE_DEV void tmem_ld16(uint32_t taddr, float (&r)[16]) {
   uint32_t* u = reinterpret_cast<uint32_t*>(r);
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
       : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
-        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
-        "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
-        "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
       : "r"(taddr));
 }
 MOE_DEV void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
@@ -241,10 +298,10 @@ MOE_DEV void epilogue8(const DenseEpi& e, int64_t m, int c, int n, bool vec, flo
   }
 }
 
-// ---- a warp's 32 rows x 32 columns through its staging buffer. 16-byte piece j of row r lies
-// at piece j ^ ((r >> 1) & 3): conflict-free both by row (one lane each) and by four lanes
-// of a row. cols: valid columns (a multiple of 8), rows: valid rows.
-MOE_DEV uint32_t stage_off(int r, int j) { return (uint32_t)(r * 64 + ((j ^ ((r >> 1) & 3)) << 4)); }
+// ---- a warp's 32 rows x 16 columns through its staging buffer. 16-byte piece j of row r lies
+// at piece j ^ ((r >> 2) & 1): conflict-free both by row (one lane each) and by two lanes of
+// a row. cols: valid columns (a multiple of 8), rows: valid rows.
+MOE_DEV uint32_t stage_off(int r, int j) { return (uint32_t)(r * 32 + ((j ^ ((r >> 2) & 1)) << 4)); }
 MOE_DEV void sts16(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -253,43 +310,54 @@ MOE_DEV uint4 lds16(uint32_t a) {
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
   return v;
 }
+// into a whole register, so that nothing has to wait for the value before its use
+MOE_DEV uint32_t ldg_u16(const uint16_t* p) {
+  uint32_t v;
+  asm volatile("ld.global.nc.u16 %0, [%1];\n" : "=r"(v) : "l"(p));
+  return v;
+}
+MOE_DEV float4 lds_cluster(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+  return v;
+}
 template <int TYPE>
-MOE_DEV void store_tile(uint32_t stage, const float (&v)[32], uint16_t* base, int64_t ld, int rows, int cols, int lane) {
+MOE_DEV void store_tile(uint32_t stage, const float (&v)[16], uint16_t* base, int64_t ld, int rows, int cols, int lane) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < 2; ++j)
     sts16(stage + stage_off(lane, j),
           make_uint4(Elem<TYPE>::pack(v[8 * j], v[8 * j + 1]), Elem<TYPE>::pack(v[8 * j + 2], v[8 * j + 3]),
                      Elem<TYPE>::pack(v[8 * j + 4], v[8 * j + 5]), Elem<TYPE>::pack(v[8 * j + 6], v[8 * j + 7])));
   __syncwarp();
-  const int j = lane & 3;
+  const int j = lane & 1;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 8 * i + (lane >> 2);
+  for (int i = 0; i < 2; ++i) {
+    const int r = 16 * i + (lane >> 1);
     const uint4 q = lds16(stage + stage_off(r, j));
     if (r < rows && 8 * j < cols) *reinterpret_cast<uint4*>(base + (int64_t)r * ld + 8 * j) = q;
   }
   __syncwarp();
 }
-struct Tile32 {
-  uint4 q[4];
+struct TileRegs {
+  uint4 q[2];
 };
-MOE_DEV void fetch_tile(Tile32& t, const uint16_t* base, int64_t ld, int rows, int cols, int lane) {
-  const int j = lane & 3;
+MOE_DEV void fetch_tile(TileRegs& t, const uint16_t* base, int64_t ld, int rows, int cols, int lane) {
+  const int j = lane & 1;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 8 * i + (lane >> 2);
+  for (int i = 0; i < 2; ++i) {
+    const int r = 16 * i + (lane >> 1);
     t.q[i] = r < rows && 8 * j < cols ? *reinterpret_cast<const uint4*>(base + (int64_t)r * ld + 8 * j)
                                       : make_uint4(0, 0, 0, 0);
   }
 }
 // The fetched tile, turned: this lane's row.
 template <int TYPE>
-MOE_DEV void turn_tile(uint32_t stage, const Tile32& t, float (&v)[32], int lane) {
+MOE_DEV void turn_tile(uint32_t stage, const TileRegs& t, float (&v)[16], int lane) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) sts16(stage + stage_off(8 * i + (lane >> 2), lane & 3), t.q[i]);
+  for (int i = 0; i < 2; ++i) sts16(stage + stage_off(16 * i + (lane >> 1), lane & 1), t.q[i]);
   __syncwarp();
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < 2; ++j) {
     const uint4 q = lds16(stage + stage_off(lane, j));
     v[8 * j] = Elem<TYPE>::lo(q.x), v[8 * j + 1] = Elem<TYPE>::hi(q.x);
     v[8 * j + 2] = Elem<TYPE>::lo(q.y), v[8 * j + 3] = Elem<TYPE>::hi(q.y);
@@ -299,34 +367,57 @@ MOE_DEV void turn_tile(uint32_t stage, const Tile32& t, float (&v)[32], int lane
   __syncwarp();
 }
 
-template <int CG, int EPI, int TYPE, bool BN_MAJOR>
-__global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
-  using C = Cfg<CG>;
+MOE_DEV void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+
+// CG: CTAs per tile; ROWS_K: the weights' rows are the summed index; SPLIT: a cluster per tile
+template <int CG, int EPI, int TYPE, bool ROWS_K, bool SPLIT, bool PACKED>
+__global__ void __launch_bounds__(Cfg<PACKED>::kThreads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
+  using C = Cfg<PACKED>;
+  constexpr int kStages = C::kStages, kSlots = C::kSlots, kGroups = C::kGroups, kEpiWarps = C::kEpiWarps;
+  constexpr int kDeqWarp = C::kDeqWarp, kTmaWarp = C::kTmaWarp, kMmaWarp = C::kMmaWarp, kPackWarp = C::kPackWarp;
+  constexpr int kPackAt = C::kPackAt, kStagingAt = C::kStagingAt, kBarsAt = C::kBarsAt;
+  static_assert(PACKED || (CG == 2 && !SPLIT), "the 16-bit form serves many tokens");
   extern __shared__ unsigned char smem_raw[];
+  // the same offset in every CTA of a cluster: the base of dynamic shared memory is
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
-  const uint32_t bar_full = sbase + C::kBars;
-  const uint32_t bar_empty = bar_full + 8 * C::kStages;
-  const uint32_t bar_accf = bar_empty + 8 * C::kStages;
+  const uint32_t bar_full = sbase + kBarsAt;
+  const uint32_t bar_empty = bar_full + 8 * kStages;
+  const uint32_t bar_accf = bar_empty + 8 * kStages;
   const uint32_t bar_acce = bar_accf + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBars + 8 * (2 * C::kStages + 4));
+  const uint32_t bar_pfull = bar_acce + 16;
+  const uint32_t bar_pempty = bar_pfull + 8 * kSlots;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kBarsAt + 8 * C::kNumBars);
   __shared__ int gone;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  uint32_t rank = 0;
-  if constexpr (CG == 2) asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(rank));
-  const int64_t first = blockIdx.x / CG, stride = gridDim.x / CG;
+  uint32_t crank = 0;
+  if constexpr (CG == 2 || SPLIT) asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(crank));
+  const int rank = CG == 2 ? (int)(crank & 1) : 0;   // in the pair
+  const int split = SPLIT ? (int)crank / CG : 0;
+  const uint32_t leader = CG == 2 ? crank & ~1u : crank;
+  const int ctas = SPLIT ? CG * p.splits : CG;       // CTAs of a tile
+  const int first = blockIdx.x / ctas, stride = gridDim.x / ctas;
+  constexpr int kHalves = 2 / CG;                    // of a tile's weight rows in this CTA
+  const int k0 = split * p.spk, k1 = k0 + p.spk < p.ks ? k0 + p.spk : p.ks;
 
   if (tid == 0) {
     gone = 0;
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(bar_full + 8 * s, 1);   // the leader's expect_tx
-      mbar_init(bar_empty + 8 * s, 1);  // one commit
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar_full + 8 * s, PACKED ? 1 + 4 * CG : 1);  // the leader's expect_tx for both CTAs' bytes, a group of each
+      mbar_init(bar_empty + 8 * s, 1);          // one commit
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar_accf + 8 * i, 1);
       mbar_init(bar_acce + 8 * i, CG * kEpiWarps);
+    }
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(bar_pfull + 8 * i, 1);
+      mbar_init(bar_pempty + 8 * i, 4);
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -343,127 +434,269 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   }
   tc_before();
   __syncthreads();
-  if constexpr (CG == 2) {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-  }
+  if constexpr (CG == 2 || SPLIT) cluster_sync();
   tc_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_wait();
+  // `early`: the launch before this one writes no weights, and let this one start only after
+  // everything before it had completed (a later product of one call)
+  const bool weights = PACKED && ((warp >= kDeqWarp && warp < kTmaWarp) || warp == kPackWarp);
+  if (!(weights && p.early)) {
+    pdl_wait();
+    pdl_trigger();
+  }
 
-  // unit -> (m tile, split, n tile), m fastest
-  auto unit_of = [&](int64_t unit, int& mt, int& sp, int& nt) {
-    mt = (int)(unit % p.tiles_m);
-    const int64_t r = unit / p.tiles_m;
-    sp = (int)(r % p.splits);
-    nt = (int)(r / p.splits);
-  };
-  auto steps_of = [&](int sp, int& k0, int& k1) {
-    k0 = sp * p.spk;
-    k1 = k0 + p.spk < p.ks ? k0 + p.spk : p.ks;
+  auto tile_m = [&](int unit) { return unit % p.tiles_m; };
+  auto tile_n = [&](int unit) { return unit / p.tiles_m; };
+  // first weight row (column of D) of this CTA's half h of n tile nt
+  auto half_row = [&](int nt, int h) {
+    const int half = CG == 2 ? rank : h;
+    return p.gated ? nt * p.hb : nt * 2 * p.hb + half * p.hb;
   };
 
   if (warp == kTmaWarp) {
     if (lane == 0) {
       int it = 0;
       bool ok = true;
-      for (int64_t unit = first; ok && unit < p.units; unit += stride) {
-        int mt, sp, nt, k0, k1;
-        unit_of(unit, mt, sp, nt);
-        steps_of(sp, k0, k1);
-        const int m0 = (mt * CG + (int)rank) * kBM;
+      for (int unit = first; ok && unit < p.units; unit += stride) {
+        const int m0 = (tile_m(unit) * CG + rank) * kBM;
         for (int k = k0; k < k1; ++k, ++it) {
-          const int s = it % C::kStages;
-          if (!mbar_wait(bar_empty + 8 * s, ((it / C::kStages) & 1) ^ 1, &gone)) {
+          const int s = it % kStages;
+          if (!mbar_wait(bar_empty + 8 * s, ((it / kStages) & 1) ^ 1, &gone)) {
             gone = 1;
             atomicOr(&g_dense_status, 1);
             ok = false;
             break;
           }
-          const uint32_t st = sbase + s * C::kStageBytes;
           uint32_t bar = bar_full + 8 * s;
-          if (rank == 0) mbar_expect_tx(bar, CG * C::kStageBytes);
-          if constexpr (CG == 2) bar = map_rank(bar, 0);
+          if (rank == 0) mbar_expect_tx(bar, PACKED ? CG * kATile : CG * (kATile + p.hb * 128));
+          if constexpr (CG == 2) bar = map_rank(bar, leader);
           const int pr = k >= p.ks0 ? 1 : 0;
           const int x = (k - (pr ? p.ks0 : 0)) * kBK;
-          tma_2d<CG>(st, &p.a[pr], x, m0, bar);
-#pragma unroll
-          for (int h = 0; h < (CG == 2 ? 1 : 2); ++h) {
-            const int half = CG == 2 ? (int)rank : h;
-            if constexpr (BN_MAJOR) {
-              const int n = nt * kBN + half * 128;
-              tma_2d<CG>(st + kATile + h * kBHalf, &p.b[pr], n, x, bar);
-              tma_2d<CG>(st + kATile + h * kBHalf + kBHalf / 2, &p.b[pr], n + 64, x, bar);
-            } else {
-              const CUtensorMap* bm = p.gated ? &p.b[half] : &p.b[pr];
-              const int y = p.gated ? nt * 128 : nt * kBN + half * 128;
-              tma_2d<CG>(st + kATile + h * kBHalf, bm, x, y, bar);
+          tma_2d<CG>(sbase + s * kStageBytes, &p.a[pr], x, m0, bar);
+          if constexpr (!PACKED) {
+            const uint32_t dst = sbase + s * kStageBytes + kATile;
+            const int n = half_row(tile_n(unit), 0);
+            if constexpr (ROWS_K) {  // boxes of 64 rows x 64 columns
+              for (int b = 0; b < p.hb / 64; ++b) tma_2d<CG>(dst + b * (kBTile / 2), &p.w[pr], n + 64 * b, x, bar);
+            } else {                 // hb rows x 64 columns
+              tma_2d<CG>(dst, &p.w[p.gated ? rank : pr], x, n, bar);
             }
           }
         }
       }
       // no copy may still be landing, and no MMA's arrival still be under way, when the CTA
       // leaves: the leader's full barriers count both CTAs' bytes, and the pair leaves together
-      for (int i = it - C::kStages < 0 ? 0 : it - C::kStages; ok && i < it; ++i)
-        if (!mbar_wait(bar_empty + 8 * (i % C::kStages), (i / C::kStages) & 1, &gone)) {
+      for (int i = it - kStages < 0 ? 0 : it - kStages; ok && i < it; ++i)
+        if (!mbar_wait(bar_empty + 8 * (i % kStages), (i / kStages) & 1, &gone)) {
           gone = 1;
           atomicOr(&g_dense_status, 1);
           ok = false;
         }
       if (!ok && rank == 0)
-        for (int i = it - C::kStages < 0 ? 0 : it - C::kStages; i < it; ++i) {
+        for (int i = it - kStages < 0 ? 0 : it - kStages; i < it; ++i) {
           int never = 0;
-          if (!mbar_wait(bar_full + 8 * (i % C::kStages), (i / C::kStages) & 1, &never)) atomicOr(&g_dense_status, 2);
+          if (!mbar_wait(bar_full + 8 * (i % kStages), (i / kStages) & 1, &never)) atomicOr(&g_dense_status, 2);
         }
     }
-  } else if (warp == kMmaWarp) {
-    if (lane == 0 && rank == 0) {
-      const uint32_t idesc = (1u << 4) | (TYPE == kBf16 ? (1u << 7) | (1u << 10) : 0u) | (BN_MAJOR ? 1u << 16 : 0u) |
-                             ((uint32_t)(kBN >> 3) << 17) | ((uint32_t)(CG * kBM >> 4) << 24);
-      int it = 0, tile = 0;
+  } else if (PACKED && warp == kPackWarp) {
+   if constexpr (PACKED)
+    if (lane == 0) {
+      int it = 0;
       bool ok = true;
-      for (int64_t unit = first; ok && unit < p.units; unit += stride, ++tile) {
-        int mt, sp, nt, k0, k1;
-        unit_of(unit, mt, sp, nt);
-        steps_of(sp, k0, k1);
-        const int buf = tile & 1;
-        if (!mbar_wait(bar_acce + 8 * buf, ((tile >> 1) & 1) ^ 1, &gone)) {
+      for (int unit = first; ok && unit < p.units; unit += stride) {
+        const int nt = tile_n(unit);
+        for (int k = k0; k < k1; ++k, ++it) {
+          const int s = it % kSlots;
+          if (!mbar_wait(bar_pempty + 8 * s, ((it / kSlots) & 1) ^ 1, &gone)) {
+            gone = 1;
+            atomicOr(&g_dense_status, 32);
+            ok = false;
+            break;
+          }
+          const uint32_t bar = bar_pfull + 8 * s;
+          mbar_expect_tx(bar, kHalves * p.hb * 32);
+          const int pr = k >= p.ks0 ? 1 : 0;
+          const int kk = k - (pr ? p.ks0 : 0);
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h) {
+            const uint32_t dst = sbase + kPackAt + s * kPackBytes + h * (kPackBytes / 2);
+            const int n = half_row(nt, h);
+            if constexpr (ROWS_K) {  // boxes of 64 rows x 64 columns
+              for (int b = 0; b < p.hb / 64; ++b) tma_2d<1>(dst + b * 2048, &p.w[pr], n / 8 + b * 8, kk * kBK, bar);
+            } else {                 // hb rows x 64 columns
+              tma_2d<1>(dst, &p.w[p.gated ? (CG == 2 ? rank : h) : pr], kk * 8, n, bar);
+            }
+          }
+        }
+      }
+      // no copy may still be landing when the CTA leaves
+      for (int i = it - kSlots < 0 ? 0 : it - kSlots; i < it; ++i) {
+        int never = 0;
+        if (!mbar_wait(bar_pfull + 8 * (i % kSlots), (i / kSlots) & 1, &never)) atomicOr(&g_dense_status, 64);
+      }
+    }
+  } else if (PACKED && warp >= kDeqWarp && warp < kTmaWarp) {
+   if constexpr (PACKED) {
+    // ---- dequantisation: group wg takes steps wg, wg + kGroups, ... of this CTA's sequence
+    const int wg = (warp - kDeqWarp) >> 2, wt = tid - (kDeqWarp + 4 * wg) * 32;
+    // Item i of a thread: 32 columns (wt % 2) of row wt / 2 of 64: rows 64 i.. of this CTA's
+    // half (CG = 2), or half i (CG = 1). With ROWS_K the 64 rows are the summed ones, and i
+    // is the block of 64 columns.
+    constexpr int kItems = 2;
+    auto item_half = [](int i) { return CG == 2 ? 0 : i; };
+    auto item_row = [](int i) { return CG == 2 ? 64 * i : 0; };
+    const int j = wt & 1, r0 = wt >> 1;
+    const int per = k1 - k0;
+    const int total = first < p.units ? (int)((p.units - first + stride - 1) / stride) * per : 0;
+    // The scales and biases of the group's next two steps, read ahead: at_k walks the steps,
+    // the pointers are those of its tile and operand pair.
+    const uint16_t* ps[kItems];
+    const uint16_t* pb[kItems];
+    uint32_t valid = 0;
+    int at_unit = first, at_k = k0 + wg, at_key = -1;
+    while (at_k >= k1) at_k -= per, at_unit += stride;
+    auto read_scales = [&](uint32_t (&vs)[kItems], uint32_t (&vb)[kItems]) {
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) vs[i] = vb[i] = 0u;
+      if (at_unit < p.units) {
+        const int pr = at_k >= p.ks0 ? 1 : 0;
+        if (at_key != 2 * at_unit + pr) {
+          at_key = 2 * at_unit + pr;
+          valid = 0;
+          const int nt = tile_n(at_unit);
+#pragma unroll
+          for (int i = 0; i < kItems; ++i) {
+            const int n = half_row(nt, item_half(i)) + item_row(i) + (ROWS_K ? 32 * j : r0);
+            const WeightSide& q = p.q[p.gated ? (CG == 2 ? rank : i) : pr];
+            const int64_t off = ROWS_K ? (int64_t)r0 * p.s_pitch + (n >> p.lg) : (int64_t)n * p.s_pitch;
+            const bool in = n < p.N && item_row(i) + (ROWS_K ? 0 : r0) < p.hb;
+            valid |= in ? 1u << i : 0u;
+            ps[i] = q.s + (in ? off : 0);
+            pb[i] = q.b ? q.b + (in ? off : 0) : nullptr;
+          }
+        }
+        const int kk = at_k - (pr ? p.ks0 : 0);
+        const int g = (kk * kBK + 32 * j) >> p.lg;
+        const int64_t off = ROWS_K ? (int64_t)(kk * kBK) * p.s_pitch : g;
+        const bool in = ROWS_K ? kk * kBK + r0 < p.rows : g < p.s_pitch;
+        if (in) {
+#pragma unroll
+          for (int i = 0; i < kItems; ++i)
+            if (valid >> i & 1) {
+              vs[i] = ldg_u16(ps[i] + off);
+              if (pb[i]) vb[i] = ldg_u16(pb[i] + off);
+            }
+        }
+      }
+      at_k += kGroups;
+      while (at_k >= k1) at_k -= per, at_unit += stride;
+    };
+    uint32_t rs[2][kItems], rb[2][kItems];
+    read_scales(rs[0], rb[0]);
+    read_scales(rs[1], rb[1]);
+    bool ok = true;
+    for (int it = wg; ok && it < total; it += 2 * kGroups) {
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {  // two steps per round: constant ring indexes
+        const int step = it + kGroups * sub;
+        if (step >= total) break;
+        const int s = step % kStages, sl = step % kSlots;
+        bool ready = mbar_wait(bar_pfull + 8 * sl, (step / kSlots) & 1, &gone);
+        uint4 q[kItems];
+        if (__all_sync(0xffffffffu, ready)) {
+#pragma unroll
+          for (int i = 0; i < kItems; ++i)
+            q[i] = lds16(sbase + kPackAt + sl * kPackBytes + (128 * i + wt) * 16);
+          ready = mbar_wait(bar_empty + 8 * s, ((step / kStages) & 1) ^ 1, &gone);
+        }
+        if (!__all_sync(0xffffffffu, ready)) {
           gone = 1;
-          atomicOr(&g_dense_status, 4);
+          if (lane == 0) atomicOr(&g_dense_status, 128);
+          ok = false;
+          break;
+        }
+        const uint32_t bt = sbase + s * kStageBytes + kATile;
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+          if (item_row(i) + (ROWS_K ? 0 : r0) >= p.hb) continue;
+          const uint32_t s2 = __byte_perm(rs[sub][i], 0, 0x1010), b2 = __byte_perm(rb[sub][i], 0, 0x1010);
+          // rows of 128 bytes; the second half (CG = 1) follows the first hb of them
+          const uint32_t row = bt + (uint32_t)(CG == 2 ? 64 * i : p.hb * i) * 128 + r0 * 128;
+          const uint32_t* w = &q[i].x;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            sts16(row + (((uint32_t)(4 * j + c) ^ (r0 & 7)) << 4), dequant8<TYPE>(w[c], s2, b2));
+        }
+        fence_proxy();
+        __syncwarp();
+        // the packed words are in use by now: only here may their slot be filled again
+        if (lane == 0) mbar_arrive(bar_pempty + 8 * sl);
+        if (lane == 0) mbar_arrive_cluster(CG == 2 ? map_rank(bar_full + 8 * s, leader) : bar_full + 8 * s);
+        read_scales(rs[sub], rb[sub]);
+      }
+    }
+   }
+  } else if (warp == kMmaWarp) {
+    // The whole warp walks the steps, so that descriptors and addresses stay in uniform
+    // registers; one elected lane issues. The next stage's barrier is asked about before this
+    // stage's MMAs are issued: an answer takes about as long as two of them.
+    if (rank == 0) {
+      const uint32_t one = elect_one();
+      const uint32_t idesc = (1u << 4) | (TYPE == kBf16 ? (1u << 7) | (1u << 10) : 0u) | (ROWS_K ? 1u << 16 : 0u) |
+                             ((uint32_t)(2 * p.hb >> 3) << 17) | ((uint32_t)(CG * kBM >> 4) << 24);
+      const uint32_t both = 3u << leader;
+      const uint64_t ad0 = sw128_desc(sbase);
+      const uint64_t bd0 = ROWS_K ? sw128_mn_desc(sbase + kATile) : sw128_desc(sbase + kATile);
+      constexpr int kBStep = ROWS_K ? (16 * 128) >> 4 : 32 >> 4;  // 16 rows, or 32 bytes of each row
+      int s = 0, tile = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      bool ready = mbar_test(bar_full, 0);
+      for (int unit = first; ok && unit < p.units; unit += stride, ++tile) {
+        const int buf = tile & 1;
+        if (!__all_sync(0xffffffffu, mbar_wait(bar_acce + 8 * buf, ((tile >> 1) & 1) ^ 1, &gone))) {
+          gone = 1;
+          if (lane == 0) atomicOr(&g_dense_status, 4);
           break;
         }
         tc_after();
-        for (int k = k0; k < k1; ++k, ++it) {
-          const int s = it % C::kStages;
-          if (!mbar_wait(bar_full + 8 * s, (it / C::kStages) & 1, &gone)) {
+        for (int k = k0; k < k1; ++k) {
+          if (!ready) ready = mbar_wait(bar_full + 8 * s, phase, &gone);
+          if (!__all_sync(0xffffffffu, ready)) {
             gone = 1;
-            atomicOr(&g_dense_status, 8);
+            if (lane == 0) atomicOr(&g_dense_status, 8);
             ok = false;
             break;
           }
           tc_after();
-          const uint64_t ad = sw128_desc(sbase + s * C::kStageBytes);
-          const uint32_t bs = sbase + s * C::kStageBytes + kATile;
-          const uint64_t bd = BN_MAJOR ? sw128_mn_desc(bs) : sw128_desc(bs);
-          constexpr int kBStep = BN_MAJOR ? (16 * 128) >> 4 : 32 >> 4;  // 16 rows, or 32 bytes of each row
+          const int next = s + 1 == kStages ? 0 : s + 1;
+          const uint32_t next_phase = next ? phase : phase ^ 1;
+          ready = mbar_test(bar_full + 8 * next, next_phase);
+          const uint32_t at = (uint32_t)(s * kStageBytes) >> 4;
+          if (one) {
 #pragma unroll
-          for (int j = 0; j < kBK / 16; ++j)
-            tc_mma<CG>(tmem + buf * kBN, ad + 2 * j, bd + kBStep * j, idesc, (k > k0 || j > 0) ? 1u : 0u);
-          tc_commit<CG>(bar_empty + 8 * s);
+            for (int j = 0; j < kBK / 16; ++j)
+              tc_mma<CG>(tmem + buf * 256, ad0 + at + 2 * j, bd0 + at + kBStep * j, idesc, (k > k0 || j > 0) ? 1u : 0u);
+            tc_commit<CG>(bar_empty + 8 * s, both);
+            if (k == k1 - 1) tc_commit<CG>(bar_accf + 8 * buf, both);
+          }
+          __syncwarp();
+          s = next;
+          phase = next_phase;
         }
-        tc_commit<CG>(bar_accf + 8 * buf);
       }
     }
   } else {
     // ---- epilogue warps
-    const int quad = warp & 3, half = warp >> 2;
+    const int quad = warp & 3;
+    constexpr int kChunkStep = kEpiWarps / 4;  // warps that share a lane quadrant take chunks in turn
     const bool vec = ((p.N | p.e.ldo) & 7) == 0;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-    const uint32_t stage = sbase + C::kStaging + warp * kStage2K;
+    const uint32_t stage = sbase + kStagingAt + warp * kStageBuf;
+    const int chunks = (EPI == kEpiGated ? p.hb : 2 * p.hb) / 16;  // of 16 output columns
     int tile = 0;
-    for (int64_t unit = first; unit < p.units; unit += stride, ++tile) {
-      int mt, sp, nt;
-      unit_of(unit, mt, sp, nt);
+    for (int unit = first; unit < p.units; unit += stride, ++tile) {
+      const int nt = tile_n(unit);
       const int buf = tile & 1;
       const bool ready = mbar_wait(bar_accf + 8 * buf, (tile >> 1) & 1, &gone);
       if (!__all_sync(0xffffffffu, ready)) {
@@ -472,32 +705,27 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
         break;
       }
       tc_after();
-      const uint32_t acc = tmem + buf * kBN + lanes;
-      const int64_t m = (int64_t)(mt * CG + (int)rank) * kBM + quad * 32 + lane;
-      if (p.splits > 1) {
-#pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          const int c = half * 128 + q * 32;
-          float d[32];
-          tmem_ld32(acc + c, d);
+      const uint32_t acc = tmem + buf * 256 + lanes;
+      const int64_t mrow = (int64_t)(tile_m(unit) * CG + rank) * kBM + quad * 32;  // the warp's first row
+      if constexpr (SPLIT) {
+        // the sums into this CTA's shared memory (the stages are free: every MMA has completed)
+        for (int q = warp >> 2; q < 2 * p.hb / 16; q += kChunkStep) {
+          float d[16];
+          tmem_ld16(acc + 16 * q, d);
           tmem_wait_ld();
-          if (m < p.M) {
-            float4* dst = reinterpret_cast<float4*>(p.partial + (((int64_t)sp * p.M + m) * p.tiles_n + nt) * kBN + c);
+          const uint32_t dst = sbase + (uint32_t)((quad * 32 + lane) * kSumPitch + 16 * q) * 4;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) dst[i] = make_float4(d[4 * i], d[4 * i + 1], d[4 * i + 2], d[4 * i + 3]);
-          }
+          for (int i = 0; i < 4; ++i)
+            sts16(dst + 16 * i, make_uint4(__float_as_uint(d[4 * i]), __float_as_uint(d[4 * i + 1]),
+                                           __float_as_uint(d[4 * i + 2]), __float_as_uint(d[4 * i + 3])));
         }
       } else {
-        constexpr int kChunks = EPI == kEpiGated ? 2 : 4;  // of 32 output columns, this warp's half
-        const int64_t mrow = m - lane;  // the warp's first row
         const int rows = p.M - mrow < 32 ? (int)(p.M - mrow) : 32;  // may be <= 0
         const int64_t ld = p.e.ldo;
-        auto column = [&](int q) {
-          return EPI == kEpiGated ? nt * 128 + half * 64 + q * 32 : nt * kBN + half * 128 + q * 32;
-        };
-        Tile32 tg, tu;
+        const int n0 = EPI == kEpiGated ? nt * p.hb : nt * 2 * p.hb;
+        TileRegs tg, tu;
         auto fetch = [&](int q) {
-          const int n = column(q);
+          const int n = n0 + 16 * q;
           const int64_t at = mrow * ld + n;
           if constexpr (EPI == kEpiGatedBackward) {
             fetch_tile(tg, p.e.gate + at, ld, rows, p.N - n, lane);
@@ -506,22 +734,21 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             if (p.e.residual) fetch_tile(tg, p.e.residual + at, ld, rows, p.N - n, lane);
           }
         };
-        if (vec) fetch(0);
+        if (vec) fetch(warp >> 2);
 #pragma unroll 1
-        for (int q = 0; q < kChunks; ++q) {
-          const int c = EPI == kEpiGated ? half * 64 + q * 32 : half * 128 + q * 32;
-          const int n = column(q);
-          float d[32], u[32];
-          tmem_ld32(acc + c, d);
-          if constexpr (EPI == kEpiGated) tmem_ld32(acc + 128 + c, u);
+        for (int q = warp >> 2; q < chunks; q += kChunkStep) {
+          const int n = n0 + 16 * q;
+          float d[16], u[16];
+          tmem_ld16(acc + 16 * q, d);
+          if constexpr (EPI == kEpiGated) tmem_ld16(acc + p.hb + 16 * q, u);
           tmem_wait_ld();
           if (!vec) {  // rows of any length: element by element
-            if (m < p.M) {
+            if (lane < rows) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
+              for (int i = 0; i < 2; ++i) {
                 float(&d8)[8] = *reinterpret_cast<float(*)[8]>(d + 8 * i);
                 const float(&u8)[8] = *reinterpret_cast<float(*)[8]>((EPI == kEpiGated ? u : d) + 8 * i);
-                if (n + 8 * i < p.N) epilogue8<EPI, TYPE>(p.e, m, n + 8 * i, p.N, false, d8, u8);
+                if (n + 8 * i < p.N) epilogue8<EPI, TYPE>(p.e, mrow + lane, n + 8 * i, p.N, false, d8, u8);
               }
             }
             continue;
@@ -531,26 +758,27 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
           if constexpr (EPI == kEpiPlain) {
             if (p.e.residual) {
               turn_tile<TYPE>(stage, tg, u, lane);
-              if (q + 1 < kChunks) fetch(q + 1);
+              if (q + kChunkStep < chunks) fetch(q + kChunkStep);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) d[i] += u[i];
+              for (int i = 0; i < 16; ++i) d[i] += u[i];
             }
             store_tile<TYPE>(stage, d, p.e.out + at, ld, rows, cols, lane);
           } else if constexpr (EPI == kEpiGated) {
+            // g and u stay in fp32 up to h, which is rounded once
             if (p.e.gate) {
               store_tile<TYPE>(stage, d, p.e.gate + at, ld, rows, cols, lane);
               store_tile<TYPE>(stage, u, p.e.up + at, ld, rows, cols, lane);
             }
 #pragma unroll
-            for (int i = 0; i < 32; ++i) d[i] = act_val(d[i], p.e.act) * u[i];
+            for (int i = 0; i < 16; ++i) d[i] = act_val(d[i], p.e.act) * u[i];
             store_tile<TYPE>(stage, d, p.e.out + at, ld, rows, cols, lane);
           } else {
-            float g[32];
+            float g[16];
             turn_tile<TYPE>(stage, tg, g, lane);
             turn_tile<TYPE>(stage, tu, u, lane);
-            if (q + 1 < kChunks) fetch(q + 1);
+            if (q + kChunkStep < chunks) fetch(q + kChunkStep);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
+            for (int i = 0; i < 16; ++i) {
               float val, grad;
               act_grad(g[i], p.e.act, val, grad);
               g[i] = d[i] * u[i] * grad;
@@ -563,17 +791,59 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       }
       tc_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(CG == 2 ? map_rank(bar_acce + 8 * buf, 0) : bar_acce + 8 * buf);
+      if (lane == 0) mbar_arrive_cluster(CG == 2 ? map_rank(bar_acce + 8 * buf, leader) : bar_acce + 8 * buf);
     }
   }
   __syncwarp();
+  if constexpr (SPLIT) {
+    // ---- every CTA's sums lie in its shared memory: this one adds its slice of the rows
+    cluster_sync();
+    {
+      const int slice = (kBM + p.splits - 1) / p.splits, r0 = split * slice;
+      const int r1 = r0 + slice < kBM ? r0 + slice : kBM;
+      const int nt = tile_n(first);
+      const int n0 = EPI == kEpiGated ? nt * p.hb : nt * 2 * p.hb;
+      const int groups = (EPI == kEpiGated ? p.hb : 2 * p.hb) / 8;
+      const bool vec = ((p.N | p.e.ldo) & 7) == 0;
+      for (int i = tid; i < (r1 - r0) * groups; i += C::kThreads) {
+        const int r = r0 + i / groups, c = (i % groups) * 8;
+        const int64_t m = (int64_t)(tile_m(first) * CG + rank) * kBM + r;
+        if (m >= p.M || n0 + c >= p.N) continue;
+        float d[8] = {}, u[8] = {};
+        constexpr int kVecs = EPI == kEpiGated ? 4 : 2;
+        constexpr int kFly = EPI == kEpiGated ? 2 : 4;  // splits' pieces in flight
+        for (int sp = 0; sp < p.splits; sp += kFly) {
+          float4 v[kFly][kVecs];
+#pragma unroll
+          for (int s = 0; s < kFly; ++s)
+            if (sp + s < p.splits) {
+              const uint32_t src = map_rank(sbase + (uint32_t)(r * kSumPitch + c) * 4, (uint32_t)((sp + s) * CG + rank));
+              v[s][0] = lds_cluster(src), v[s][1] = lds_cluster(src + 16);
+              if constexpr (EPI == kEpiGated)
+                v[s][2] = lds_cluster(src + p.hb * 4), v[s][3] = lds_cluster(src + p.hb * 4 + 16);
+            }
+#pragma unroll
+          for (int s = 0; s < kFly; ++s)
+            if (sp + s < p.splits) {
+              const float* x = &v[s][0].x;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) d[e] += x[e];
+              if constexpr (EPI == kEpiGated) {
+                const float* y = &v[s][2].x;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) u[e] += y[e];
+              }
+            }
+        }
+        epilogue8<EPI, TYPE>(p.e, m, n0 + c, p.N, vec, d, u);
+      }
+    }
+    __syncwarp();
+  }
   tc_before();
   __syncthreads();
-  if constexpr (CG == 2) {
-    // the peer's MMAs read this CTA's shared memory and arrive on its barriers
-    asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-  }
+  // the peers' MMAs and sums read this CTA's shared memory and arrive on its barriers
+  if constexpr (CG == 2 || SPLIT) cluster_sync();
   if (warp == kMmaWarp) {
     tc_after();
     if constexpr (CG == 2)
@@ -581,32 +851,6 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     else
       asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
   }
-}
-
-// Adds the splits' partial sums in split order and applies the epilogue: a thread owns eight
-// columns of one token.
-template <int EPI, int TYPE>
-__global__ void __launch_bounds__(256) reduce_kernel(const __grid_constant__ GemmParams p) {
-  pdl_wait();
-  const int groups = (p.N + 7) / 8;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= p.M * groups) return;
-  const int64_t m = i / groups;
-  const int c = (int)(i - m * groups) * 8;
-  const int64_t pitch = (int64_t)p.tiles_n * kBN;
-  // gated: tile c / 128 holds 128 gate sums, then the 128 up sums
-  const int64_t at = EPI == kEpiGated ? (int64_t)(c / 128) * kBN + c % 128 : c;
-  float d[8] = {}, u[8] = {};
-  for (int s = 0; s < p.splits; ++s) {
-    const float* row = p.partial + ((int64_t)s * p.M + m) * pitch + at;
-    const float4 a = *reinterpret_cast<const float4*>(row), b = *reinterpret_cast<const float4*>(row + 4);
-    d[0] += a.x, d[1] += a.y, d[2] += a.z, d[3] += a.w, d[4] += b.x, d[5] += b.y, d[6] += b.z, d[7] += b.w;
-    if constexpr (EPI == kEpiGated) {
-      const float4 e = *reinterpret_cast<const float4*>(row + 128), f = *reinterpret_cast<const float4*>(row + 132);
-      u[0] += e.x, u[1] += e.y, u[2] += e.z, u[3] += e.w, u[4] += f.x, u[5] += f.y, u[6] += f.z, u[7] += f.w;
-    }
-  }
-  epilogue8<EPI, TYPE>(p.e, m, c, p.N, ((p.N | p.e.ldo) & 7) == 0, d, u);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
@@ -621,61 +865,99 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   return fn;
 }
 
-// [rows][cols] 16-bit elements, rows ld apart, boxes of box_rows rows x 64 elements.
-cudaError_t encode(CUtensorMap* map, const uint16_t* ptr, int64_t rows, int cols, int64_t ld, int box_rows, int type) {
+cudaError_t encode(CUtensorMap* map, CUtensorMapDataType type, const void* ptr, int64_t rows, int64_t cols,
+                   int64_t pitch_bytes, int box_cols, int box_rows, CUtensorMapSwizzle swizzle) {
   auto enc = encoder();
   if (!enc) return cudaErrorNotSupported;
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-  const cuuint32_t box[2] = {kBK, (cuuint32_t)box_rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)pitch_bytes};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   const cuuint32_t one[2] = {1, 1};
-  const CUresult r =
-      enc(map, type == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-          const_cast<uint16_t*>(ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = enc(map, type, 2, const_cast<void*>(ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-struct Plan {
-  int cg, tiles_m, tiles_n, splits, ks0, ks, spk;
-};
-constexpr int kSms = 148;
-
-// Tiles and splits of a product. One CTA per 128 tokens when there is one such tile, pairs
-// above. Splits: while the tiles leave at least half of the SMs idle and a split keeps eight
-// K steps (a split's partial sums cost a write and a read of 4 bytes per output).
-Plan plan(int64_t M, int N, int K, int pairs, bool gated) {
-  Plan q{};
-  q.cg = M > kBM ? 2 : 1;
-  q.tiles_m = (int)((M + q.cg * kBM - 1) / (q.cg * kBM));
-  q.tiles_n = gated ? (N + 127) / 128 : (N + kBN - 1) / kBN;
-  q.ks0 = (K + kBK - 1) / kBK;
-  q.ks = q.ks0 * pairs;
-  const int64_t ctas = (int64_t)q.tiles_m * q.tiles_n * q.cg;
-  q.splits = 1;
-  while (ctas * q.splits * 2 <= kSms && q.ks / (q.splits * 2) >= 8) q.splits *= 2;
-  q.spk = (q.ks + q.splits - 1) / q.splits;
-  q.splits = (q.ks + q.spk - 1) / q.spk;  // no empty split
-  return q;
+// Clusters of n CTAs of the kernel that the device holds at once: the SMs of a GPC beyond a
+// multiple of n stay empty. Asked once per device and size.
+int resident_clusters(int n) {
+  if (n == 1) return kSms;
+  static std::atomic<int> known[64][9];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return kSms / n;
+  int got = known[dev][n].load(std::memory_order_relaxed);
+  if (got) return got;
+  auto kern = gemm_kernel<2, kEpiPlain, kBf16, false, true, true>;  // every form has the same shape
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(n * kSms);
+  cfg.blockDim = dim3(Cfg<true>::kThreads);
+  cfg.dynamicSmemBytes = Cfg<true>::kSmem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = n;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<true>::kSmem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&got, kern, &cfg) != cudaSuccess || got < 1) {
+    (void)cudaGetLastError();
+    got = kSms / n;
+  }
+  known[dev][n].store(got, std::memory_order_relaxed);
+  return got;
 }
 
-template <int CG, int EPI, int TYPE, bool BN_MAJOR>
+struct Plan {
+  int cg, hb, tiles_m, tiles_n, splits, ks0, ks, spk;
+};
+
+// Tile width and K split of a product: the pair that takes the fewest K steps' time over the
+// rounds of tiles. A step costs about 0.36 us at 256 columns and no less than 0.2 (the token
+// tile's bytes and the barriers); a tile's start and epilogue about 2 us, the exchange of a
+// split's sums 3 us. (512 tokens, 2048 -> 2 x 5632 gated: see the table of cases.)
+Plan plan(int64_t M, int N, int K, int pairs, bool gated, bool rows_k, bool wide) {
+  Plan best{};
+  double least = 0;
+  const int cg = M > kBM ? 2 : 1;
+  const int tiles_m = (int)((M + cg * kBM - 1) / (cg * kBM));
+  const int ks0 = (K + kBK - 1) / kBK, ks = ks0 * pairs;
+  // a CTA holds at most 128 weight rows: a half over a pair, both halves alone
+  for (int hb = cg == 2 ? 128 : 64; hb >= (cg == 2 || rows_k ? 64 : 32); hb -= rows_k ? 64 : 32) {
+    const int tiles_n = gated ? (N + hb - 1) / hb : (N + 2 * hb - 1) / (2 * hb);
+    for (int sp = 1; sp * cg <= (wide ? cg : 8); ++sp) {
+      const int spk = (ks + sp - 1) / sp;
+      if ((ks + spk - 1) / spk != sp) continue;  // no empty split
+      const int64_t slots = resident_clusters(cg * sp);
+      const double rounds = (double)(((int64_t)tiles_m * tiles_n + slots - 1) / slots);
+      const double step = std::max(0.2, 0.36 * (cg == 2 ? hb : 2 * hb) / 128);
+      const double t = rounds * (spk * step + 2.0) + (sp > 1 ? 3.0 : 0.0);
+      if (best.cg == 0 || t < least * 0.98) {
+        least = t;
+        best = Plan{cg, hb, tiles_m, tiles_n, sp, ks0, ks, spk};
+      }
+    }
+  }
+  return best;
+}
+
+template <int CG, int EPI, int TYPE, bool ROWS_K, bool SPLIT, bool PACKED>
 cudaError_t launch_t(const GemmParams& p, cudaStream_t st) {
-  using C = Cfg<CG>;
-  auto kern = gemm_kernel<CG, EPI, TYPE, BN_MAJOR>;
+  using C = Cfg<PACKED>;
+  auto kern = gemm_kernel<CG, EPI, TYPE, ROWS_K, SPLIT, PACKED>;
   cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (err != cudaSuccess) return err;
-  const int64_t most = kSms / CG;
+  const int ctas = SPLIT ? CG * p.splits : CG;
+  const int most = SPLIT ? p.units : kSms / CG;  // a split tile has its cluster to itself
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((p.units < most ? p.units : most) * CG));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3((unsigned)((p.units < most ? p.units : most) * ctas));
+  cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   int n = 0;
-  if (CG == 2) {
+  if (ctas > 1) {
     attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = 2;
+    attr[n].val.clusterDim.x = ctas;
     attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
     ++n;
   }
@@ -686,55 +968,66 @@ cudaError_t launch_t(const GemmParams& p, cudaStream_t st) {
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  err = cudaLaunchKernelEx(&cfg, kern, p);
-  if (err != cudaSuccess || p.splits == 1) return err;
-  const int64_t threads = p.M * ((p.N + 7) / 8);
-  return launch_k(reduce_kernel<EPI, TYPE>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, p);
+  return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
+template <int CG, int EPI, int TYPE, bool ROWS_K>
+cudaError_t launch_s(const GemmParams& p, cudaStream_t st) {
+  if constexpr (CG == 2)
+    if (p.wide) return launch_t<CG, EPI, TYPE, ROWS_K, false, false>(p, st);
+  return p.splits > 1 ? launch_t<CG, EPI, TYPE, ROWS_K, true, true>(p, st)
+                      : launch_t<CG, EPI, TYPE, ROWS_K, false, true>(p, st);
+}
 template <int CG, int TYPE>
-cudaError_t launch_e(const GemmParams& p, int epi, bool n_major, cudaStream_t st) {
-  if (epi == kEpiGated) return launch_t<CG, kEpiGated, TYPE, false>(p, st);
-  if (epi == kEpiGatedBackward) return launch_t<CG, kEpiGatedBackward, TYPE, true>(p, st);
-  return n_major ? launch_t<CG, kEpiPlain, TYPE, true>(p, st) : launch_t<CG, kEpiPlain, TYPE, false>(p, st);
+cudaError_t launch_e(const GemmParams& p, int epi, bool rows_k, cudaStream_t st) {
+  if (epi == kEpiGated) return launch_s<CG, kEpiGated, TYPE, false>(p, st);
+  if (epi == kEpiGatedBackward) return launch_s<CG, kEpiGatedBackward, TYPE, true>(p, st);
+  return rows_k ? launch_s<CG, kEpiPlain, TYPE, true>(p, st) : launch_s<CG, kEpiPlain, TYPE, false>(p, st);
 }
 
 }  // namespace
 
-size_t dense_partial_bytes(int64_t M, int N, int K, int pairs, bool gated) {
-  const Plan q = plan(M, N, K, pairs, gated);
-  return q.splits == 1 ? 0 : (size_t)q.splits * M * q.tiles_n * kBN * sizeof(float);
-}
-
 cudaError_t launch_dense_gemm(const DenseGemm& g, cudaStream_t st) {
-  const bool gated = g.epilogue == kEpiGated;
-  if (g.b_rows_k ? gated : g.epilogue == kEpiGatedBackward) return cudaErrorInvalidValue;
-  const Plan q = plan(g.M, g.N, g.K, g.pairs, gated);
+  const bool gated = g.epilogue == kEpiGated, wide = g.wide[0] != nullptr;
+  if (wide && g.M <= kBM) return cudaErrorInvalidValue;
+  if (g.rows_k ? gated : g.epilogue == kEpiGatedBackward) return cudaErrorInvalidValue;
+  const Plan q = plan(g.M, g.N, g.K, g.pairs, gated, g.rows_k, wide);
   GemmParams p;
   p.M = g.M;
   p.N = g.N;
+  p.rows = g.rows_k ? g.K : g.N;
+  const int cols = g.rows_k ? g.N : g.K;
+  p.s_pitch = cols / g.group;
+  p.lg = g.group == 32 ? 5 : g.group == 64 ? 6 : 7;
   p.gated = gated;
+  p.hb = q.hb;
   p.ks0 = q.ks0;
   p.ks = q.ks;
   p.tiles_m = q.tiles_m;
-  p.tiles_n = q.tiles_n;
   p.splits = q.splits;
   p.spk = q.spk;
-  p.units = (int64_t)q.tiles_m * q.tiles_n * q.splits;
-  p.partial = g.partial;
+  if ((int64_t)q.tiles_m * q.tiles_n * 8 > INT32_MAX / 2) return cudaErrorInvalidValue;
+  p.units = q.tiles_m * q.tiles_n;
+  p.wide = wide;
+  p.early = g.early;
   p.e = g.e;
-  if (q.splits > 1 && g.partial_bytes < (size_t)q.splits * g.M * q.tiles_n * kBN * sizeof(float))
-    return cudaErrorInvalidValue;
+  const auto t16 = g.type == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   for (int i = 0; i < 2; ++i) {
-    const int ai = g.pairs > 1 ? i : 0, bi = (g.pairs > 1 || gated) ? i : 0;
-    cudaError_t err = encode(&p.a[i], g.a[ai], g.M, g.K, g.lda[ai], kBM, g.type);
-    if (err == cudaSuccess)
-      err = g.b_rows_k ? encode(&p.b[i], g.b[bi], g.K, g.N, g.ldb[bi], kBK, g.type)
-                       : encode(&p.b[i], g.b[bi], g.N, g.K, g.ldb[bi], 128, g.type);
+    const int ai = g.pairs > 1 ? i : 0, wi = (g.pairs > 1 || gated) ? i : 0;
+    cudaError_t err = cudaSuccess;
+    if (i == 0 || ai) err = encode(&p.a[i], t16, g.a[ai], g.M, g.K, g.lda * 2, kBK, kBM, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (err == cudaSuccess && (i == 0 || wi))
+      err = wide ? encode(&p.w[i], t16, g.wide[wi], p.rows, cols, (int64_t)cols * 2, kBK, g.rows_k ? kBK : q.hb,
+                          CU_TENSOR_MAP_SWIZZLE_128B)
+                 : encode(&p.w[i], CU_TENSOR_MAP_DATA_TYPE_UINT32, g.w[wi].w, p.rows, cols / 8, (int64_t)cols / 2, 8,
+                          g.rows_k ? kBK : q.hb, CU_TENSOR_MAP_SWIZZLE_NONE);
     if (err != cudaSuccess) return err;
+    if (i && !ai) p.a[1] = p.a[0];
+    if (i && !wi) p.w[1] = p.w[0];
+    p.q[i] = {g.w[wi].s, g.w[wi].b};
   }
-  if (g.type == kF16) return q.cg == 2 ? launch_e<2, kF16>(p, g.epilogue, g.b_rows_k, st) : launch_e<1, kF16>(p, g.epilogue, g.b_rows_k, st);
-  return q.cg == 2 ? launch_e<2, kBf16>(p, g.epilogue, g.b_rows_k, st) : launch_e<1, kBf16>(p, g.epilogue, g.b_rows_k, st);
+  if (g.type == kF16) return q.cg == 2 ? launch_e<2, kF16>(p, g.epilogue, g.rows_k, st) : launch_e<1, kF16>(p, g.epilogue, g.rows_k, st);
+  return q.cg == 2 ? launch_e<2, kBf16>(p, g.epilogue, g.rows_k, st) : launch_e<1, kBf16>(p, g.epilogue, g.rows_k, st);
 }
 
 cudaError_t dense_status(int32_t* status, cudaStream_t st) {

@@ -283,14 +283,14 @@ def _ffn_forward(cfg, wts, x, residual, save):
         g = torch.empty((*x.shape[:-1], cfg.inter), dtype=x.dtype, device=x.device)
         u = torch.empty_like(g)
     need = _ffn_workspace(cfg.hidden, cfg.inter, cfg.group_size, cfg.dtype, T, 0)
-    ws = _workspace(need, x.device)
+    ws = _workspace(need, x.device) if need else None
     ctx = _context(fn, x)
     with ctx.lock:
         ctx.bind_stream(_raw_stream(ctx.device))
         rc = library().moe_gated_ffn_forward(ctx.handle, cfg, wts, x.data_ptr(), T,
                                              None if residual is None else residual.data_ptr(),
                                              g.data_ptr() if save else None, u.data_ptr() if save else None,
-                                             out.data_ptr(), ws.data_ptr(), need)
+                                             out.data_ptr(), ws.data_ptr() if need else None, need)
         ctx.check(fn, rc)
     return (out, g, u) if save else out
 
@@ -302,12 +302,13 @@ def _ffn_backward(cfg, wts, g, u, dy):
     _like(fn, "up", u, (*dy.shape[:-1], cfg.inter), dy)
     dx, dgate, dup = torch.empty_like(dy), torch.empty_like(g), torch.empty_like(u)
     need = _ffn_workspace(cfg.hidden, cfg.inter, cfg.group_size, cfg.dtype, T, 1)
-    ws = _workspace(need, dy.device)
+    ws = _workspace(need, dy.device) if need else None
     ctx = _context(fn, dy)
     with ctx.lock:
         ctx.bind_stream(_raw_stream(ctx.device))
         rc = library().moe_gated_ffn_backward(ctx.handle, cfg, wts, g.data_ptr(), u.data_ptr(), dy.data_ptr(), T,
-                                              dgate.data_ptr(), dup.data_ptr(), dx.data_ptr(), ws.data_ptr(), need)
+                                              dgate.data_ptr(), dup.data_ptr(), dx.data_ptr(),
+                                              ws.data_ptr() if need else None, need)
         ctx.check(fn, rc)
     return dx, dgate, dup
 

@@ -36,7 +36,9 @@ QMM = [  # M, N, K, group, dtype, biases
     (9, 129, 640, 128, F16, True), (16, 33, 4096, 64, F16, True), (17, 96, 5632, 32, BF16, True),
     (31, 511, 512, 32, F16, False), (33, 300, 352, 32, BF16, True), (64, 257, 1024, 128, BF16, True),
     (127, 1000, 256, 64, F16, True), (128, 512, 704, 64, F16, True), (129, 513, 736, 32, BF16, True),
-    (300, 1408, 2048, 128, BF16, False), (1000, 2048, 768, 32, BF16, True)]
+    (300, 1408, 2048, 128, BF16, False), (1000, 2048, 768, 32, BF16, True),
+    (1100, 700, 416, 32, BF16, True), (2049, 513, 256, 128, F16, False), (1024, 66001, 512, 64, F16, True),
+    (200, 2048, 8192, 32, BF16, True)]
 
 
 @pytest.mark.parametrize("M,N,K,g,dt,biases", QMM)
@@ -55,7 +57,8 @@ def test_quantized_matmul(M, N, K, g, dt, biases):
 
 @pytest.mark.parametrize("M,K,N,g,dt,biases", [
     (1, 2048, 2048, 64, BF16, True), (5, 33, 64, 64, BF16, True), (32, 1001, 128, 128, F16, False),
-    (130, 100, 352, 32, F16, True), (512, 5632, 2048, 32, BF16, True), (257, 768, 1408, 64, BF16, False)])
+    (130, 100, 352, 32, F16, True), (512, 5632, 2048, 32, BF16, True), (257, 768, 1408, 64, BF16, False),
+    (1030, 520, 320, 64, F16, True), (1025, 99, 256, 128, BF16, True), (130, 8192, 544, 32, F16, True)])
 def test_quantized_matmul_not_transposed(M, K, N, g, dt, biases):
     from mlx_rs_b200 import ops
     gen = _gen(M, K, N)
@@ -101,7 +104,8 @@ FFN = [  # T, H, I, group, dtype, act
     (1, 2048, 5632, 64, BF16, "silu"), (1, 32, 32, 32, F16, "gelu"), (2, 256, 128, 128, BF16, "gelu"),
     (8, 2048, 1792, 32, F16, "gelu"), (9, 96, 1120, 32, BF16, "silu"), (32, 704, 320, 64, BF16, "silu"),
     (33, 384, 256, 128, F16, "silu"), (128, 192, 448, 64, F16, "gelu"), (129, 2048, 768, 128, BF16, "silu"),
-    (333, 1024, 736, 32, BF16, "gelu"), (700, 640, 1408, 64, BF16, "silu")]
+    (333, 1024, 736, 32, BF16, "gelu"), (700, 640, 1408, 64, BF16, "silu"),
+    (1025, 256, 352, 32, F16, "silu"), (2500, 384, 640, 128, BF16, "gelu")]
 
 
 def _ffn_case(T, H, I, g, dt):
@@ -282,12 +286,12 @@ def test_c_entry_refusals_launch_nothing():
     t = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
     p = t.data_ptr()
     q = lib.moe_quantized_matmul_ex
-    need = C.c_size_t()
-    assert lib.moe_quantized_matmul_workspace(0, 200, 64, 64, 1, 32, 4, C.byref(need)) == 0 and need.value > 0
-    assert q(ctx.handle, 0, p, 200, 64, p, p, p, 64, 1, 32, 4, p, p, need.value - 1) == 1
+    need = C.c_size_t()  # rows of 33 elements are copied to rows of 40
+    assert lib.moe_quantized_matmul_workspace(0, 200, 33, 64, 0, 32, 4, C.byref(need)) == 0 and need.value >= 200 * 80
+    assert q(ctx.handle, 0, p, 200, 33, p, p, p, 64, 0, 32, 4, p, p, need.value - 1) == 1
     assert b"workspace" in lib.moe_last_error(ctx.handle)
-    assert q(ctx.handle, 0, p, 200, 64, p, p, p, 64, 1, 32, 4, p, None, 0) == 1
-    assert q(ctx.handle, 0, p, 200, 64, p, p, p, 64, 1, 32, 4, p, p + 16, need.value) == 1
+    assert q(ctx.handle, 0, p, 200, 33, p, p, p, 64, 0, 32, 4, p, None, 0) == 1
+    assert q(ctx.handle, 0, p, 200, 33, p, p, p, 64, 0, 32, 4, p, p + 16, need.value) == 1
     assert q(ctx.handle, 0, p + 2, 1, 64, p, p, p, 64, 1, 32, 4, p, p, 1 << 16) == 1
     assert q(ctx.handle, 0, p, 1, 64, p, p + 2, p, 64, 1, 32, 4, p, p, 1 << 16) == 1
     assert q(ctx.handle, 0, p, 1, 64, None, p, p, 64, 1, 32, 4, p, p, 1 << 16) == 1
