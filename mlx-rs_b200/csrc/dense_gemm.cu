@@ -7,9 +7,9 @@
 // columns), weights its columns; K runs in steps of 64.
 //   warp 20     streams the token tile with TMA (128 rows x 128 bytes, swizzled);
 //   warp 22     streams the packed tiles with TMA into a ring of their own;
-//   warps 4-19  four groups, taking the K steps in turn: 16 bytes of packed weights (32 weights,
-//               within one quantization group) per thread and item become four 16-byte
-//               pieces of the B tile, w = RN16(s q + b) (one rounding: a tcgen05 product
+//   warps 4-19  four groups, taking the K steps in turn: a thread turns the 64 weights of one row
+//               (32 bytes packed, one or two quantization groups) into eight 16-byte pieces
+//               of the B tile, w = RN16(s q + b) (one rounding: a tcgen05 product
 //               takes both operands in one 16-bit type). With the rows summed, a word's eight
 //               weights are neighbours along N and the tile is MN-major; the addresses are
 //               the same in both layouts, only the meaning of a row differs;
@@ -231,70 +231,73 @@ MOE_DEV void tmem_ld16(uint32_t taddr, float (&r)[16]) {
 }
 MOE_DEV void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 
-// ---- eight consecutive elements of a 16-bit row, at column c of n (vec: rows are 16-byte
+// ---- W (4 or 8) consecutive elements of a 16-bit row, at column c of n (vec: rows of 16-byte
 // aligned multiples of 8; otherwise element by element, columns beyond n left alone)
-template <int TYPE>
-MOE_DEV void load8(const uint16_t* row, int c, int n, bool vec, float (&v)[8]) {
+template <int TYPE, int W>
+MOE_DEV void load_n(const uint16_t* row, int c, int n, bool vec, float (&v)[W]) {
   if (vec) {
-    const uint4 q = *reinterpret_cast<const uint4*>(row + c);
-    v[0] = Elem<TYPE>::lo(q.x), v[1] = Elem<TYPE>::hi(q.x), v[2] = Elem<TYPE>::lo(q.y), v[3] = Elem<TYPE>::hi(q.y);
-    v[4] = Elem<TYPE>::lo(q.z), v[5] = Elem<TYPE>::hi(q.z), v[6] = Elem<TYPE>::lo(q.w), v[7] = Elem<TYPE>::hi(q.w);
+    uint32_t q[W / 2];
+    if constexpr (W == 8) *reinterpret_cast<uint4*>(q) = *reinterpret_cast<const uint4*>(row + c);
+    else *reinterpret_cast<uint2*>(q) = *reinterpret_cast<const uint2*>(row + c);
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) v[2 * i] = Elem<TYPE>::lo(q[i]), v[2 * i + 1] = Elem<TYPE>::hi(q[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < n ? Elem<TYPE>::to_f(row[c + i]) : 0.0f;
+    for (int i = 0; i < W; ++i) v[i] = c + i < n ? Elem<TYPE>::to_f(row[c + i]) : 0.0f;
   }
 }
-template <int TYPE>
-MOE_DEV void store8(uint16_t* row, int c, int n, bool vec, const float (&v)[8]) {
-  uint32_t q[4];
+template <int TYPE, int W>
+MOE_DEV void store_n(uint16_t* row, int c, int n, bool vec, const float (&v)[W]) {
+  uint32_t q[W / 2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = Elem<TYPE>::pack(v[2 * i], v[2 * i + 1]);
+  for (int i = 0; i < W / 2; ++i) q[i] = Elem<TYPE>::pack(v[2 * i], v[2 * i + 1]);
   if (vec) {
-    *reinterpret_cast<uint4*>(row + c) = make_uint4(q[0], q[1], q[2], q[3]);
+    if constexpr (W == 8) *reinterpret_cast<uint4*>(row + c) = make_uint4(q[0], q[1], q[2], q[3]);
+    else *reinterpret_cast<uint2*>(row + c) = make_uint2(q[0], q[1]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < W; ++i)
       if (c + i < n) row[c + i] = (uint16_t)(i & 1 ? q[i >> 1] >> 16 : q[i >> 1] & 0xffffu);
   }
 }
 
-// The epilogues on eight columns [c, c + 8) of token m (c < n). d: the sums; in the gated
-// form the gate's, with u the up projection's.
-template <int EPI, int TYPE>
-MOE_DEV void epilogue8(const DenseEpi& e, int64_t m, int c, int n, bool vec, float (&d)[8], const float (&u)[8]) {
+// The epilogues on columns [c, c + W) of token m (c < n). d: the sums; in the gated form the
+// gate's, with u the up projection's.
+template <int EPI, int TYPE, int W>
+MOE_DEV void epilogue_n(const DenseEpi& e, int64_t m, int c, int n, bool vec, float (&d)[W], const float (&u)[W]) {
   const int64_t off = m * e.ldo;
   if constexpr (EPI == kEpiPlain) {
     if (e.residual) {
-      float r[8];
-      load8<TYPE>(e.residual + off, c, n, vec, r);
+      float r[W];
+      load_n<TYPE, W>(e.residual + off, c, n, vec, r);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) d[i] += r[i];
+      for (int i = 0; i < W; ++i) d[i] += r[i];
     }
-    store8<TYPE>(e.out + off, c, n, vec, d);
+    store_n<TYPE, W>(e.out + off, c, n, vec, d);
   } else if constexpr (EPI == kEpiGated) {
     // g and u stay in fp32 up to h, which is rounded once (the down projection's operand)
     if (e.gate) {
-      store8<TYPE>(e.gate + off, c, n, vec, d);
-      store8<TYPE>(e.up + off, c, n, vec, u);
+      store_n<TYPE, W>(e.gate + off, c, n, vec, d);
+      store_n<TYPE, W>(e.up + off, c, n, vec, u);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) d[i] = act_val(d[i], e.act) * u[i];
-    store8<TYPE>(e.out + off, c, n, vec, d);
+    for (int i = 0; i < W; ++i) d[i] = act_val(d[i], e.act) * u[i];
+    store_n<TYPE, W>(e.out + off, c, n, vec, d);
   } else {
     // d = dh: dup = dh act(g), dgate = dh u act'(g), each rounded once
-    float g[8], up[8];
-    load8<TYPE>(e.gate + off, c, n, vec, g);
-    load8<TYPE>(e.up + off, c, n, vec, up);
+    float g[W], up[W];
+    load_n<TYPE, W>(e.gate + off, c, n, vec, g);
+    load_n<TYPE, W>(e.up + off, c, n, vec, up);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < W; ++i) {
       float val, grad;
       act_grad(g[i], e.act, val, grad);
       const float dh = d[i];
       g[i] = dh * up[i] * grad;
       up[i] = dh * val;
     }
-    store8<TYPE>(e.dgate + off, c, n, vec, g);
-    store8<TYPE>(e.dup + off, c, n, vec, up);
+    store_n<TYPE, W>(e.dgate + off, c, n, vec, g);
+    store_n<TYPE, W>(e.dup + off, c, n, vec, up);
   }
 }
 
@@ -455,13 +458,16 @@ __global__ void __launch_bounds__(Cfg<PACKED>::kThreads, 1) gemm_kernel(const __
 
   if (warp == kTmaWarp) {
     if (lane == 0) {
-      int it = 0;
+      int it = 0, s = 0;
+      uint32_t phase = 1;
       bool ok = true;
       for (int unit = first; ok && unit < p.units; unit += stride) {
         const int m0 = (tile_m(unit) * CG + rank) * kBM;
+        const int n = half_row(tile_n(unit), 0);
+        int pr = k0 >= p.ks0 ? 1 : 0, x = (k0 - (pr ? p.ks0 : 0)) * kBK;
         for (int k = k0; k < k1; ++k, ++it) {
-          const int s = it % kStages;
-          if (!mbar_wait(bar_empty + 8 * s, ((it / kStages) & 1) ^ 1, &gone)) {
+          if (k == p.ks0) pr = 1, x = 0;
+          if (!mbar_wait(bar_empty + 8 * s, phase, &gone)) {
             gone = 1;
             atomicOr(&g_dense_status, 1);
             ok = false;
@@ -470,18 +476,18 @@ __global__ void __launch_bounds__(Cfg<PACKED>::kThreads, 1) gemm_kernel(const __
           uint32_t bar = bar_full + 8 * s;
           if (rank == 0) mbar_expect_tx(bar, PACKED ? CG * kATile : CG * (kATile + p.hb * 128));
           if constexpr (CG == 2) bar = map_rank(bar, leader);
-          const int pr = k >= p.ks0 ? 1 : 0;
-          const int x = (k - (pr ? p.ks0 : 0)) * kBK;
-          tma_2d<CG>(sbase + s * kStageBytes, &p.a[pr], x, m0, bar);
+          const uint32_t dst = sbase + s * kStageBytes;
+          tma_2d<CG>(dst, &p.a[pr], x, m0, bar);
           if constexpr (!PACKED) {
-            const uint32_t dst = sbase + s * kStageBytes + kATile;
-            const int n = half_row(tile_n(unit), 0);
             if constexpr (ROWS_K) {  // boxes of 64 rows x 64 columns
-              for (int b = 0; b < p.hb / 64; ++b) tma_2d<CG>(dst + b * (kBTile / 2), &p.w[pr], n + 64 * b, x, bar);
+              tma_2d<CG>(dst + kATile, &p.w[pr], n, x, bar);
+              if (p.hb == 128) tma_2d<CG>(dst + kATile + kBTile / 2, &p.w[pr], n + 64, x, bar);
             } else {                 // hb rows x 64 columns
-              tma_2d<CG>(dst, &p.w[p.gated ? rank : pr], x, n, bar);
+              tma_2d<CG>(dst + kATile, &p.w[p.gated ? rank : pr], x, n, bar);
             }
           }
+          x += kBK;
+          if (++s == kStages) s = 0, phase ^= 1;
         }
       }
       // no copy may still be landing, and no MMA's arrival still be under way, when the CTA
@@ -519,10 +525,11 @@ __global__ void __launch_bounds__(Cfg<PACKED>::kThreads, 1) gemm_kernel(const __
           const int kk = k - (pr ? p.ks0 : 0);
 #pragma unroll
           for (int h = 0; h < kHalves; ++h) {
-            const uint32_t dst = sbase + kPackAt + s * kPackBytes + h * (kPackBytes / 2);
+            const uint32_t dst = sbase + kPackAt + s * kPackBytes + h * p.hb * 32;
             const int n = half_row(nt, h);
             if constexpr (ROWS_K) {  // boxes of 64 rows x 64 columns
-              for (int b = 0; b < p.hb / 64; ++b) tma_2d<1>(dst + b * 2048, &p.w[pr], n / 8 + b * 8, kk * kBK, bar);
+              tma_2d<1>(dst, &p.w[pr], n / 8, kk * kBK, bar);
+              if (CG == 2 && p.hb == 128) tma_2d<1>(dst + 2048, &p.w[pr], n / 8 + 8, kk * kBK, bar);
             } else {                 // hb rows x 64 columns
               tma_2d<1>(dst, &p.w[p.gated ? (CG == 2 ? rank : h) : pr], kk * 8, n, bar);
             }
@@ -539,61 +546,55 @@ __global__ void __launch_bounds__(Cfg<PACKED>::kThreads, 1) gemm_kernel(const __
    if constexpr (PACKED) {
     // ---- dequantisation: group wg takes steps wg, wg + kGroups, ... of this CTA's sequence
     const int wg = (warp - kDeqWarp) >> 2, wt = tid - (kDeqWarp + 4 * wg) * 32;
-    // Item i of a thread: 32 columns (wt % 2) of row wt / 2 of 64: rows 64 i.. of this CTA's
-    // half (CG = 2), or half i (CG = 1). With ROWS_K the 64 rows are the summed ones, and i
-    // is the block of 64 columns.
-    constexpr int kItems = 2;
-    auto item_half = [](int i) { return CG == 2 ? 0 : i; };
-    auto item_row = [](int i) { return CG == 2 ? 64 * i : 0; };
-    const int j = wt & 1, r0 = wt >> 1;
+    // A thread owns one row of 64 weights of the tile (128 bytes of it, eight words packed):
+    // row wt of this CTA's weight rows (both halves when CG = 1); with ROWS_K row wt % 64 of
+    // the step, in the block wt / 64 of 64 columns. Two groups of weights at group size 32.
     const int per = k1 - k0;
     const int total = first < p.units ? (int)((p.units - first + stride - 1) / stride) * per : 0;
+    const bool mine = wt < kHalves * p.hb;
+    const int half = CG == 1 && wt >= p.hb ? 1 : 0;
+    const bool two = p.lg == 5;
     // The scales and biases of the group's next two steps, read ahead: at_k walks the steps,
     // the pointers are those of its tile and operand pair.
-    const uint16_t* ps[kItems];
-    const uint16_t* pb[kItems];
-    uint32_t valid = 0;
+    const uint16_t* ps = nullptr;
+    const uint16_t* pb = nullptr;
+    bool valid = false, second = false;
     int at_unit = first, at_k = k0 + wg, at_key = -1;
     while (at_k >= k1) at_k -= per, at_unit += stride;
-    auto read_scales = [&](uint32_t (&vs)[kItems], uint32_t (&vb)[kItems]) {
-#pragma unroll
-      for (int i = 0; i < kItems; ++i) vs[i] = vb[i] = 0u;
+    auto read_scales = [&](uint32_t (&vs)[2], uint32_t (&vb)[2]) {
+      vs[0] = vs[1] = vb[0] = vb[1] = 0u;
       if (at_unit < p.units) {
         const int pr = at_k >= p.ks0 ? 1 : 0;
         if (at_key != 2 * at_unit + pr) {
           at_key = 2 * at_unit + pr;
-          valid = 0;
-          const int nt = tile_n(at_unit);
-#pragma unroll
-          for (int i = 0; i < kItems; ++i) {
-            const int n = half_row(nt, item_half(i)) + item_row(i) + (ROWS_K ? 32 * j : r0);
-            const WeightSide& q = p.q[p.gated ? (CG == 2 ? rank : i) : pr];
-            const int64_t off = ROWS_K ? (int64_t)r0 * p.s_pitch + (n >> p.lg) : (int64_t)n * p.s_pitch;
-            const bool in = n < p.N && item_row(i) + (ROWS_K ? 0 : r0) < p.hb;
-            valid |= in ? 1u << i : 0u;
-            ps[i] = q.s + (in ? off : 0);
-            pb[i] = q.b ? q.b + (in ? off : 0) : nullptr;
-          }
+          const int n = half_row(tile_n(at_unit), half) + (ROWS_K ? (CG == 2 ? wt & 64 : 0) : wt - half * p.hb);
+          const WeightSide& q = p.q[p.gated ? (CG == 2 ? rank : half) : pr];
+          valid = mine && n < p.N;
+          second = valid && two && (!ROWS_K || n + 32 < p.N);
+          const int64_t off = !valid ? 0 : ROWS_K ? (int64_t)(wt & 63) * p.s_pitch + (n >> p.lg) : (int64_t)n * p.s_pitch;
+          ps = q.s + off;
+          pb = q.b ? q.b + off : nullptr;
         }
         const int kk = at_k - (pr ? p.ks0 : 0);
-        const int g = (kk * kBK + 32 * j) >> p.lg;
+        const int g = (kk * kBK) >> p.lg;
         const int64_t off = ROWS_K ? (int64_t)(kk * kBK) * p.s_pitch : g;
-        const bool in = ROWS_K ? kk * kBK + r0 < p.rows : g < p.s_pitch;
-        if (in) {
-#pragma unroll
-          for (int i = 0; i < kItems; ++i)
-            if (valid >> i & 1) {
-              vs[i] = ldg_u16(ps[i] + off);
-              if (pb[i]) vb[i] = ldg_u16(pb[i] + off);
-            }
+        const bool in = ROWS_K ? kk * kBK + (wt & 63) < p.rows : true;  // the first group of a step exists
+        if (valid && in) {
+          vs[0] = ldg_u16(ps + off);
+          if (pb) vb[0] = ldg_u16(pb + off);
+        }
+        if (second && in && (ROWS_K || g + 1 < p.s_pitch)) {
+          vs[1] = ldg_u16(ps + off + 1);
+          if (pb) vb[1] = ldg_u16(pb + off + 1);
         }
       }
       at_k += kGroups;
       while (at_k >= k1) at_k -= per, at_unit += stride;
     };
-    uint32_t rs[2][kItems], rb[2][kItems];
+    uint32_t rs[2][2], rb[2][2];
     read_scales(rs[0], rb[0]);
     read_scales(rs[1], rb[1]);
+    const uint32_t to = (uint32_t)wt * 128;
     bool ok = true;
     for (int it = wg; ok && it < total; it += 2 * kGroups) {
 #pragma unroll
@@ -602,11 +603,10 @@ __global__ void __launch_bounds__(Cfg<PACKED>::kThreads, 1) gemm_kernel(const __
         if (step >= total) break;
         const int s = step % kStages, sl = step % kSlots;
         bool ready = mbar_wait(bar_pfull + 8 * sl, (step / kSlots) & 1, &gone);
-        uint4 q[kItems];
+        uint4 q0, q1;
         if (__all_sync(0xffffffffu, ready)) {
-#pragma unroll
-          for (int i = 0; i < kItems; ++i)
-            q[i] = lds16(sbase + kPackAt + sl * kPackBytes + (128 * i + wt) * 16);
+          const uint32_t src = sbase + kPackAt + sl * kPackBytes + wt * 32;
+          q0 = lds16(src), q1 = lds16(src + 16);
           ready = mbar_wait(bar_empty + 8 * s, ((step / kStages) & 1) ^ 1, &gone);
         }
         if (!__all_sync(0xffffffffu, ready)) {
@@ -615,23 +615,25 @@ __global__ void __launch_bounds__(Cfg<PACKED>::kThreads, 1) gemm_kernel(const __
           ok = false;
           break;
         }
-        const uint32_t bt = sbase + s * kStageBytes + kATile;
+        if (mine) {
+          const uint32_t row = sbase + s * kStageBytes + kATile + to;
+          const uint32_t s2 = __byte_perm(rs[sub][0], 0, 0x1010), b2 = __byte_perm(rb[sub][0], 0, 0x1010);
+          const uint32_t* w = &q0.x;
 #pragma unroll
-        for (int i = 0; i < kItems; ++i) {
-          if (item_row(i) + (ROWS_K ? 0 : r0) >= p.hb) continue;
-          const uint32_t s2 = __byte_perm(rs[sub][i], 0, 0x1010), b2 = __byte_perm(rb[sub][i], 0, 0x1010);
-          // rows of 128 bytes; the second half (CG = 1) follows the first hb of them
-          const uint32_t row = bt + (uint32_t)(CG == 2 ? 64 * i : p.hb * i) * 128 + r0 * 128;
-          const uint32_t* w = &q[i].x;
+          for (int c = 0; c < 4; ++c) sts16(row + (((uint32_t)c ^ (wt & 7)) << 4), dequant8<TYPE>(w[c], s2, b2));
+          const uint32_t s3 = two ? __byte_perm(rs[sub][1], 0, 0x1010) : s2;
+          const uint32_t b3 = two ? __byte_perm(rb[sub][1], 0, 0x1010) : b2;
+          const uint32_t* v = &q1.x;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            sts16(row + (((uint32_t)(4 * j + c) ^ (r0 & 7)) << 4), dequant8<TYPE>(w[c], s2, b2));
+          for (int c = 0; c < 4; ++c) sts16(row + (((uint32_t)(4 + c) ^ (wt & 7)) << 4), dequant8<TYPE>(v[c], s3, b3));
         }
         fence_proxy();
         __syncwarp();
         // the packed words are in use by now: only here may their slot be filled again
-        if (lane == 0) mbar_arrive(bar_pempty + 8 * sl);
-        if (lane == 0) mbar_arrive_cluster(CG == 2 ? map_rank(bar_full + 8 * s, leader) : bar_full + 8 * s);
+        if (lane == 0) {
+          mbar_arrive(bar_pempty + 8 * sl);
+          mbar_arrive_cluster(CG == 2 ? map_rank(bar_full + 8 * s, leader) : bar_full + 8 * s);
+        }
         read_scales(rs[sub], rb[sub]);
       }
     }
@@ -694,10 +696,33 @@ __global__ void __launch_bounds__(Cfg<PACKED>::kThreads, 1) gemm_kernel(const __
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t stage = sbase + kStagingAt + warp * kStageBuf;
     const int chunks = (EPI == kEpiGated ? p.hb : 2 * p.hb) / 16;  // of 16 output columns
+    // chunks of gate / up (residual) fetched ahead: the first ones before the accumulator is ready
+    constexpr int kAhead = PACKED ? 1 : 2;
     int tile = 0;
     for (int unit = first; unit < p.units; unit += stride, ++tile) {
       const int nt = tile_n(unit);
       const int buf = tile & 1;
+      const uint32_t acc = tmem + buf * 256 + lanes;
+      const int64_t mrow = (int64_t)(tile_m(unit) * CG + rank) * kBM + quad * 32;  // the warp's first row
+      const int rows = p.M - mrow < 32 ? (int)(p.M - mrow) : 32;  // may be <= 0
+      const int64_t ld = p.e.ldo;
+      const int n0 = EPI == kEpiGated ? nt * p.hb : nt * 2 * p.hb;
+      TileRegs tg[kAhead], tu[kAhead];
+      auto fetch = [&](int q, int slot) {
+        if (q >= chunks) return;
+        const int n = n0 + 16 * q;
+        const int64_t at = mrow * ld + n;
+        if constexpr (EPI == kEpiGatedBackward) {
+          fetch_tile(tg[slot], p.e.gate + at, ld, rows, p.N - n, lane);
+          fetch_tile(tu[slot], p.e.up + at, ld, rows, p.N - n, lane);
+        } else if constexpr (EPI == kEpiPlain) {
+          if (p.e.residual) fetch_tile(tg[slot], p.e.residual + at, ld, rows, p.N - n, lane);
+        }
+      };
+      if (!SPLIT && vec) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) fetch((warp >> 2) + i * kChunkStep, i);
+      }
       const bool ready = mbar_wait(bar_accf + 8 * buf, (tile >> 1) & 1, &gone);
       if (!__all_sync(0xffffffffu, ready)) {
         gone = 1;
@@ -705,8 +730,6 @@ __global__ void __launch_bounds__(Cfg<PACKED>::kThreads, 1) gemm_kernel(const __
         break;
       }
       tc_after();
-      const uint32_t acc = tmem + buf * 256 + lanes;
-      const int64_t mrow = (int64_t)(tile_m(unit) * CG + rank) * kBM + quad * 32;  // the warp's first row
       if constexpr (SPLIT) {
         // the sums into this CTA's shared memory (the stages are free: every MMA has completed)
         for (int q = warp >> 2; q < 2 * p.hb / 16; q += kChunkStep) {
@@ -720,72 +743,62 @@ __global__ void __launch_bounds__(Cfg<PACKED>::kThreads, 1) gemm_kernel(const __
                                            __float_as_uint(d[4 * i + 2]), __float_as_uint(d[4 * i + 3])));
         }
       } else {
-        const int rows = p.M - mrow < 32 ? (int)(p.M - mrow) : 32;  // may be <= 0
-        const int64_t ld = p.e.ldo;
-        const int n0 = EPI == kEpiGated ? nt * p.hb : nt * 2 * p.hb;
-        TileRegs tg, tu;
-        auto fetch = [&](int q) {
-          const int n = n0 + 16 * q;
-          const int64_t at = mrow * ld + n;
-          if constexpr (EPI == kEpiGatedBackward) {
-            fetch_tile(tg, p.e.gate + at, ld, rows, p.N - n, lane);
-            fetch_tile(tu, p.e.up + at, ld, rows, p.N - n, lane);
-          } else if constexpr (EPI == kEpiPlain) {
-            if (p.e.residual) fetch_tile(tg, p.e.residual + at, ld, rows, p.N - n, lane);
-          }
-        };
-        if (vec) fetch(warp >> 2);
 #pragma unroll 1
-        for (int q = warp >> 2; q < chunks; q += kChunkStep) {
-          const int n = n0 + 16 * q;
-          float d[16], u[16];
-          tmem_ld16(acc + 16 * q, d);
-          if constexpr (EPI == kEpiGated) tmem_ld16(acc + p.hb + 16 * q, u);
-          tmem_wait_ld();
-          if (!vec) {  // rows of any length: element by element
-            if (lane < rows) {
+        for (int q0 = warp >> 2; q0 < chunks; q0 += kAhead * kChunkStep) {
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                float(&d8)[8] = *reinterpret_cast<float(*)[8]>(d + 8 * i);
-                const float(&u8)[8] = *reinterpret_cast<float(*)[8]>((EPI == kEpiGated ? u : d) + 8 * i);
-                if (n + 8 * i < p.N) epilogue8<EPI, TYPE>(p.e, mrow + lane, n + 8 * i, p.N, false, d8, u8);
+          for (int slot = 0; slot < kAhead; ++slot) {
+            const int q = q0 + slot * kChunkStep;
+            if (q >= chunks) break;
+            const int n = n0 + 16 * q;
+            float d[16], u[16];
+            tmem_ld16(acc + 16 * q, d);
+            if constexpr (EPI == kEpiGated) tmem_ld16(acc + p.hb + 16 * q, u);
+            tmem_wait_ld();
+            if (!vec) {  // rows of any length: element by element
+              if (lane < rows) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  float(&d8)[8] = *reinterpret_cast<float(*)[8]>(d + 8 * i);
+                  const float(&u8)[8] = *reinterpret_cast<float(*)[8]>((EPI == kEpiGated ? u : d) + 8 * i);
+                  if (n + 8 * i < p.N) epilogue_n<EPI, TYPE, 8>(p.e, mrow + lane, n + 8 * i, p.N, false, d8, u8);
+                }
               }
+              continue;
             }
-            continue;
-          }
-          const int64_t at = mrow * ld + n;
-          const int cols = p.N - n;
-          if constexpr (EPI == kEpiPlain) {
-            if (p.e.residual) {
-              turn_tile<TYPE>(stage, tg, u, lane);
-              if (q + kChunkStep < chunks) fetch(q + kChunkStep);
+            const int64_t at = mrow * ld + n;
+            const int cols = p.N - n;
+            if constexpr (EPI == kEpiPlain) {
+              if (p.e.residual) {
+                turn_tile<TYPE>(stage, tg[slot], u, lane);
+                fetch(q + kAhead * kChunkStep, slot);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) d[i] += u[i];
-            }
-            store_tile<TYPE>(stage, d, p.e.out + at, ld, rows, cols, lane);
-          } else if constexpr (EPI == kEpiGated) {
-            // g and u stay in fp32 up to h, which is rounded once
-            if (p.e.gate) {
-              store_tile<TYPE>(stage, d, p.e.gate + at, ld, rows, cols, lane);
-              store_tile<TYPE>(stage, u, p.e.up + at, ld, rows, cols, lane);
-            }
+                for (int i = 0; i < 16; ++i) d[i] += u[i];
+              }
+              store_tile<TYPE>(stage, d, p.e.out + at, ld, rows, cols, lane);
+            } else if constexpr (EPI == kEpiGated) {
+              // g and u stay in fp32 up to h, which is rounded once
+              if (p.e.gate) {
+                store_tile<TYPE>(stage, d, p.e.gate + at, ld, rows, cols, lane);
+                store_tile<TYPE>(stage, u, p.e.up + at, ld, rows, cols, lane);
+              }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) d[i] = act_val(d[i], p.e.act) * u[i];
-            store_tile<TYPE>(stage, d, p.e.out + at, ld, rows, cols, lane);
-          } else {
-            float g[16];
-            turn_tile<TYPE>(stage, tg, g, lane);
-            turn_tile<TYPE>(stage, tu, u, lane);
-            if (q + kChunkStep < chunks) fetch(q + kChunkStep);
+              for (int i = 0; i < 16; ++i) d[i] = act_val(d[i], p.e.act) * u[i];
+              store_tile<TYPE>(stage, d, p.e.out + at, ld, rows, cols, lane);
+            } else {
+              float g[16];
+              turn_tile<TYPE>(stage, tg[slot], g, lane);
+              turn_tile<TYPE>(stage, tu[slot], u, lane);
+              fetch(q + kAhead * kChunkStep, slot);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float val, grad;
-              act_grad(g[i], p.e.act, val, grad);
-              g[i] = d[i] * u[i] * grad;
-              d[i] *= val;
+              for (int i = 0; i < 16; ++i) {
+                float val, grad;
+                act_grad(g[i], p.e.act, val, grad);
+                g[i] = d[i] * u[i] * grad;
+                d[i] *= val;
+              }
+              store_tile<TYPE>(stage, g, p.e.dgate + at, ld, rows, cols, lane);
+              store_tile<TYPE>(stage, d, p.e.dup + at, ld, rows, cols, lane);
             }
-            store_tile<TYPE>(stage, g, p.e.dgate + at, ld, rows, cols, lane);
-            store_tile<TYPE>(stage, d, p.e.dup + at, ld, rows, cols, lane);
           }
         }
       }
@@ -803,39 +816,33 @@ __global__ void __launch_bounds__(Cfg<PACKED>::kThreads, 1) gemm_kernel(const __
       const int r1 = r0 + slice < kBM ? r0 + slice : kBM;
       const int nt = tile_n(first);
       const int n0 = EPI == kEpiGated ? nt * p.hb : nt * 2 * p.hb;
-      const int groups = (EPI == kEpiGated ? p.hb : 2 * p.hb) / 8;
+      // four columns per thread: a warp's reads from another CTA cover whole 128-byte lines
+      // (eight columns in two reads with gaps took three times as long)
+      const int groups = (EPI == kEpiGated ? p.hb : 2 * p.hb) / 4;
       const bool vec = ((p.N | p.e.ldo) & 7) == 0;
       for (int i = tid; i < (r1 - r0) * groups; i += C::kThreads) {
-        const int r = r0 + i / groups, c = (i % groups) * 8;
+        const int r = r0 + i / groups, c = (i % groups) * 4;
         const int64_t m = (int64_t)(tile_m(first) * CG + rank) * kBM + r;
         if (m >= p.M || n0 + c >= p.N) continue;
-        float d[8] = {}, u[8] = {};
-        constexpr int kVecs = EPI == kEpiGated ? 4 : 2;
-        constexpr int kFly = EPI == kEpiGated ? 2 : 4;  // splits' pieces in flight
-        for (int sp = 0; sp < p.splits; sp += kFly) {
-          float4 v[kFly][kVecs];
+        float d[4] = {}, u[4] = {};
+        const uint32_t mine = sbase + (uint32_t)(r * kSumPitch + c) * 4;
+        for (int sp = 0; sp < p.splits; sp += 4) {  // four splits' pieces in flight
+          float4 v[4], w[4];
 #pragma unroll
-          for (int s = 0; s < kFly; ++s)
+          for (int s = 0; s < 4; ++s)
             if (sp + s < p.splits) {
-              const uint32_t src = map_rank(sbase + (uint32_t)(r * kSumPitch + c) * 4, (uint32_t)((sp + s) * CG + rank));
-              v[s][0] = lds_cluster(src), v[s][1] = lds_cluster(src + 16);
-              if constexpr (EPI == kEpiGated)
-                v[s][2] = lds_cluster(src + p.hb * 4), v[s][3] = lds_cluster(src + p.hb * 4 + 16);
+              const uint32_t src = map_rank(mine, (uint32_t)((sp + s) * CG + rank));
+              v[s] = lds_cluster(src);
+              if constexpr (EPI == kEpiGated) w[s] = lds_cluster(src + p.hb * 4);
             }
 #pragma unroll
-          for (int s = 0; s < kFly; ++s)
+          for (int s = 0; s < 4; ++s)
             if (sp + s < p.splits) {
-              const float* x = &v[s][0].x;
-#pragma unroll
-              for (int e = 0; e < 8; ++e) d[e] += x[e];
-              if constexpr (EPI == kEpiGated) {
-                const float* y = &v[s][2].x;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) u[e] += y[e];
-              }
+              d[0] += v[s].x, d[1] += v[s].y, d[2] += v[s].z, d[3] += v[s].w;
+              if constexpr (EPI == kEpiGated) u[0] += w[s].x, u[1] += w[s].y, u[2] += w[s].z, u[3] += w[s].w;
             }
         }
-        epilogue8<EPI, TYPE>(p.e, m, n0 + c, p.N, vec, d, u);
+        epilogue_n<EPI, TYPE, 4>(p.e, m, n0 + c, p.N, vec, d, u);
       }
     }
     __syncwarp();
