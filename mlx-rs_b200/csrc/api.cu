@@ -1483,8 +1483,8 @@ int moe_ctx_status(moe_ctx* ctx, int32_t* status) {
   *status = 0;
   DeviceGuard g(ctx->device);
   if (!g.ok) return fail(ctx, MOE_ERR_CUDA, "cudaSetDevice(%d) failed", ctx->device);
-  int32_t dense = 0;  // the dense operators' kernels share one word per device
-  MOE_CUDA(ctx, moe::dense_status(&dense, ctx->stream));
+  int32_t dense = 0;  // the dense operators' products share one word per device
+  MOE_CUDA(ctx, moe::dense_gemm_status(&dense, ctx->stream));
   if (ctx->scratch) {
     MOE_CUDA(ctx, cudaMemcpyAsync(status, ctx->scratch, sizeof(int32_t), cudaMemcpyDeviceToHost, ctx->stream));
     MOE_CUDA(ctx, cudaStreamSynchronize(ctx->stream));

@@ -218,7 +218,7 @@ int moe_quantized_matmul_ex(moe_ctx* ctx, int dtype, const void* x, int64_t M, i
   if (!g.ok) return fail(ctx, MOE_ERR_CUDA, "%s: cudaSetDevice failed", fn);
   const cudaStream_t st = static_cast<cudaStream_t>(moe_internal::ctx_stream(ctx));
 
-  if (transpose && M <= moe::kQmvMaxM) {
+  if (transpose && moe::qmv_fits(M, N, K, false)) {
     moe::QmvArgs a{};
     a.x = static_cast<const uint16_t*>(x);
     a.m[0] = packed(q, N, K);
@@ -308,7 +308,9 @@ int moe_gated_ffn_forward(moe_ctx* ctx, const moe_ffn_config* cfg, const moe_ffn
   const cudaStream_t st = static_cast<cudaStream_t>(moe_internal::ctx_stream(ctx));
   const int H = cfg->hidden, I = cfg->inter;
 
-  if (T <= moe::kQmvMaxM) {
+  Wide wide;
+  DENSE_CUDA(ctx, fn, widen(cfg, wts, ws, workspace, wide, st));
+  if (moe::qmv_fits(T, I, H, true)) {
     moe::QmvArgs a{};
     a.x = static_cast<const uint16_t*>(x);
     a.m[0] = packed(wts->gate, I, H);
@@ -323,6 +325,29 @@ int moe_gated_ffn_forward(moe_ctx* ctx, const moe_ffn_config* cfg, const moe_ffn
     a.up = static_cast<uint16_t*>(up);
     a.act = cfg->activation;
     DENSE_CUDA(ctx, fn, moe::launch_qmv(a, true, st));
+  } else {
+    moe::DenseGemm gu{};
+    gu.a[0] = static_cast<const uint16_t*>(x);
+    gu.w[0] = packed(wts->gate, I, H);
+    gu.w[1] = packed(wts->up, I, H);
+    gu.wide[0] = wide.gate;
+    gu.wide[1] = wide.up;
+    gu.lda = H;
+    gu.pairs = 1;
+    gu.M = T;
+    gu.N = I;
+    gu.K = H;
+    gu.group = cfg->group_size;
+    gu.type = cfg->dtype;
+    gu.epilogue = moe::kEpiGated;
+    gu.e.out = h;
+    gu.e.ldo = I;
+    gu.e.gate = static_cast<uint16_t*>(gate);
+    gu.e.up = static_cast<uint16_t*>(up);
+    gu.e.act = cfg->activation;
+    DENSE_CUDA(ctx, fn, moe::launch_dense_gemm(gu, st));
+  }
+  if (moe::qmv_fits(T, H, I, false)) {
     moe::QmvArgs d{};
     d.x = h;
     d.m[0] = packed(wts->down, H, I);
@@ -335,48 +360,25 @@ int moe_gated_ffn_forward(moe_ctx* ctx, const moe_ffn_config* cfg, const moe_ffn
     d.residual = static_cast<const uint16_t*>(residual);
     d.early = 1;
     DENSE_CUDA(ctx, fn, moe::launch_qmv(d, false, st));
-    return MOE_OK;
+  } else {
+    moe::DenseGemm dn{};
+    dn.a[0] = h;
+    dn.w[0] = packed(wts->down, H, I);
+    dn.wide[0] = wide.down;
+    dn.lda = I;
+    dn.pairs = 1;
+    dn.M = T;
+    dn.N = H;
+    dn.K = I;
+    dn.group = cfg->group_size;
+    dn.type = cfg->dtype;
+    dn.early = 1;
+    dn.epilogue = moe::kEpiPlain;
+    dn.e.out = static_cast<uint16_t*>(out);
+    dn.e.ldo = H;
+    dn.e.residual = static_cast<const uint16_t*>(residual);
+    DENSE_CUDA(ctx, fn, moe::launch_dense_gemm(dn, st));
   }
-  Wide wide;
-  DENSE_CUDA(ctx, fn, widen(cfg, wts, ws, workspace, wide, st));
-  moe::DenseGemm gu{};
-  gu.a[0] = static_cast<const uint16_t*>(x);
-  gu.w[0] = packed(wts->gate, I, H);
-  gu.w[1] = packed(wts->up, I, H);
-  gu.wide[0] = wide.gate;
-  gu.wide[1] = wide.up;
-  gu.lda = H;
-  gu.pairs = 1;
-  gu.M = T;
-  gu.N = I;
-  gu.K = H;
-  gu.group = cfg->group_size;
-  gu.type = cfg->dtype;
-  gu.epilogue = moe::kEpiGated;
-  gu.e.out = h;
-  gu.e.ldo = I;
-  gu.e.gate = static_cast<uint16_t*>(gate);
-  gu.e.up = static_cast<uint16_t*>(up);
-  gu.e.act = cfg->activation;
-  DENSE_CUDA(ctx, fn, moe::launch_dense_gemm(gu, st));
-
-  moe::DenseGemm dn{};
-  dn.a[0] = h;
-  dn.w[0] = packed(wts->down, H, I);
-  dn.wide[0] = wide.down;
-  dn.lda = I;
-  dn.pairs = 1;
-  dn.M = T;
-  dn.N = H;
-  dn.K = I;
-  dn.group = cfg->group_size;
-  dn.type = cfg->dtype;
-  dn.early = 1;
-  dn.epilogue = moe::kEpiPlain;
-  dn.e.out = static_cast<uint16_t*>(out);
-  dn.e.ldo = H;
-  dn.e.residual = static_cast<const uint16_t*>(residual);
-  DENSE_CUDA(ctx, fn, moe::launch_dense_gemm(dn, st));
   return MOE_OK;
 }
 

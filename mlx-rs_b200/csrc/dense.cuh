@@ -73,8 +73,8 @@ struct DenseGemm {
   DenseEpi e;
 };
 cudaError_t launch_dense_gemm(const DenseGemm& g, cudaStream_t st);
-// Device status word of the dense kernels on the current device (bounded waits).
-cudaError_t dense_status(int32_t* status, cudaStream_t st);
+// Device status word of these kernels on the current device (bounded waits that expired).
+cudaError_t dense_gemm_status(int32_t* status, cudaStream_t st);
 
 // ---- 4-bit products for few tokens (qmv.cu): out = x m[0]^T, or gated out = act(g) * u
 struct QmvArgs {
@@ -88,9 +88,10 @@ struct QmvArgs {
   uint16_t* up;
   int act;
   int early;                 // the weights may be read before the launch before has completed
+  int tiles;                 // set by launch_qmv
 };
-// Tokens up to which these kernels are used instead of dequantisation and dense_gemm.cu.
-constexpr int kQmvMaxM = 32;
+// Whether these kernels, and not dense_gemm.cu's, serve a product.
+bool qmv_fits(int64_t M, int64_t N, int64_t K, bool gated);
 cudaError_t launch_qmv(const QmvArgs& a, bool gated, cudaStream_t st);
 
 // ---- rotary positions (rope.cu)
@@ -111,7 +112,57 @@ struct RopeArgs {
 };
 cudaError_t launch_rope(const RopeArgs& a, cudaStream_t st);
 
-// ---- device helpers
+// ---- device helpers: mbarriers. Every wait is bounded (2 s): a kernel whose wait expires
+// records a code in its status word and runs to its end without waiting further.
+constexpr uint64_t kWaitLimitNs = 2000ull * 1000 * 1000;
+MOE_DEV uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+MOE_DEV void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count) : "memory");
+}
+MOE_DEV void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
+}
+MOE_DEV bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(1000u)
+      : "memory");
+  return ok != 0;
+}
+// Non-blocking (a try_wait may hold the thread until the phase completes).
+MOE_DEV bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+MOE_DEV uint64_t now_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(t));
+  return t;
+}
+// Bounded wait; false when it gave up. `gone` is the CTA's abort flag: once one role has
+// given up, the others stop waiting.
+MOE_DEV bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* gone) {
+  if (mbar_try(bar, parity)) return true;
+  const uint64_t t0 = now_ns();
+  while (!mbar_try(bar, parity))
+    if (*gone || now_ns() - t0 > kWaitLimitNs) return false;
+  return true;
+}
+MOE_DEV void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+
 template <int TYPE>
 struct Elem;  // conversions of the 16-bit element types
 template <>

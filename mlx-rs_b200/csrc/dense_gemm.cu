@@ -45,7 +45,6 @@ constexpr int kATile = kBM * kBK * 2;      // 16 KB
 constexpr int kBTile = 128 * kBK * 2;      // 16 KB: this CTA's weight rows of a tile, at most 128
 constexpr int kPackBytes = 128 * 32;       // 4 KB: their packed K step
 constexpr int kStageBuf = 1024;            // 32 rows x 16 columns of 16 bits, per epilogue warp
-constexpr uint64_t kWaitLimitNs = 2000ull * 1000 * 1000;
 constexpr int kSms = 148;
 
 __device__ int32_t g_dense_status;
@@ -100,53 +99,6 @@ struct GemmParams {
   DenseEpi e;
 };
 
-MOE_DEV uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-MOE_DEV void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count) : "memory");
-}
-MOE_DEV void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
-}
-MOE_DEV bool mbar_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.b32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity), "r"(1000u)
-      : "memory");
-  return ok != 0;
-}
-// Non-blocking (a try_wait may hold the thread until the phase completes).
-MOE_DEV bool mbar_test(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.b32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-MOE_DEV uint64_t now_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(t));
-  return t;
-}
-// Bounded wait; false when it gave up. `gone` is the CTA's abort flag: once one role has
-// given up, the others stop waiting.
-MOE_DEV bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* gone) {
-  if (mbar_try(bar, parity)) return true;
-  const uint64_t t0 = now_ns();
-  while (!mbar_try(bar, parity))
-    if (*gone || now_ns() - t0 > kWaitLimitNs) return false;
-  return true;
-}
-MOE_DEV void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
-}
 // The address of `a` in CTA `rank` of the cluster.
 MOE_DEV uint32_t map_rank(uint32_t a, uint32_t rank) {
   uint32_t r;
@@ -1037,7 +989,7 @@ cudaError_t launch_dense_gemm(const DenseGemm& g, cudaStream_t st) {
   return q.cg == 2 ? launch_e<2, kBf16>(p, g.epilogue, g.rows_k, st) : launch_e<1, kBf16>(p, g.epilogue, g.rows_k, st);
 }
 
-cudaError_t dense_status(int32_t* status, cudaStream_t st) {
+cudaError_t dense_gemm_status(int32_t* status, cudaStream_t st) {
   cudaError_t err = cudaMemcpyFromSymbolAsync(status, g_dense_status, sizeof(int32_t), 0, cudaMemcpyDeviceToHost, st);
   return err != cudaSuccess ? err : cudaStreamSynchronize(st);
 }

@@ -7,217 +7,329 @@
 // becomes the top mantissa bits under the exponent of 16). D and X are mma.sync products
 // with fp32 accumulators (X with a matrix of ones); the weights are never rounded.
 //
-// A CTA owns 16 weight rows (gated: 8 of gate and the same 8 of up, so that a thread holds
-// both projections of an element) and all of K: its warps take spans of 128 columns in turn,
-// add up in registers, and the CTA adds the warps' sums through shared memory in warp order.
-// Lane (g, t) reads 16 bytes (32 columns) of rows g and g + 8 straight into registers: four
-// lanes cover 64 contiguous bytes of a row, and every load of a batch is in flight before
-// the first is used. An MMA sums over the four lanes of a row, so all of its k must lie in
-// one group: the lanes first exchange words by shuffles (none at G = 128, one step at 64,
-// two at 32); the tokens are read to match (x is small and stays in L1), each 16-byte piece
-// permuted to the order in which the fields leave a word.
-// Bound by the bytes of W for up to 8 tokens; beyond, by the MMAs and the permutations of x
-// (8 tokens more share the weight fragments).
+// A CTA takes tiles of 16 weight rows (gated: 8 of gate and the same 8 of up, so that a thread
+// holds both projections of an element), one after the other, and all of K: its warps take
+// spans of 128 columns in turn, add up in registers, and the CTA adds the warps' sums through
+// shared memory in warp order. Each warp copies its spans (16 rows x 64 bytes) ahead with
+// cp.async into a ring of its own, across tile borders, so that the copies run under the
+// products. An MMA sums over the four lanes of a row, so all of its k must lie in one group:
+// lane (g, t) reads from the ring the words of rows g and g + 8 that make it so (16-byte piece
+// j of row r lies at piece j ^ swz(r): conflict-free for reads of 16, 8 and 4 bytes a lane).
+// The tokens are read to match (x is small and stays in L1), each 16-byte piece permuted to
+// the order in which the fields leave a word.
+// Bound by the instructions of a span (about 280 for 16 x 128 weights: 64 to extract the
+// fields, 16 MMAs) at the 20 warps per SM that 96 registers allow: one token, 2048 -> 32768
+// 16 us (2.2 TB/s), 2048 -> 11264 7.4 us, 5632 -> 2048 5.1 us, 2048 -> 2048 2.9 us. Measured
+// against it: a warp that does the copies of a CTA, bulk copies and scales through shared
+// memory (fewer instructions, but 1.5 us more before the first product: 2048 -> 2048 4.5 us),
+// 32 rows per warp (19.7 us for 2048 -> 32768), the span's tokens loaded ahead (19.2 us: the
+// registers), 24 warps of 80 registers (21 us).
+#include <algorithm>
+
 #include "dense.cuh"
 
 namespace moe {
 
 namespace {
 
-template <int TYPE>
+// d = a . b, or d += a . b (ADD)
+template <int TYPE, bool ADD>
 MOE_DEV void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  const float c0 = ADD ? d[0] : 0.0f, c1 = ADD ? d[1] : 0.0f, c2 = ADD ? d[2] : 0.0f, c3 = ADD ? d[3] : 0.0f;
   if constexpr (TYPE == kBf16)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
   else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
-MOE_DEV void swap_words(uint32_t& keep_lo, uint32_t& keep_hi, bool hi, int mask) {
-  // a lane with !hi gives keep_hi and takes the partner's keep_lo in its place; one with hi
-  // gives keep_lo and takes the partner's keep_hi
-  const uint32_t give = hi ? keep_lo : keep_hi;
-  const uint32_t got = __shfl_xor_sync(0xffffffffu, give, mask);
-  if (hi) keep_lo = got;
-  else keep_hi = got;
+// 16 bytes, or zeros
+MOE_DEV void copy16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
-
-// Words so that step i's four lanes hold words of one group (see word_of for which).
-template <int G>
-MOE_DEV void exchange(uint4& w, int t) {
-  if constexpr (G == 64) {
-    swap_words(w.x, w.z, t >= 2, 2);
-    swap_words(w.y, w.w, t >= 2, 2);
-  } else if constexpr (G == 32) {
-    swap_words(w.x, w.y, t & 1, 1);
-    swap_words(w.z, w.w, t & 1, 1);
-    swap_words(w.x, w.z, t >= 2, 2);
-    swap_words(w.y, w.w, t >= 2, 2);
+MOE_DEV uint32_t lds4(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+MOE_DEV uint2 lds8(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
+MOE_DEV uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+// GP consecutive scales into whole registers, so that nothing has to wait for them before
+// their use: in one access where every row allows it.
+template <int GP>
+MOE_DEV void ldg_scales(const uint16_t* p, bool wide, int have, uint32_t (&v)[GP]) {
+  if (GP == 1) {
+    asm volatile("ld.global.nc.u16 %0, [%1];\n" : "=r"(v[0]) : "l"(p));
+  } else if (wide) {  // v[i]: values 2 i and 2 i + 1
+    if constexpr (GP == 2) asm volatile("ld.global.nc.u32 %0, [%1];\n" : "=r"(v[0]) : "l"(p));
+    if constexpr (GP == 4) asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];\n" : "=r"(v[0]), "=r"(v[1]) : "l"(p));
+  } else {
+#pragma unroll
+    for (int i = 0; i < GP; ++i)
+      if (i < have) asm volatile("ld.global.nc.u16 %0, [%1];\n" : "=r"(v[i]) : "l"(p + i));
   }
 }
-template <int G>
-MOE_DEV int word_of(int t, int i) {
-  if constexpr (G == 128) return 4 * t + i;
-  if constexpr (G == 64) return 4 * ((t & 1) + (i & 2)) + (t & 2) + (i & 1);
-  return 4 * i + t;
+template <int TYPE, int GP>
+MOE_DEV float scale_of(const uint32_t (&v)[GP], bool wide, int i) {
+  const uint32_t x = GP > 1 && wide ? v[i >> 1] : v[i];
+  return GP > 1 && wide && (i & 1) ? Elem<TYPE>::hi(x) : Elem<TYPE>::lo(x);
 }
 
-MOE_DEV uint4 ldg16(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
+constexpr int kSms = 148;
+constexpr int kRing = 6;             // spans in flight per warp
+constexpr int kSpanBytes = 16 * 64;  // 16 rows x 128 weights
+
+MOE_DEV int swz(int row) { return ((row >> 1) & 1) * 2 | ((row >> 2) & 1); }
+MOE_DEV uint32_t piece_at(int row, int piece) { return (uint32_t)(row * 64 + ((piece ^ swz(row)) << 4)); }
+
+// This lane's words of row `row` of a span for the steps of a group.
+template <int G>
+MOE_DEV void row_words(uint32_t span, int row, int gr, int t, uint32_t (&w)[G / 32]) {
+  if constexpr (G == 128) {
+    *reinterpret_cast<uint4*>(w) = lds16(span + piece_at(row, t));
+  } else if constexpr (G == 64) {
+    *reinterpret_cast<uint2*>(w) = lds8(span + piece_at(row, 2 * gr + (t >> 1)) + (t & 1) * 8);
+  } else {
+    w[0] = lds4(span + piece_at(row, gr) + t * 4);
+  }
 }
 
 template <int TYPE, int G, bool GATED, int NC>
-__global__ void __launch_bounds__(512) qmv_kernel(const __grid_constant__ QmvArgs a) {
-  constexpr int GP = 128 / G;           // groups per span
-  constexpr int kBatch = NC == 1 ? 4 : 2;  // spans of weights in flight per warp
-  extern __shared__ float red[];        // [warps][16][8 NC]
+__global__ void __maxnreg__(NC == 4 ? 128 : 96) qmv_kernel(const __grid_constant__ QmvArgs a) {
+  constexpr int GP = 128 / G;      // groups per span
+  constexpr int kSteps = G / 32;   // words of a lane per group
+  constexpr int kCols = 8 * NC;
+  constexpr int kChains = NC == 1 ? 2 : 1;
+  extern __shared__ __align__(128) unsigned char smem[];  // [warps][kRing][1 KB] | [2][warps][16][kCols] floats
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int g = lane >> 2, t = lane & 3;
   const int K = a.K, spans = (K + 127) >> 7, groups = K / G;
-  const int64_t n0 = (int64_t)blockIdx.x * (GATED ? 8 : 16);
-  const int64_t last = a.N - 1;  // rows past the last read it again and are not stored
-  const int64_t r0 = n0 + g < last ? n0 + g : last;
-  const int64_t r1 = GATED ? r0 : (n0 + 8 + g < last ? n0 + 8 + g : last);
-  const PackedMatrix& m1 = GATED ? a.m[1] : a.m[0];
-  const uint32_t* w0 = a.m[0].w + r0 * (K >> 3) + t * 4;
-  const uint32_t* w1 = m1.w + r1 * (K >> 3) + t * 4;
-  const uint16_t* s0 = a.m[0].s + r0 * groups;
-  const uint16_t* s1 = m1.s + r1 * groups;
-  const uint16_t* b0 = a.m[0].b ? a.m[0].b + r0 * groups : nullptr;
-  const uint16_t* b1 = m1.b ? m1.b + r1 * groups : nullptr;
+  const int mine = (spans - warp + warps - 1) / warps;  // this warp's spans of a tile (warps <= spans)
+  const uint32_t ring = smem_u32(smem) + warp * (kRing * kSpanBytes), ring_end = ring + kRing * kSpanBytes;
+  float* red = reinterpret_cast<float*>(smem + warps * (kRing * kSpanBytes));
+  const int tiles = a.tiles, rows = (int)a.N;
+  const bool wide = groups % GP == 0;  // every row's scales start at a multiple of GP
 
-  uint4 wa[kBatch], wb[kBatch];
-  uint32_t sa[kBatch], sb[kBatch];  // scale | bias << 16 of group `span * GP + t` (t < GP)
-  auto load = [&](int base) {
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int s = base + i * warps;
-      const bool in = s < spans && s * 128 + t * 32 < K;
-      wa[i] = in ? ldg16(w0 + s * 16) : make_uint4(0, 0, 0, 0);
-      wb[i] = in ? ldg16(w1 + s * 16) : make_uint4(0, 0, 0, 0);
-      const int gi = s * GP + (GP == 1 ? 0 : t);
-      const bool sin = s < spans && (GP == 1 || t < GP) && gi < groups;
-      sa[i] = sin ? (uint32_t)__ldg(s0 + gi) | (b0 ? (uint32_t)__ldg(b0 + gi) << 16 : 0u) : 0u;
-      sb[i] = sin ? (uint32_t)__ldg(s1 + gi) | (b1 ? (uint32_t)__ldg(b1 + gi) << 16 : 0u) : 0u;
-    }
+  // this lane's rows of a tile, g and g + 8 (gated: row g of gate and of up). Rows past the
+  // last read it again and are not stored.
+  auto row_of = [&](int tile, int i) {
+    const int n = GATED ? tile * 8 + g : tile * 16 + g + 8 * i;
+    return n < rows ? n : rows - 1;
   };
+  auto mat = [&](int i) -> const PackedMatrix& { return a.m[GATED ? i : 0]; };
+
+  // ---- copies, span by span across tiles (lane (g, t): piece t of its rows)
+  int c_tile = blockIdx.x, c_i = 0;
+  uint32_t c_slot = ring;
+  uint32_t c_at[2];  // words into the matrix
+  auto copy_next = [&]() {
+    if (c_tile < tiles) {
+      if (c_i == 0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) c_at[i] = (uint32_t)row_of(c_tile, i) * (uint32_t)(K >> 3) + warp * 16 + t * 4;
+      }
+      const bool in = (warp + c_i * warps) * 128 + t * 32 < K;  // the last span may be short
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        copy16(c_slot + piece_at(g + 8 * i, t), mat(i).w + (in ? c_at[i] : 0u), in);
+        c_at[i] += warps * 16;
+      }
+      if (++c_i == mine) c_i = 0, c_tile += gridDim.x;
+    }
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+    c_slot += kSpanBytes;
+    if (c_slot == ring_end) c_slot = ring;
+  };
+  // ---- scales and biases of a span's groups, read one span ahead
+  int q_tile = blockIdx.x, q_i = 0;
+  uint32_t q_at[2];  // scales into the matrix
+  struct Scales {
+    uint32_t s[2][GP] = {}, b[2][GP] = {};
+  };
+  auto read_scales = [&](Scales& v) {
+    if (q_tile >= tiles) return;
+    if (q_i == 0) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) q_at[i] = (uint32_t)row_of(q_tile, i) * (uint32_t)groups + warp * GP;
+    }
+    const int have = groups - (warp + q_i * warps) * GP;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      ldg_scales<GP>(mat(i).s + q_at[i], wide, have, v.s[i]);
+      if (mat(i).b) ldg_scales<GP>(mat(i).b + q_at[i], wide, have, v.b[i]);
+      q_at[i] += warps * GP;
+    }
+    if (++q_i == mine) q_i = 0, q_tile += gridDim.x;
+  };
+
   // `early`: the launch before this one does not write the weights and let this one start
   // only after everything before it had completed (the second product of a block)
-  if (a.early) load(warp);
-  pdl_wait();
-  pdl_trigger();
-  if (!a.early) load(warp);
+  if (!a.early) {
+    pdl_wait();
+    pdl_trigger();
+  }
+#pragma unroll 1
+  for (int i = 0; i < kRing - 1; ++i) copy_next();
+  Scales ahead;
+  read_scales(ahead);
+  if (a.early) {
+    pdl_wait();
+    pdl_trigger();
+  }
 
-  const int mbase = blockIdx.y * (8 * NC);
+  // Columns of the MMA without a token read the last token again and are not stored.
+  const int mbase = blockIdx.y * kCols;
   const uint16_t* xr[NC];
-  bool xin[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int m = mbase + c * 8 + g;
-    xin[c] = m < a.M;
-    xr[c] = a.x + (int64_t)(xin[c] ? m : 0) * K;
+    constexpr int kLaneWords = G == 128 ? 4 : G == 64 ? 2 : 1;
+    xr[c] = a.x + (int64_t)(m < a.M ? m : a.M - 1) * K + warp * 128 + t * kLaneWords * 8;
   }
-  float acc[NC][4] = {};
-  for (int base = warp; base < spans; base += warps * kBatch) {
-    if (base != warp) load(base);
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int s = base + i * warps;
-      if (s >= spans) break;
-      exchange<G>(wa[i], t);
-      exchange<G>(wb[i], t);
-      const uint32_t* pa = &wa[i].x;
-      const uint32_t* pb = &wb[i].x;
+  uint32_t slot = ring;
+  int buf = 0;
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, buf ^= 1) {
+    float acc[NC][4] = {};
+    for (int i = 0; i < mine; ++i) {
+      copy_next();
+      asm volatile("cp.async.wait_group %0;\n" ::"n"(kRing - 1) : "memory");
+      __syncwarp();
+      const int xoff = i * warps * 128;
+      const int have = groups - (warp + i * warps) * GP;  // groups of this span
+      const Scales cur = ahead;
+      read_scales(ahead);
 #pragma unroll
       for (int gr = 0; gr < GP; ++gr) {
-        float d[NC][4] = {}, x1[NC][4] = {};
+        if (GP > 1 && gr >= have) break;
+        uint32_t w[2][kSteps];
 #pragma unroll
-        for (int j = 0; j < 4 / GP; ++j) {
-          const int step = gr * (4 / GP) + j;
-          const int col = (s * 16 + word_of<G>(t, step)) * 8;
-          const uint32_t u = pa[step], v = pb[step];
+        for (int r = 0; r < 2; ++r) row_words<G>(slot, g + 8 * r, gr, t, w[r]);
+        // two chains each for eight tokens, so that an MMA does not wait for the one before
+        float d[kChains][NC][4], x1[kChains][NC][4];
+        constexpr int kLast = kChains - 1;
+        constexpr uint32_t one = Nib<TYPE>::kOne;
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+          uint32_t e[NC][4];
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const uint4 q = __ldg(reinterpret_cast<const uint4*>(xr[c] + xoff + gr * G + j * 8));
+            e[c][0] = __byte_perm(q.x, q.z, 0x5410), e[c][1] = __byte_perm(q.x, q.z, 0x7632);
+            e[c][2] = __byte_perm(q.y, q.w, 0x5410), e[c][3] = __byte_perm(q.y, q.w, 0x7632);
+          }
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            if (j == 0) {
+              mma<TYPE, false>(x1[0][c], one, one, one, one, e[c][0], e[c][1]);
+              mma<TYPE, kChains == 1>(x1[kLast][c], one, one, one, one, e[c][2], e[c][3]);
+            } else {
+              mma<TYPE, true>(x1[0][c], one, one, one, one, e[c][0], e[c][1]);
+              mma<TYPE, true>(x1[kLast][c], one, one, one, one, e[c][2], e[c][3]);
+            }
+          }
+          const uint32_t u = w[0][j], v = w[1][j];
           const uint32_t u0 = fields<TYPE, 0>(u), u1 = fields<TYPE, 1>(u), u2 = fields<TYPE, 2>(u), u3 = fields<TYPE, 3>(u);
           const uint32_t v0 = fields<TYPE, 0>(v), v1 = fields<TYPE, 1>(v), v2 = fields<TYPE, 2>(v), v3 = fields<TYPE, 3>(v);
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
-            uint4 q = make_uint4(0, 0, 0, 0);
-            if (xin[c] && col < K) q = __ldg(reinterpret_cast<const uint4*>(xr[c] + col));
-            const uint32_t e0 = __byte_perm(q.x, q.z, 0x5410), e1 = __byte_perm(q.x, q.z, 0x7632);
-            const uint32_t e2 = __byte_perm(q.y, q.w, 0x5410), e3 = __byte_perm(q.y, q.w, 0x7632);
-            constexpr uint32_t one = Nib<TYPE>::kOne;
-            mma<TYPE>(d[c], u0, v0, u1, v1, e0, e1);
-            mma<TYPE>(x1[c], one, one, one, one, e0, e1);
-            mma<TYPE>(d[c], u2, v2, u3, v3, e2, e3);
-            mma<TYPE>(x1[c], one, one, one, one, e2, e3);
+            if (j == 0) {
+              mma<TYPE, false>(d[0][c], u0, v0, u1, v1, e[c][0], e[c][1]);
+              mma<TYPE, kChains == 1>(d[kLast][c], u2, v2, u3, v3, e[c][2], e[c][3]);
+            } else {
+              mma<TYPE, true>(d[0][c], u0, v0, u1, v1, e[c][0], e[c][1]);
+              mma<TYPE, true>(d[kLast][c], u2, v2, u3, v3, e[c][2], e[c][3]);
+            }
           }
         }
-        const int src = (lane & ~3) | gr;
-        const uint32_t qa = GP == 1 ? sa[i] : __shfl_sync(0xffffffffu, sa[i], src);
-        const uint32_t qb = GP == 1 ? sb[i] : __shfl_sync(0xffffffffu, sb[i], src);
-        const float sc0 = Elem<TYPE>::lo(qa), sc1 = Elem<TYPE>::lo(qb);
-        const float bi0 = __fmaf_rn(-16.0f, sc0, Elem<TYPE>::hi(qa)), bi1 = __fmaf_rn(-16.0f, sc1, Elem<TYPE>::hi(qb));
+        if constexpr (kChains == 2) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) d[0][0][k] += d[1][0][k];
+          x1[0][0][0] += x1[1][0][0], x1[0][0][1] += x1[1][0][1];
+        }
+        const float sc0 = scale_of<TYPE, GP>(cur.s[0], wide, gr), sc1 = scale_of<TYPE, GP>(cur.s[1], wide, gr);
+        const float bi0 = __fmaf_rn(-16.0f, sc0, scale_of<TYPE, GP>(cur.b[0], wide, gr));
+        const float bi1 = __fmaf_rn(-16.0f, sc1, scale_of<TYPE, GP>(cur.b[1], wide, gr));
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          acc[c][0] = __fmaf_rn(sc0, d[c][0], __fmaf_rn(bi0, x1[c][0], acc[c][0]));
-          acc[c][1] = __fmaf_rn(sc0, d[c][1], __fmaf_rn(bi0, x1[c][1], acc[c][1]));
-          acc[c][2] = __fmaf_rn(sc1, d[c][2], __fmaf_rn(bi1, x1[c][0], acc[c][2]));
-          acc[c][3] = __fmaf_rn(sc1, d[c][3], __fmaf_rn(bi1, x1[c][1], acc[c][3]));
+          acc[c][0] = __fmaf_rn(sc0, d[0][c][0], __fmaf_rn(bi0, x1[0][c][0], acc[c][0]));
+          acc[c][1] = __fmaf_rn(sc0, d[0][c][1], __fmaf_rn(bi0, x1[0][c][1], acc[c][1]));
+          acc[c][2] = __fmaf_rn(sc1, d[0][c][2], __fmaf_rn(bi1, x1[0][c][0], acc[c][2]));
+          acc[c][3] = __fmaf_rn(sc1, d[0][c][3], __fmaf_rn(bi1, x1[0][c][1], acc[c][3]));
         }
       }
+      // The slot is filled again by the copy that the next round issues: this warp's own, and
+      // every word above has gone into an MMA whose sum the line before waited for.
+      __syncwarp();
+      slot += kSpanBytes;
+      if (slot == ring_end) slot = ring;
     }
-  }
-  // ---- the warps' sums, in warp order
-  constexpr int kCols = 8 * NC;
+    // ---- the warps' sums, in warp order (two buffers: one barrier per tile)
+    float* rb = red + buf * (warps * 16 * kCols);
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    float* r = red + (warp * 16 + g) * kCols + c * 8 + 2 * t;
-    *reinterpret_cast<float2*>(r) = make_float2(acc[c][0], acc[c][1]);
-    *reinterpret_cast<float2*>(r + 8 * kCols) = make_float2(acc[c][2], acc[c][3]);
-  }
-  __syncthreads();
-  constexpr int kRows = GATED ? 8 : 16;
-  for (int i = threadIdx.x; i < kRows * kCols; i += blockDim.x) {
-    const int row = i % kRows, col = i / kRows;
-    const int64_t n = n0 + row;
-    const int m = mbase + col;
-    if (n >= a.N || m >= a.M) continue;
-    float v = 0.0f, u = 0.0f;
-    for (int w = 0; w < warps; ++w) {
-      v += red[(w * 16 + row) * kCols + col];
-      if (GATED) u += red[(w * 16 + 8 + row) * kCols + col];
+    for (int c = 0; c < NC; ++c) {
+      float* at = rb + (warp * 16 + g) * kCols + c * 8 + 2 * t;
+      *reinterpret_cast<float2*>(at) = make_float2(acc[c][0], acc[c][1]);
+      *reinterpret_cast<float2*>(at + 8 * kCols) = make_float2(acc[c][2], acc[c][3]);
     }
-    const int64_t at = (int64_t)m * a.N + n;
-    if constexpr (GATED) {
-      if (a.gate) {
-        a.gate[at] = (uint16_t)Elem<TYPE>::pack(v, 0.0f);
-        a.up[at] = (uint16_t)Elem<TYPE>::pack(u, 0.0f);
+    __syncthreads();
+    constexpr int kOut = GATED ? 8 : 16;
+    for (int i = threadIdx.x; i < kOut * kCols; i += blockDim.x) {
+      const int row = i % kOut, col = i / kOut;
+      const int n = tile * kOut + row;
+      const int m = mbase + col;
+      if (n >= rows || m >= a.M) continue;
+      float v = 0.0f, u = 0.0f;
+      for (int w = 0; w < warps; ++w) {
+        v += rb[(w * 16 + row) * kCols + col];
+        if (GATED) u += rb[(w * 16 + 8 + row) * kCols + col];
       }
-      v = act_val(v, a.act) * u;
-    } else if (a.residual) {
-      v += Elem<TYPE>::to_f(a.residual[at]);
+      const int64_t at = (int64_t)m * rows + n;
+      if constexpr (GATED) {
+        if (a.gate) {
+          a.gate[at] = (uint16_t)Elem<TYPE>::pack(v, 0.0f);
+          a.up[at] = (uint16_t)Elem<TYPE>::pack(u, 0.0f);
+        }
+        v = act_val(v, a.act) * u;
+      } else if (a.residual) {
+        v += Elem<TYPE>::to_f(a.residual[at]);
+      }
+      a.out[at] = (uint16_t)Elem<TYPE>::pack(v, 0.0f);
     }
-    a.out[at] = (uint16_t)Elem<TYPE>::pack(v, 0.0f);
   }
+  asm volatile("cp.async.wait_all;\n" ::: "memory");
 }
 
 template <int TYPE, int G, bool GATED, int NC>
-cudaError_t launch_nc(const QmvArgs& a, cudaStream_t st) {
-  const int64_t tiles = GATED ? (a.N + 7) / 8 : (a.N + 15) / 16;
+cudaError_t launch_nc(const QmvArgs& args, cudaStream_t st) {
+  QmvArgs a = args;
+  const int per_tile = GATED ? 8 : 16;
+  a.tiles = (int)((a.N + per_tile - 1) / per_tile);
   const int spans = (a.K + 127) / 128;
-  // warps per CTA: a warp takes up to four spans at once; more warps with fewer spans each
-  // while the tiles alone would not give the SMs 16 warps
-  int warps = 4;
-  while (warps < 16 && (spans > 4 * warps || (tiles * warps < 148 * 16 && spans > warps))) warps *= 2;
-  const dim3 grid((unsigned)tiles, (unsigned)((a.M + 8 * NC - 1) / (8 * NC)));
-  return launch_k(qmv_kernel<TYPE, G, GATED, NC>, grid, dim3(32 * warps), (size_t)warps * 16 * 8 * NC * sizeof(float),
-                  st, a);
+  // warps per CTA: four; more with fewer spans each while the tiles alone would not give the
+  // SMs 16 warps
+  int warps = spans < 4 ? spans : 4;
+  while (warps < 16 && a.tiles * warps < kSms * 16 && spans >= 2 * warps) warps *= 2;
+  const size_t smem = (size_t)warps * (kRing * kSpanBytes + 2 * 16 * 8 * NC * sizeof(float));
+  auto kern = qmv_kernel<TYPE, G, GATED, NC>;
+  cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (err != cudaSuccess) return err;
+  // CTAs that the SMs hold at once (20 warps of 96 registers, 227 KB of shared memory)
+  const int per_sm = std::max(1, std::min((NC == 4 ? 16 : 20) / warps, (int)((227 * 1024) / (smem + 1024))));
+  const int m_tiles = (a.M + 8 * NC - 1) / (8 * NC);
+  const int most = std::max(1, kSms * per_sm / m_tiles);
+  const dim3 grid((unsigned)std::min(a.tiles, most), (unsigned)m_tiles);
+  return launch_k(kern, grid, dim3(32 * warps), smem, st, a);
 }
 template <int TYPE, int G, bool GATED>
 cudaError_t launch_g(const QmvArgs& a, cudaStream_t st) {
@@ -234,7 +346,20 @@ cudaError_t launch_ty(const QmvArgs& a, cudaStream_t st) {
 
 }  // namespace
 
+bool qmv_fits(int64_t M, int64_t N, int64_t K, bool gated) {
+  // offsets into a matrix are 32-bit words
+  if (M > 32 || N >= (int64_t(1) << 30) || N * (K / 8) >= (int64_t(1) << 32)) return false;
+  // Up to eight tokens the weights' bytes count, and these kernels read them best. Above, a
+  // warp's MMAs and permutations of x do, and the tensor-memory products are faster once they
+  // have enough weights to work on (us here / there): 16 tokens, 2048 -> 11264 10.4 / 15,
+  // 2048 -> 32768 29 / 26; 32 tokens, 2048 -> 2048 6.7 / 9.1, 5632 -> 2048 10.9 / 12.9,
+  // 2048 -> 11264 23 / 15.
+  const int64_t weights = N * (gated ? 2 : 1) * K;
+  return M <= 8 || weights <= (int64_t(M <= 16 ? 48 : 12) << 20);
+}
+
 cudaError_t launch_qmv(const QmvArgs& a, bool gated, cudaStream_t st) {
+  if (!qmv_fits(a.M, a.N, a.K, gated)) return cudaErrorInvalidValue;
   if (a.type == kF16) return gated ? launch_ty<kF16, true>(a, st) : launch_ty<kF16, false>(a, st);
   return gated ? launch_ty<kBf16, true>(a, st) : launch_ty<kBf16, false>(a, st);
 }
