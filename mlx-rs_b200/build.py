@@ -1,7 +1,8 @@
-"""Build libmoe_b200.so (the C-ABI library) in-tree with nvcc for sm_100a.
+"""Build libmoe_b200.so (the C-ABI library) in-tree with nvcc for sm_100a, and _calls.so (the
+dense operators' calls from Python) with g++ against torch's headers.
 
 Usage: python mlx-rs_b200/build.py [--force] [--verbose]
-Objects go to mlx-rs_b200/_build/, the library to mlx-rs_b200/libmoe_b200.so.
+Objects go to mlx-rs_b200/_build/, the libraries to mlx-rs_b200/.
 """
 from __future__ import annotations
 
@@ -16,6 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libmoe_b200.so")
+CALLS = os.path.join(HERE, "_calls.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -72,7 +74,23 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None) -> str:
     if force or jobs or _stale(LIB, objs):
         cmd = [nvcc()] + ARCH + ["-shared", "-o", LIB] + objs + ["-lcudart"]
         run(cmd)
+    src = os.path.join(CSRC, "torch_calls.cpp")
+    if force or _stale(CALLS, [src] + [h for h in hdrs if h.startswith(INCLUDE)]):
+        run(calls_command(src))
     return LIB
+
+
+def calls_command(src: str):
+    import sysconfig
+
+    import torch
+    troot = os.path.dirname(os.path.abspath(torch.__file__))
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
+    inc = [os.path.join(troot, "include"), os.path.join(troot, "include", "torch", "csrc", "api", "include"),
+           os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    return ["g++", "-O2", "-fPIC", "-shared", "-std=c++17", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *[f"-I{d}" for d in inc], src, "-o", CALLS, f"-L{HERE}", "-l:libmoe_b200.so", f"-L{os.path.join(troot, 'lib')}",
+            "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
 
 
 if __name__ == "__main__":

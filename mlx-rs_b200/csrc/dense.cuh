@@ -7,6 +7,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "kernels.cuh"
 
@@ -111,6 +113,19 @@ struct RopeArgs {
   const float* freqs;    // [dims / 2] or null
 };
 cudaError_t launch_rope(const RopeArgs& a, cudaStream_t st);
+
+// Allows `kern` its dynamic shared memory, once per device (`done`: a static of the caller).
+template <class K>
+cudaError_t allow_smem(K kern, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return err;
+}
 
 // ---- device helpers: mbarriers. Every wait is bounded (2 s): a kernel whose wait expires
 // records a code in its status word and runs to its end without waiting further.

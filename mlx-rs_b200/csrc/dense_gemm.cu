@@ -903,7 +903,8 @@ template <int CG, int EPI, int TYPE, bool ROWS_K, bool SPLIT, bool PACKED>
 cudaError_t launch_t(const GemmParams& p, cudaStream_t st) {
   using C = Cfg<PACKED>;
   auto kern = gemm_kernel<CG, EPI, TYPE, ROWS_K, SPLIT, PACKED>;
-  cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  static std::atomic<uint64_t> done{0};
+  cudaError_t err = allow_smem(kern, C::kSmem, done);
   if (err != cudaSuccess) return err;
   const int ctas = SPLIT ? CG * p.splits : CG;
   const int most = SPLIT ? p.units : kSms / CG;  // a split tile has its cluster to itself

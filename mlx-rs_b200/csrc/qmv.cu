@@ -322,7 +322,8 @@ cudaError_t launch_nc(const QmvArgs& args, cudaStream_t st) {
   while (warps < 16 && a.tiles * warps < kSms * 16 && spans >= 2 * warps) warps *= 2;
   const size_t smem = (size_t)warps * (kRing * kSpanBytes + 2 * 16 * 8 * NC * sizeof(float));
   auto kern = qmv_kernel<TYPE, G, GATED, NC>;
-  cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> done{0};
+  cudaError_t err = allow_smem(kern, 16 * (kRing * kSpanBytes + 2 * 16 * 8 * NC * (int)sizeof(float)), done);
   if (err != cudaSuccess) return err;
   // CTAs that the SMs hold at once (20 warps of 96 registers, 227 KB of shared memory)
   const int per_sm = std::max(1, std::min((NC == 4 ? 16 : 20) / warps, (int)((227 * 1024) / (smem + 1024))));

@@ -25,6 +25,12 @@ import torch
 from ._lib import (ACT_GELU, ACT_SILU, DTYPE_BF16, DTYPE_F16, DTYPE_F32, FfnConfig, FfnWeights, MlxError, QWeight,
                    RopeConfig, context_for, library)
 
+try:  # the dense operators' calls without ctypes (build.py); what it declines is made here
+    from . import _calls
+    _calls.set_error(MlxError)
+except ImportError:
+    _calls = None
+
 _WORD_DTYPES = {torch.int32} | ({torch.uint32} if hasattr(torch, "uint32") else set())
 
 
@@ -147,8 +153,13 @@ def quantized_matmul(x, w, scales, biases=None, transpose=True, group_size=64, b
     """out[..., N] = x[..., K] @ dequant(w)^T (transpose=True), or x[..., K] @ dequant(w)
     for w [K, N*bits/32] (transpose=False: the gradient of the first with respect to x).
     bf16 or f16, group_size 32, 64 or 128, bits 4."""
-    if x.dtype != torch.bfloat16 or not transpose or group_size in (32, 128):
-        return _quantized_matmul_ex(x, w, scales, biases, transpose, group_size, bits)
+    if group_size != 64 or x.dtype != torch.bfloat16 or not transpose:
+        if _calls is not None and bits == 4:
+            out = _calls.quantized_matmul(x, w, scales, biases, transpose, group_size)
+            if out is not None:
+                return out
+        if group_size in (32, 64, 128) or x.dtype != torch.bfloat16 or not transpose:
+            return _quantized_matmul_ex(x, w, scales, biases, transpose, group_size, bits)
     _need(x, {torch.bfloat16}, "x")
     _need(w, _WORD_DTYPES, "w")
     _need(scales, {torch.bfloat16}, "scales")
@@ -276,6 +287,10 @@ def _like(fn, name, t, shape, x):
 
 def _ffn_forward(cfg, wts, x, residual, save):
     fn = "moe_gated_ffn_forward"
+    if _calls is not None:
+        r = _calls.ffn_forward(C.addressof(cfg), C.addressof(wts), x, residual, save)
+        if r is not None:
+            return r
     T = x.numel() // cfg.hidden
     out = torch.empty_like(x)
     g = u = None
@@ -297,6 +312,10 @@ def _ffn_forward(cfg, wts, x, residual, save):
 
 def _ffn_backward(cfg, wts, g, u, dy):
     fn = "moe_gated_ffn_backward"
+    if _calls is not None:
+        r = _calls.ffn_backward(C.addressof(cfg), C.addressof(wts), g, u, dy)
+        if r is not None:
+            return r
     T = dy.numel() // cfg.hidden
     _like(fn, "gate", g, (*dy.shape[:-1], cfg.inter), dy)
     _like(fn, "up", u, (*dy.shape[:-1], cfg.inter), dy)
@@ -342,6 +361,10 @@ def fast_rope(x, dims, traditional=False, base=10000.0, scale=1.0, offset=0, fre
     int, or an int32 / int64 tensor [B] with one offset per batch element. inverse: the
     transposed rotation, the gradient with respect to x. out: where to write, x itself
     included (default: a new contiguous tensor). bf16, f16 or f32."""
+    if out is None and _calls is not None:
+        r = _calls.fast_rope(x, dims, traditional, base, scale, offset, freqs, mscale, inverse)
+        if r is not None:
+            return r
     fn = "mlx_fast_rope"
     dt = _DTYPES.get(x.dtype)
     nd = x.dim()
