@@ -10,11 +10,13 @@
 // Bound by the bytes (one read and one write of the tensor). A CTA takes `tokens` positions
 // with all of their heads: it fills a table of cosines and sines in shared memory once, one
 // pair per thread, so that the 64-bit work is spread over the threads and shared by the heads,
-// then moves the heads through two vectors per thread. 36 heads of 128 bf16 channels out of a
-// fused projection: 4096 positions 15.4 us (4.9 TB/s), 8192 28.1 us (5.4 TB/s); one position of
-// 64 sequences 2.6 us. Measured against it: CTAs of 256 / 512 threads (17.6 / 22 us for 4096
-// positions: fewer of them in flight per SM), two or three items ahead per thread (15.7 / 18.2:
-// registers), 64-bit index arithmetic (20.7).
+// then moves the heads through two vectors per item, the loads of two items in flight.
+// 36 heads of 128 bf16 channels out of a fused projection: 4096 positions 15.8 us (4.8 TB/s),
+// 8192 30.9 us (4.9 TB/s); one position of 64 sequences 2.5 us; 2 x 1023 x 16 heads of 80, f32,
+// interleaved, 5.3 us. Measured against it, the same four in us: one item in flight 15.4, 28.1,
+// 2.5, 6.3; three 18.2, 36.1, 2.6, 7.1 (registers); one in flight as two named copies, with CTAs
+// of 128 threads 16.5, 31.0, 2.7, 6.3, of 256 17.5, 34.5, 2.4, 6.1, of 512 22.1, 36.6, 2.2, 7.7;
+// 64-bit index arithmetic 19.2, 33.1, 3.0, 6.6.
 #include "dense.cuh"
 
 namespace moe {
@@ -22,6 +24,7 @@ namespace moe {
 namespace {
 
 constexpr int kRopeThreads = 128;
+constexpr int kAhead = 2;  // items per thread whose loads are in flight
 
 template <int BYTES>
 struct Vec;
@@ -107,9 +110,11 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
 
   pdl_wait();
   pdl_trigger();
-  // the first item is on its way while the table is made, the next one while one is turned
-  Item cur;
-  if (threadIdx.x < total) fetch(threadIdx.x, cur);
+  // the first items are on their way while the table is made
+  Item ring[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    if (threadIdx.x + k * kRopeThreads < total) fetch(threadIdx.x + k * kRopeThreads, ring[k]);
   for (int i = threadIdx.x; i < here * half; i += kRopeThreads) {
     const int t = i / half, k = i - t * half;
     const uint32_t b = p.len(t0 + t), l = t0 + t - b * p.len.d;
@@ -126,9 +131,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
     table[i] = make_float2(a.mscale * c, a.mscale * a.sign * s);
   }
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < total; i += kRopeThreads) {
-    Item next;
-    if (i + kRopeThreads < total) fetch(i + kRopeThreads, next);
+  auto turn = [&](Item& cur) {
     if (cur.rot >= 0) {
       const float2* cs = table + cur.row + cur.rot;
       if constexpr (TYPE != kF32 && VE > 1) {  // two 16-bit channels of a word at a time
@@ -170,7 +173,16 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
     }
     *reinterpret_cast<V*>(ob + cur.o0) = cur.v0;
     if (cur.two) *reinterpret_cast<V*>(ob + cur.o1) = cur.v1;
-    cur = next;
+  };
+  for (uint32_t i = threadIdx.x; i < total; i += kAhead * kRopeThreads) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const uint32_t at = i + k * kRopeThreads;
+      if (at >= total) break;
+      Item cur = ring[k];
+      if (at + kAhead * kRopeThreads < total) fetch(at + kAhead * kRopeThreads, ring[k]);
+      turn(cur);
+    }
   }
 }
 
