@@ -97,7 +97,7 @@ QmmWs qmm_workspace(int64_t M, int64_t N, int64_t K, int transpose) {
   QmmWs w{};
   w.xpad = K % 8 ? up256((size_t)M * up8(K) * sizeof(uint16_t)) : 0;
   const int64_t piece = qmm_piece(N, K);
-  w.wide = M >= moe::kWideMinM && (transpose || piece == N);
+  w.wide = M >= (transpose ? moe::kWideMinM : moe::kWideMinRowsM) && (transpose || piece == N);
   w.total = w.xpad + (w.wide ? (size_t)piece * K * sizeof(uint16_t) : 0);
   return w;
 }
@@ -145,7 +145,7 @@ struct FfnWs {
 };
 FfnWs ffn_workspace(const moe_ffn_config* c, int64_t T, bool backward) {
   FfnWs w{};
-  w.wide = T >= moe::kWideMinM;
+  w.wide = T >= (backward ? moe::kWideMinRowsM : moe::kWideMinM);
   w.h = backward ? 0 : up256((size_t)T * c->inter * sizeof(uint16_t));
   w.each = w.wide ? up256((size_t)c->hidden * c->inter * sizeof(uint16_t)) : 0;
   w.total = w.h + 3 * w.each;

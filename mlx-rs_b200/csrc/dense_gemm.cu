@@ -870,10 +870,13 @@ struct Plan {
   int cg, hb, tiles_m, tiles_n, splits, ks0, ks, spk;
 };
 
-// Tile width and K split of a product: the pair that takes the fewest K steps' time over the
-// rounds of tiles. A step costs about 0.36 us at 256 columns and no less than 0.2 (the token
-// tile's bytes and the barriers); a tile's start and epilogue about 2 us, the exchange of a
-// split's sums 3 us. (512 tokens, 2048 -> 2 x 5632 gated: see the table of cases.)
+// Tile width and K split of a product: the pair that takes the least time over the rounds of
+// tiles, by a line fitted to every allowed pair of 16 products (64 to 800 tokens, 768 to 5632
+// summed, both directions). With r weight rows per CTA a K step costs 0.11 + 0.21 r / 64 us, a
+// round 4.5 us (its start and epilogue), the exchange of a split's sums 1 + 1.4 r / 64 us. The
+// pair taken is within 1.5 % of the fastest measured one for those 16, and within 3.4 % (0.3 %
+// in the mean) for 16 others that had no part in the fit (40 to 1500 tokens, 1024 to 7168
+// summed). Over 16-bit weights a step takes 0.36 us at 128 rows and no less than 0.2.
 Plan plan(int64_t M, int N, int K, int pairs, bool gated, bool rows_k, bool wide) {
   Plan best{};
   double least = 0;
@@ -888,8 +891,9 @@ Plan plan(int64_t M, int N, int K, int pairs, bool gated, bool rows_k, bool wide
       if ((ks + spk - 1) / spk != sp) continue;  // no empty split
       const int64_t slots = resident_clusters(cg * sp);
       const double rounds = (double)(((int64_t)tiles_m * tiles_n + slots - 1) / slots);
-      const double step = std::max(0.2, 0.36 * (cg == 2 ? hb : 2 * hb) / 128);
-      const double t = rounds * (spk * step + 2.0) + (sp > 1 ? 3.0 : 0.0);
+      const double r = (cg == 2 ? hb : 2 * hb) / 64.0;
+      const double t = wide ? rounds * (spk * std::max(0.2, 0.18 * r) + 2.0)
+                            : rounds * (spk * (0.11 + 0.21 * r) + 4.5 + (sp > 1 ? 1.0 + 1.4 * r : 0.0));
       if (best.cg == 0 || t < least * 0.98) {
         least = t;
         best = Plan{cg, hb, tiles_m, tiles_n, sp, ks0, ks, spk};

@@ -38,7 +38,7 @@ QMM = [  # M, N, K, group, dtype, biases
     (127, 1000, 256, 64, F16, True), (128, 512, 704, 64, F16, True), (129, 513, 736, 32, BF16, True),
     (300, 1408, 2048, 128, BF16, False), (1000, 2048, 768, 32, BF16, True),
     (1100, 700, 416, 32, BF16, True), (2049, 513, 256, 128, F16, False), (1024, 66001, 512, 64, F16, True),
-    (200, 2048, 8192, 32, BF16, True)]
+    (200, 2048, 8192, 32, BF16, True), (2050, 66001, 512, 64, F16, True), (1024, 300, 256, 32, BF16, True)]
 
 
 @pytest.mark.parametrize("M,N,K,g,dt,biases", QMM)
