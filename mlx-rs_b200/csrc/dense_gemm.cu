@@ -94,6 +94,7 @@ struct GemmParams {
   int ks0, ks;          // K steps of the first operand pair, of all
   int tiles_m, splits, spk;
   int units;            // tiles
+  int a_rows;           // token rows of a box: all 128 of a tile, or those of the only tile
   int wide;             // the weights are 16-bit (w maps them), not packed
   int early;            // the weights may be read before the launch before has completed
   DenseEpi e;
@@ -426,7 +427,7 @@ __global__ void __launch_bounds__(Cfg<PACKED>::kThreads, 1) gemm_kernel(const __
             break;
           }
           uint32_t bar = bar_full + 8 * s;
-          if (rank == 0) mbar_expect_tx(bar, PACKED ? CG * kATile : CG * (kATile + p.hb * 128));
+          if (rank == 0) mbar_expect_tx(bar, CG * (p.a_rows + (PACKED ? 0 : p.hb)) * 128);
           if constexpr (CG == 2) bar = map_rank(bar, leader);
           const uint32_t dst = sbase + s * kStageBytes;
           tma_2d<CG>(dst, &p.a[pr], x, m0, bar);
@@ -972,6 +973,9 @@ cudaError_t launch_dense_gemm(const DenseGemm& g, cudaStream_t st) {
   p.spk = q.spk;
   if ((int64_t)q.tiles_m * q.tiles_n * 8 > INT32_MAX / 2) return cudaErrorInvalidValue;
   p.units = q.tiles_m * q.tiles_n;
+  // The rows of a short tile behind its box keep what the stage held: they only reach
+  // accumulator rows that are not stored.
+  p.a_rows = (int)std::min<int64_t>(kBM, (g.M + 7) / 8 * 8);
   p.wide = wide;
   p.early = g.early;
   p.e = g.e;
@@ -979,7 +983,7 @@ cudaError_t launch_dense_gemm(const DenseGemm& g, cudaStream_t st) {
   for (int i = 0; i < 2; ++i) {
     const int ai = g.pairs > 1 ? i : 0, wi = (g.pairs > 1 || gated) ? i : 0;
     cudaError_t err = cudaSuccess;
-    if (i == 0 || ai) err = encode(&p.a[i], t16, g.a[ai], g.M, g.K, g.lda * 2, kBK, kBM, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (i == 0 || ai) err = encode(&p.a[i], t16, g.a[ai], g.M, g.K, g.lda * 2, kBK, p.a_rows, CU_TENSOR_MAP_SWIZZLE_128B);
     if (err == cudaSuccess && (i == 0 || wi))
       err = wide ? encode(&p.w[i], t16, g.wide[wi], p.rows, cols, (int64_t)cols * 2, kBK, g.rows_k ? kBK : q.hb,
                           CU_TENSOR_MAP_SWIZZLE_128B)
