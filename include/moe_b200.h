@@ -186,8 +186,9 @@ int moe_gated_ffn_backward(moe_ctx* ctx, const moe_ffn_config* cfg, const moe_ff
  * (i, i + dims / 2). The rotated channels are multiplied by mscale; channels from dims on
  * are copied. inverse: the transposed rotation (the gradient). Angles are formed in 64 bits.
  * x_strides / out_strides: element strides of B, H and L (host arrays; D is contiguous);
- * out is x itself with the same strides, or overlaps it nowhere. offsets: [B] device
- * integers of offsets_bits 32 or 64, or NULL. D <= 4096.
+ * out is x itself with the same strides, or overlaps it nowhere; its rows lie apart (by
+ * rising stride, each step is longer than all that the smaller ones reach). |offset| <= 2^53.
+ * offsets: [B] device integers of offsets_bits 32 or 64, or NULL. D <= 4096.
  */
 typedef struct moe_rope_config {
     int32_t dtype;

@@ -237,7 +237,8 @@ class DenseMlp:
                                                group_size, bits)
 
     def _check(self, fn, x):
-        if x.dtype != self.dtype or x.device != self.device or not x.is_contiguous() or x.shape[-1] != self.hidden:
+        if (x.dtype != self.dtype or x.device != self.device or not x.is_contiguous() or x.dim() < 1
+                or x.shape[-1] != self.hidden):
             raise MlxError(fn, 1, f"contiguous {self.dtype} [..., {self.hidden}] on {self.device} expected, "
                                   f"got {x.dtype} {tuple(x.shape)} on {x.device}")
 

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <utility>
 #include <cstdarg>
 #include <cstdio>
 #include <cmath>
@@ -171,6 +172,20 @@ cudaError_t widen(const moe_ffn_config* c, const moe_ffn_weights* w, const FfnWs
   da.job[1] = {packed(w->up, c->inter, c->hidden), out.up};
   da.job[2] = {packed(w->down, c->hidden, c->inter), out.down};
   return moe::launch_dequant(da, st);
+}
+
+// Whether rows of D elements at these strides (of B, H and L) lie apart: by rising stride, each
+// step is longer than all that the smaller ones reach.
+bool separate_rows(int64_t B, int64_t H, int64_t L, int64_t D, const int64_t* strides) {
+  std::pair<int64_t, int64_t> axis[3] = {{strides[0], B}, {strides[1], H}, {strides[2], L}};
+  std::sort(axis, axis + 3);
+  int64_t reach = D - 1;
+  for (const auto& [stride, size] : axis) {
+    if (size == 1) continue;
+    if (stride <= reach || stride > (INT64_MAX / 4) / size) return false;
+    reach += (size - 1) * stride;
+  }
+  return true;
 }
 
 int check_workspace(moe_ctx* ctx, const char* fn, const void* ws, size_t have, size_t need) {
@@ -467,6 +482,10 @@ int moe_fast_rope(moe_ctx* ctx, const moe_rope_config* cfg, const void* x, const
     return fail(ctx, MOE_ERR_UNSUPPORTED, "%s: shape [%lld, %lld, %lld, %lld] is too large", fn, (long long)B,
                 (long long)H, (long long)L, (long long)D);
   if (!x || !x_strides || !out || !out_strides) return fail(ctx, MOE_ERR_INVALID, "%s: null pointer", fn);
+  if (!separate_rows(B, H, L, D, out_strides))
+    return fail(ctx, MOE_ERR_INVALID, "%s: rows of out overlap one another", fn);
+  if (offset > (int64_t(1) << 53) || offset < -(int64_t(1) << 53))
+    return fail(ctx, MOE_ERR_INVALID, "%s: offset=%lld is beyond 2^53", fn, (long long)offset);
   if (offsets && offsets_bits != 32 && offsets_bits != 64)
     return fail(ctx, MOE_ERR_INVALID, "%s: offsets_bits=%d", fn, offsets_bits);
   if (!freqs && !(cfg->base > 0.0 && std::isfinite(cfg->base)))

@@ -270,14 +270,15 @@ MOE_DEV float sigmoid_hw(float x) {
 }
 // The activation and its derivative. Both are x * sigmoid(z): SiLU with z = x, GELU's tanh
 // form with z = 2 sqrt(2/pi) (x + 0.044715 x^3), since (1 + tanh(y)) / 2 = sigmoid(2 y);
-// the derivative is sig + x sig (1 - sig) z'.
+// the derivative is sig + x sig (1 - sig) z'. Where z' would overflow (|x| > 1.8e19)
+// x sig (1 - sig) is zero: z' is held finite, so that their product is too.
 MOE_DEV float act_val(float x, int act) {
   const float z = act ? 1.5957691216057308f * x * __fmaf_rn(0.044715f * x, x, 1.0f) : x;
   return x * sigmoid_hw(z);
 }
 MOE_DEV void act_grad(float x, int act, float& val, float& grad) {
   const float z = act ? 1.5957691216057308f * x * __fmaf_rn(0.044715f * x, x, 1.0f) : x;
-  const float zp = act ? 1.5957691216057308f * __fmaf_rn(0.134145f * x, x, 1.0f) : 1.0f;
+  const float zp = act ? fminf(1.5957691216057308f * __fmaf_rn(0.134145f * x, x, 1.0f), 1e30f) : 1.0f;
   const float s = sigmoid_hw(z);
   val = x * s;
   grad = __fmaf_rn(val * (1.0f - s), zp, s);

@@ -203,7 +203,12 @@ PyObject* fast_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (type < 0 || (x->size(3) > 1 && x->stride(3) != 1)) Py_RETURN_NONE;
     moe_rope_config cfg{};
     cfg.dtype = type;
-    cfg.dims = (int32_t)PyLong_AsLong(a[1]);
+    const long dims = PyLong_AsLong(a[1]);
+    if (dims < 0 || dims > x->size(3)) {  // an error of the conversion too
+      PyErr_Clear();
+      Py_RETURN_NONE;
+    }
+    cfg.dims = (int32_t)dims;
     cfg.traditional = PyObject_IsTrue(a[2]);
     cfg.inverse = PyObject_IsTrue(a[8]);
     cfg.base = a[3] == Py_None ? 0.0 : PyFloat_AsDouble(a[3]);

@@ -360,7 +360,8 @@ def fast_rope(x, dims, traditional=False, base=10000.0, scale=1.0, offset=0, fre
     pairs (2i, 2i+1), else (i, i + dims/2); channels from dims on are copied. offset: an
     int, or an int32 / int64 tensor [B] with one offset per batch element. inverse: the
     transposed rotation, the gradient with respect to x. out: where to write, x itself
-    included (default: a new contiguous tensor). bf16, f16 or f32."""
+    included, else memory apart from x's (default: a new contiguous tensor). An int offset is
+    at most 2**53 in magnitude. bf16, f16 or f32."""
     if out is None and _calls is not None:
         r = _calls.fast_rope(x, dims, traditional, base, scale, offset, freqs, mscale, inverse)
         if r is not None:
@@ -390,6 +391,14 @@ def fast_rope(x, dims, traditional=False, base=10000.0, scale=1.0, offset=0, fre
         xs = os_ = (0, L * D, D, 1)
     if D > 1 and (xs[3] != 1 or os_[3] != 1):
         raise MlxError(fn, 1, "the channels of x and out must be contiguous")
+    if not 0 < dims <= D or dims % 2:
+        raise MlxError(fn, 1, f"dims={dims} must be even and in 2..{D}")
+    reach = D - 1  # by rising stride, each step of out is longer than all that the smaller ones reach
+    for s, n in sorted(zip(os_[:3], (B, H, L))):
+        if n > 1:
+            if s <= reach:
+                raise MlxError(fn, 1, "rows of out overlap one another")
+            reach += (n - 1) * s
     offs, offs_bits, off = None, 0, 0
     if isinstance(offset, torch.Tensor):
         if nd not in (3, 4) and offset.dim():
@@ -400,6 +409,8 @@ def fast_rope(x, dims, traditional=False, base=10000.0, scale=1.0, offset=0, fre
         offs, offs_bits = offset.data_ptr(), 32 if offset.dtype == torch.int32 else 64
     else:
         off = int(offset)
+        if abs(off) > 2 ** 53:
+            raise MlxError(fn, 1, f"offset={off} is beyond 2**53")
     if freqs is not None and (freqs.dtype != torch.float32 or freqs.device != x.device or
                               freqs.shape != (dims // 2,) or not freqs.is_contiguous()):
         raise MlxError(fn, 1, f"freqs: contiguous float32 [{dims // 2}] on {x.device} expected")

@@ -137,3 +137,32 @@ def test_rope_refusals():
     assert "freqs" in _refused(r, freqs=torch.ones(7))
     assert "out" in _refused(r, out=torch.zeros(2, 3, 5, 23))
     assert "other strides" in _refused(r, out=torch.as_strided(x, x.shape, (24, 240, 48, 1)))
+
+
+@pytest.mark.parametrize("offset", [2 ** 53 + 1, -2 ** 60, 2 ** 63, 2 ** 64])
+def test_rope_refuses_offsets_beyond_64_bit_angles(offset):
+    assert "offset" in _refused(ops.fast_rope, torch.zeros(1, 1, 2, 8), 8, offset=offset)
+
+
+@pytest.mark.parametrize("dims", [0, -2, 7, 10, 2 ** 32 + 8])
+def test_rope_refuses_dims(dims):
+    assert "dims" in _refused(ops.fast_rope, torch.zeros(1, 1, 2, 8), dims)
+
+
+def test_rope_refuses_an_output_that_overlaps_itself():
+    row = torch.zeros(1, 1, 5, 8)
+    x = row.expand(2, 3, 5, 8)
+    assert "overlap" in _refused(ops.fast_rope, x, 8, out=x)
+    assert "overlap" in _refused(ops.fast_rope, x[0], 8, out=x[0])
+    rows = torch.zeros(64).as_strided((1, 1, 5, 8), (40, 40, 6, 1))
+    assert "overlap" in _refused(ops.fast_rope, rows, 8, out=rows)
+    # heads of a fused projection do not: this gets as far as the device
+    fused = torch.zeros(2, 5, 6, 8)[:, :, 1:4].transpose(1, 2)
+    assert "CUDA" in _refused(ops.fast_rope, fused, 8, out=fused)
+
+
+def test_dense_mlp_refuses_a_scalar():
+    gen = _gen(9)
+    mk = lambda r, c: (lambda q: QWeight(q.w, q.scales, q.biases))(R.QW(gen, r, c, 32, torch.bfloat16))  # noqa: E731
+    mlp = DenseMlp(mk(96, 64), mk(96, 64), mk(64, 96), group_size=32)
+    assert "expected" in _refused(mlp, torch.zeros((), dtype=torch.bfloat16))

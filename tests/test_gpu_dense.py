@@ -105,7 +105,8 @@ FFN = [  # T, H, I, group, dtype, act
     (8, 2048, 1792, 32, F16, "gelu"), (9, 96, 1120, 32, BF16, "silu"), (32, 704, 320, 64, BF16, "silu"),
     (33, 384, 256, 128, F16, "silu"), (128, 192, 448, 64, F16, "gelu"), (129, 2048, 768, 128, BF16, "silu"),
     (333, 1024, 736, 32, BF16, "gelu"), (700, 640, 1408, 64, BF16, "silu"),
-    (1025, 256, 352, 32, F16, "silu"), (2500, 384, 640, 128, BF16, "gelu")]
+    (1025, 256, 352, 32, F16, "silu"), (2500, 384, 640, 128, BF16, "gelu"),
+    (20, 1024, 8192, 64, BF16, "silu"), (13, 512, 64, 32, F16, "gelu"), (2047, 128, 192, 64, BF16, "silu")]
 
 
 def _ffn_case(T, H, I, g, dt):
@@ -423,3 +424,102 @@ def test_backward_captured_in_a_graph():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_gradients_of_huge_activations_are_finite():
+    """Where the derivative is 0 or 1 to the last bit, its factors must not overflow: dg and du
+    of large g, u, against the formulas' limits."""
+    from mlx_rs_b200 import ops
+    H, I, T = 64, 64, 140
+    gen = _gen(91)
+    from mlx_rs_b200.synth import QWeight
+    q = [R.QW(gen, r, c, 32, BF16, True, "cuda") for r, c in ((I, H), (I, H), (H, I))]
+    w = [QWeight(a.w, a.scales, a.biases) for a in q]
+    g = torch.tensor([1e4, -1e4, 1e15, -1e15, 1e25, -1e25, 3e38, -3e38], device="cuda").to(BF16).repeat(T, I // 8)
+    u, dy = torch.ones_like(g), R.rand(gen, T, H, dtype=BF16, device="cuda")
+    dh = R.qmm(dy, q[2], transpose=False)[0]
+    for act in ("silu", "gelu"):
+        _, dg, du = ops.gated_ffn_vjp(g, u, dy, *w, activation=act, group_size=32)
+        assert bool(torch.isfinite(dg).all())
+        # u = 1, act' = 1 or 0: dg is dh (weights and result rounded once each) or 0
+        assert R.rel(dg[g > 0], dh[g > 0]) <= 2 * R.U[BF16] and float(dg[g < 0].abs().max()) == 0
+        assert float(du[g < 0].abs().max()) == 0
+
+
+def test_calls_with_and_without_ctypes_agree(monkeypatch):
+    from mlx_rs_b200 import ops
+    assert ops._calls is not None
+    qs, ws, x, dy = _ffn_case(37, 256, 384, 64, BF16)
+    xr = R.rand(_gen(92), 2, 3, 5, 64, dtype=F32, device="cuda")
+    off = torch.tensor([4, 9], device="cuda")
+    freqs = torch.linspace(1, 50, 16, device="cuda")
+
+    def run():
+        out, g, u = ops.gated_ffn(x, *ws, residual=x, save=True)
+        return [out, g, u, *ops.gated_ffn_vjp(g, u, dy, *ws),
+                ops.quantized_matmul(x, qs[0].w, qs[0].scales, qs[0].biases, transpose=True, group_size=64),
+                ops.quantized_matmul(dy, qs[2].w, qs[2].scales, qs[2].biases, transpose=False, group_size=64),
+                ops.quantized_matmul(x.view(1, 37, 256), qs[1].w.view(torch.uint32), qs[1].scales, None, group_size=64),
+                ops.fast_rope(xr, 32, True, 1000.0, 0.5, off, None, 1.5, True), ops.fast_rope(xr, 32, freqs=freqs, offset=-3)]
+
+    with_c = run()
+    monkeypatch.setattr(ops, "_calls", None)
+    for a, b in zip(with_c, run()):
+        assert a.shape == b.shape and a.dtype == b.dtype and torch.equal(a, b)
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first calls of every operator are captured, with sizes of each form."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from mlx_rs_b200 import ops
+import dense_ref as R
+from mlx_rs_b200.synth import QWeight
+gen = torch.Generator().manual_seed(5)
+bf = torch.bfloat16
+q = [R.QW(gen, r, c, 32, bf, True, "cuda") for r, c in ((192, 128), (192, 128), (128, 192))]
+w = [QWeight(a.w, a.scales, a.biases) for a in q]
+xs = [R.rand(gen, T, 128, dtype=bf, device="cuda") for T in (1, 40, 300, 2100)]
+def step(x):
+    out, g, u = ops.gated_ffn(x, *w, group_size=32, save=True)
+    y = ops.quantized_matmul(out, q[0].w, q[0].scales, q[0].biases, group_size=32)
+    return [*ops.gated_ffn_vjp(g, u, out, *w, group_size=32), ops.fast_rope(y.view(1, -1, 3, 64).transpose(1, 2), 64)]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = [step(x) for x in xs]
+graph.replay()
+torch.cuda.synchronize()
+for x, g in zip(xs, got):
+    assert all(torch.equal(a, b) for a, b in zip(step(x), g))
+print("same")
+"""
+    import os
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([here, os.path.dirname(here)]))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240, env=env)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+def test_rope_entry_refuses_overlapping_rows_and_far_offsets():
+    import mlx_rs_b200
+    from mlx_rs_b200 import _lib, ops
+    from mlx_rs_b200._lib import MlxError
+    ctx = _lib.context_for(0)
+    lib = mlx_rs_b200.library()
+    t = torch.ones(1 << 12, dtype=torch.float32, device="cuda")
+    cfg = _lib.RopeConfig(2, 8, 0, 0, 10000.0, 1.0, 1.0)
+
+    def call(strides, offset=0, sizes=(2, 2, 2)):
+        s = (C.c_int64 * 3)(*strides)
+        return lib.moe_fast_rope(ctx.handle, C.byref(cfg), t.data_ptr(), s, *sizes, 8, offset, None, 0, None, t.data_ptr(), s)
+    assert call((0, 16, 8)) == 1 and b"overlap" in lib.moe_last_error(ctx.handle)
+    assert call((32, 16, 4)) == 1 and call((8, 8, 16)) == 1 and call((-32, 16, 8)) == 1 and call((2 ** 61, 16, 8)) == 1
+    assert call((32, 16, 8), 2 ** 53 + 1) == 1 and call((32, 16, 8), -2 ** 60) == 1
+    torch.cuda.synchronize()
+    assert float(t.sum()) == t.numel()
+    with pytest.raises(MlxError, match="offset"):
+        ops.fast_rope(t.view(1, 1, -1, 8), 8, offset=2 ** 53 + 1)
+    with pytest.raises(MlxError, match="dims"):
+        ops.fast_rope(t.view(1, 1, -1, 8), 2 ** 32 + 8)
