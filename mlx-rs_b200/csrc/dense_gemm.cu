@@ -1,34 +1,46 @@
 // dense_gemm.cu — 4-bit matrix products on tcgen05 with the feed-forward block's epilogues.
 //
 // D[m, n] = sum_p A_p[m, :] . W_p[n, :]^T, or A_p . W_p with the weights' rows as the summed
-// index (the gradient's direction), fp32 accumulators in tensor memory. The weights go from
-// their packed form straight into the operand tile: no 16-bit copy of them exists in global
-// memory. Tokens are the MMA's rows (an epilogue thread owns one token and walks its
-// columns), weights its columns; K runs in steps of 64.
-//   warp 20     streams the token tile with TMA (128 rows x 128 bytes, swizzled);
-//   warp 22     streams the packed tiles with TMA into a ring of their own;
-//   warps 4-19  four groups, taking the K steps in turn: a thread turns the 64 weights of one row
-//               (32 bytes packed, one or two quantization groups) into eight 16-byte pieces
-//               of the B tile, w = RN16(s q + b) (one rounding: a tcgen05 product
-//               takes both operands in one 16-bit type). With the rows summed, a word's eight
-//               weights are neighbours along N and the tile is MN-major; the addresses are
-//               the same in both layouts, only the meaning of a row differs;
-//   warp 21     allocates the tensor memory (two accumulators) and issues tcgen05.mma from one
-//               lane: M = 128 (256 over a pair of CTAs), K = 16;
+// index (the gradient's direction), fp32 accumulators in tensor memory. Tokens are the MMA's
+// rows (an epilogue thread owns one token and walks its columns), weights its columns; K runs
+// in steps of 64. w = RN16(s q + b): one rounding, because a tcgen05 product takes both
+// operands in one 16-bit type.
+// The packed form dequantises in the product, so that no 16-bit copy of the weights exists in
+// global memory; 23 warps:
 //   warps 0-3   read the finished accumulator back and apply the epilogue, while the next
 //               tile accumulates in the other buffer. A warp's global accesses go through a
-//               1 KB buffer, so that they cover 32 contiguous bytes of 16 rows each.
-// CTA pairs (CG = 2, more than 128 tokens): each CTA loads its own 128 tokens and dequantises
-// its half of the weight rows, once per 256 tokens; the leader (even rank) owns the full and
+//               1 KB buffer, so that they cover 32 contiguous bytes of 16 rows each;
+//   warps 4-19  four groups, taking the K steps in turn: a thread turns the 64 weights of one
+//               row (32 bytes packed, one or two quantization groups) into eight 16-byte
+//               pieces of the B tile. With the rows summed, a word's eight weights are
+//               neighbours along N and the tile is MN-major; the addresses are the same in
+//               both layouts, only the meaning of a row differs;
+//   warp 20     streams the token tile with TMA (128 bytes of each row, swizzled);
+//   warp 21     allocates the tensor memory (two accumulators) and issues tcgen05.mma from one
+//               lane: M = 128 (256 over a pair of CTAs), K = 16;
+//   warp 22     streams the packed tiles with TMA into a ring of their own.
+// The wide form (weights already in 16 bits, kWideMinM) has eight epilogue warps, then the TMA
+// warp, which streams the weights' tile beside the tokens', and the MMA warp.
+// CTA pairs (CG = 2, more than 128 tokens): each CTA loads its own 128 tokens and its half of
+// the weight rows, once per 256 tokens; the leader (even rank) owns the full and
 // accumulator-empty barriers and issues the MMAs of both. In the gated form the two halves of
 // a tile's columns are gate rows and the same rows of up, so that one thread holds g and u of
 // the same element.
-// Few tiles: K is split over the CTAs of a cluster (up to 8). Each leaves its fp32 sums in its
-// own shared memory, and after a cluster barrier every CTA adds one slice of the tokens over
-// the cluster in split order (distributed shared memory; no atomics, the same bits on every
-// run) and applies the epilogue to it.
+// Few tiles (packed form): K is split over the CTAs of a cluster (up to 8). Each leaves its
+// fp32 sums in its own shared memory, and after a cluster barrier every CTA adds one slice of
+// the tokens over the cluster in split order (distributed shared memory; no atomics, the same
+// bits on every run) and applies the epilogue to it.
 // Every wait is bounded (2 s): on expiry the CTA records a code in the device's status word,
 // stops working and leaves through the same barriers as the rest of its cluster.
+//
+// What bounds it. Packed: the dequantising warps, 0.32 / 0.53 us per K step at 64 / 128 weight
+// rows per CTA, and for few steps the 4.5 us of a round's start, first loads and epilogue: 512
+// tokens of the block 2048 x 5632 44.7 us (0.79 PFLOP/s), 5632 -> 2048 22.7 us with the rows
+// summed. Wide: the tensor pipe in the forward products (4096 tokens: 110 us for gate and up,
+// 1.72 PFLOP/s; 60 us for down, 1.57), the epilogue's reads of g and u and writes of dg and du
+// in dh (88 us). Measured against it: a fused pass that leaves 16-bit weights for every size
+// (64.6 us for 512 tokens), cluster-scope arrivals on the step barriers (twice the time per
+// step: each is a fence over global memory), two groups of dequantising warps instead of four.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -458,139 +470,140 @@ __global__ void __launch_bounds__(Cfg<PACKED>::kThreads, 1) gemm_kernel(const __
         }
     }
   } else if (PACKED && warp == kPackWarp) {
-   if constexpr (PACKED)
-    if (lane == 0) {
-      int it = 0;
-      bool ok = true;
-      for (int unit = first; ok && unit < p.units; unit += stride) {
-        const int nt = tile_n(unit);
-        for (int k = k0; k < k1; ++k, ++it) {
-          const int s = it % kSlots;
-          if (!mbar_wait(bar_pempty + 8 * s, ((it / kSlots) & 1) ^ 1, &gone)) {
-            gone = 1;
-            atomicOr(&g_dense_status, 32);
-            ok = false;
-            break;
-          }
-          const uint32_t bar = bar_pfull + 8 * s;
-          mbar_expect_tx(bar, kHalves * p.hb * 32);
-          const int pr = k >= p.ks0 ? 1 : 0;
-          const int kk = k - (pr ? p.ks0 : 0);
+    if constexpr (PACKED) {
+      if (lane == 0) {
+        int it = 0;
+        bool ok = true;
+        for (int unit = first; ok && unit < p.units; unit += stride) {
+          const int nt = tile_n(unit);
+          for (int k = k0; k < k1; ++k, ++it) {
+            const int s = it % kSlots;
+            if (!mbar_wait(bar_pempty + 8 * s, ((it / kSlots) & 1) ^ 1, &gone)) {
+              gone = 1;
+              atomicOr(&g_dense_status, 32);
+              ok = false;
+              break;
+            }
+            const uint32_t bar = bar_pfull + 8 * s;
+            mbar_expect_tx(bar, kHalves * p.hb * 32);
+            const int pr = k >= p.ks0 ? 1 : 0;
+            const int kk = k - (pr ? p.ks0 : 0);
 #pragma unroll
-          for (int h = 0; h < kHalves; ++h) {
-            const uint32_t dst = sbase + kPackAt + s * kPackBytes + h * p.hb * 32;
-            const int n = half_row(nt, h);
-            if constexpr (ROWS_K) {  // boxes of 64 rows x 64 columns
-              tma_2d<1>(dst, &p.w[pr], n / 8, kk * kBK, bar);
-              if (CG == 2 && p.hb == 128) tma_2d<1>(dst + 2048, &p.w[pr], n / 8 + 8, kk * kBK, bar);
-            } else {                 // hb rows x 64 columns
-              tma_2d<1>(dst, &p.w[p.gated ? (CG == 2 ? rank : h) : pr], kk * 8, n, bar);
+            for (int h = 0; h < kHalves; ++h) {
+              const uint32_t dst = sbase + kPackAt + s * kPackBytes + h * p.hb * 32;
+              const int n = half_row(nt, h);
+              if constexpr (ROWS_K) {  // boxes of 64 rows x 64 columns
+                tma_2d<1>(dst, &p.w[pr], n / 8, kk * kBK, bar);
+                if (CG == 2 && p.hb == 128) tma_2d<1>(dst + 2048, &p.w[pr], n / 8 + 8, kk * kBK, bar);
+              } else {                 // hb rows x 64 columns
+                tma_2d<1>(dst, &p.w[p.gated ? (CG == 2 ? rank : h) : pr], kk * 8, n, bar);
+              }
             }
           }
         }
-      }
-      // no copy may still be landing when the CTA leaves
-      for (int i = it - kSlots < 0 ? 0 : it - kSlots; i < it; ++i) {
-        int never = 0;
-        if (!mbar_wait(bar_pfull + 8 * (i % kSlots), (i / kSlots) & 1, &never)) atomicOr(&g_dense_status, 64);
+        // no copy may still be landing when the CTA leaves
+        for (int i = it - kSlots < 0 ? 0 : it - kSlots; i < it; ++i) {
+          int never = 0;
+          if (!mbar_wait(bar_pfull + 8 * (i % kSlots), (i / kSlots) & 1, &never)) atomicOr(&g_dense_status, 64);
+        }
       }
     }
   } else if (PACKED && warp >= kDeqWarp && warp < kTmaWarp) {
-   if constexpr (PACKED) {
-    // ---- dequantisation: group wg takes steps wg, wg + kGroups, ... of this CTA's sequence
-    const int wg = (warp - kDeqWarp) >> 2, wt = tid - (kDeqWarp + 4 * wg) * 32;
-    // A thread owns one row of 64 weights of the tile (128 bytes of it, eight words packed):
-    // row wt of this CTA's weight rows (both halves when CG = 1); with ROWS_K row wt % 64 of
-    // the step, in the block wt / 64 of 64 columns. Two groups of weights at group size 32.
-    const int per = k1 - k0;
-    const int total = first < p.units ? (int)((p.units - first + stride - 1) / stride) * per : 0;
-    const bool mine = wt < kHalves * p.hb;
-    const int half = CG == 1 && wt >= p.hb ? 1 : 0;
-    const bool two = p.lg == 5;
-    // The scales and biases of the group's next two steps, read ahead: at_k walks the steps,
-    // the pointers are those of its tile and operand pair.
-    const uint16_t* ps = nullptr;
-    const uint16_t* pb = nullptr;
-    bool valid = false, second = false;
-    int at_unit = first, at_k = k0 + wg, at_key = -1;
-    while (at_k >= k1) at_k -= per, at_unit += stride;
-    auto read_scales = [&](uint32_t (&vs)[2], uint32_t (&vb)[2]) {
-      vs[0] = vs[1] = vb[0] = vb[1] = 0u;
-      if (at_unit < p.units) {
-        const int pr = at_k >= p.ks0 ? 1 : 0;
-        if (at_key != 2 * at_unit + pr) {
-          at_key = 2 * at_unit + pr;
-          const int n = half_row(tile_n(at_unit), half) + (ROWS_K ? (CG == 2 ? wt & 64 : 0) : wt - half * p.hb);
-          const WeightSide& q = p.q[p.gated ? (CG == 2 ? rank : half) : pr];
-          valid = mine && n < p.N;
-          second = valid && two && (!ROWS_K || n + 32 < p.N);
-          const int64_t off = !valid ? 0 : ROWS_K ? (int64_t)(wt & 63) * p.s_pitch + (n >> p.lg) : (int64_t)n * p.s_pitch;
-          ps = q.s + off;
-          pb = q.b ? q.b + off : nullptr;
-        }
-        const int kk = at_k - (pr ? p.ks0 : 0);
-        const int g = (kk * kBK) >> p.lg;
-        const int64_t off = ROWS_K ? (int64_t)(kk * kBK) * p.s_pitch : g;
-        const bool in = ROWS_K ? kk * kBK + (wt & 63) < p.rows : true;  // the first group of a step exists
-        if (valid && in) {
-          vs[0] = ldg_u16(ps + off);
-          if (pb) vb[0] = ldg_u16(pb + off);
-        }
-        if (second && in && (ROWS_K || g + 1 < p.s_pitch)) {
-          vs[1] = ldg_u16(ps + off + 1);
-          if (pb) vb[1] = ldg_u16(pb + off + 1);
-        }
-      }
-      at_k += kGroups;
+    if constexpr (PACKED) {
+      // ---- dequantisation: group wg takes steps wg, wg + kGroups, ... of this CTA's sequence
+      const int wg = (warp - kDeqWarp) >> 2, wt = tid - (kDeqWarp + 4 * wg) * 32;
+      // A thread owns one row of 64 weights of the tile (128 bytes of it, eight words packed):
+      // row wt of this CTA's weight rows (both halves when CG = 1); with ROWS_K row wt % 64 of
+      // the step, in the block wt / 64 of 64 columns. Two groups of weights at group size 32.
+      const int per = k1 - k0;
+      const int total = first < p.units ? (int)((p.units - first + stride - 1) / stride) * per : 0;
+      const bool mine = wt < kHalves * p.hb;
+      const int half = CG == 1 && wt >= p.hb ? 1 : 0;
+      const bool two = p.lg == 5;
+      // The scales and biases of the group's next two steps, read ahead: at_k walks the steps,
+      // the pointers are those of its tile and operand pair.
+      const uint16_t* ps = nullptr;
+      const uint16_t* pb = nullptr;
+      bool valid = false, second = false;
+      int at_unit = first, at_k = k0 + wg, at_key = -1;
       while (at_k >= k1) at_k -= per, at_unit += stride;
-    };
-    uint32_t rs[2][2], rb[2][2];
-    read_scales(rs[0], rb[0]);
-    read_scales(rs[1], rb[1]);
-    const uint32_t to = (uint32_t)wt * 128;
-    bool ok = true;
-    for (int it = wg; ok && it < total; it += 2 * kGroups) {
+      auto read_scales = [&](uint32_t (&vs)[2], uint32_t (&vb)[2]) {
+        vs[0] = vs[1] = vb[0] = vb[1] = 0u;
+        if (at_unit < p.units) {
+          const int pr = at_k >= p.ks0 ? 1 : 0;
+          if (at_key != 2 * at_unit + pr) {
+            at_key = 2 * at_unit + pr;
+            const int n = half_row(tile_n(at_unit), half) + (ROWS_K ? (CG == 2 ? wt & 64 : 0) : wt - half * p.hb);
+            const WeightSide& q = p.q[p.gated ? (CG == 2 ? rank : half) : pr];
+            valid = mine && n < p.N;
+            second = valid && two && (!ROWS_K || n + 32 < p.N);
+            const int64_t off = !valid ? 0 : ROWS_K ? (int64_t)(wt & 63) * p.s_pitch + (n >> p.lg) : (int64_t)n * p.s_pitch;
+            ps = q.s + off;
+            pb = q.b ? q.b + off : nullptr;
+          }
+          const int kk = at_k - (pr ? p.ks0 : 0);
+          const int g = (kk * kBK) >> p.lg;
+          const int64_t off = ROWS_K ? (int64_t)(kk * kBK) * p.s_pitch : g;
+          const bool in = ROWS_K ? kk * kBK + (wt & 63) < p.rows : true;  // the first group of a step exists
+          if (valid && in) {
+            vs[0] = ldg_u16(ps + off);
+            if (pb) vb[0] = ldg_u16(pb + off);
+          }
+          if (second && in && (ROWS_K || g + 1 < p.s_pitch)) {
+            vs[1] = ldg_u16(ps + off + 1);
+            if (pb) vb[1] = ldg_u16(pb + off + 1);
+          }
+        }
+        at_k += kGroups;
+        while (at_k >= k1) at_k -= per, at_unit += stride;
+      };
+      uint32_t rs[2][2], rb[2][2];
+      read_scales(rs[0], rb[0]);
+      read_scales(rs[1], rb[1]);
+      const uint32_t to = (uint32_t)wt * 128;
+      bool ok = true;
+      for (int it = wg; ok && it < total; it += 2 * kGroups) {
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {  // two steps per round: constant ring indexes
-        const int step = it + kGroups * sub;
-        if (step >= total) break;
-        const int s = step % kStages, sl = step % kSlots;
-        bool ready = mbar_wait(bar_pfull + 8 * sl, (step / kSlots) & 1, &gone);
-        uint4 q0, q1;
-        if (__all_sync(0xffffffffu, ready)) {
-          const uint32_t src = sbase + kPackAt + sl * kPackBytes + wt * 32;
-          q0 = lds16(src), q1 = lds16(src + 16);
-          ready = mbar_wait(bar_empty + 8 * s, ((step / kStages) & 1) ^ 1, &gone);
-        }
-        if (!__all_sync(0xffffffffu, ready)) {
-          gone = 1;
-          if (lane == 0) atomicOr(&g_dense_status, 128);
-          ok = false;
-          break;
-        }
-        if (mine) {
-          const uint32_t row = sbase + s * kStageBytes + kATile + to;
-          const uint32_t s2 = __byte_perm(rs[sub][0], 0, 0x1010), b2 = __byte_perm(rb[sub][0], 0, 0x1010);
-          const uint32_t* w = &q0.x;
+        for (int sub = 0; sub < 2; ++sub) {  // two steps per round: constant ring indexes
+          const int step = it + kGroups * sub;
+          if (step >= total) break;
+          const int s = step % kStages, sl = step % kSlots;
+          bool ready = mbar_wait(bar_pfull + 8 * sl, (step / kSlots) & 1, &gone);
+          uint4 q0, q1;
+          if (__all_sync(0xffffffffu, ready)) {
+            const uint32_t src = sbase + kPackAt + sl * kPackBytes + wt * 32;
+            q0 = lds16(src), q1 = lds16(src + 16);
+            ready = mbar_wait(bar_empty + 8 * s, ((step / kStages) & 1) ^ 1, &gone);
+          }
+          if (!__all_sync(0xffffffffu, ready)) {
+            gone = 1;
+            if (lane == 0) atomicOr(&g_dense_status, 128);
+            ok = false;
+            break;
+          }
+          if (mine) {
+            const uint32_t row = sbase + s * kStageBytes + kATile + to;
+            const uint32_t s2 = __byte_perm(rs[sub][0], 0, 0x1010), b2 = __byte_perm(rb[sub][0], 0, 0x1010);
+            const uint32_t* w = &q0.x;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) sts16(row + (((uint32_t)c ^ (wt & 7)) << 4), dequant8<TYPE>(w[c], s2, b2));
-          const uint32_t s3 = two ? __byte_perm(rs[sub][1], 0, 0x1010) : s2;
-          const uint32_t b3 = two ? __byte_perm(rb[sub][1], 0, 0x1010) : b2;
-          const uint32_t* v = &q1.x;
+            for (int c = 0; c < 4; ++c) sts16(row + (((uint32_t)c ^ (wt & 7)) << 4), dequant8<TYPE>(w[c], s2, b2));
+            const uint32_t s3 = two ? __byte_perm(rs[sub][1], 0, 0x1010) : s2;
+            const uint32_t b3 = two ? __byte_perm(rb[sub][1], 0, 0x1010) : b2;
+            const uint32_t* v = &q1.x;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) sts16(row + (((uint32_t)(4 + c) ^ (wt & 7)) << 4), dequant8<TYPE>(v[c], s3, b3));
+            for (int c = 0; c < 4; ++c) sts16(row + (((uint32_t)(4 + c) ^ (wt & 7)) << 4), dequant8<TYPE>(v[c], s3, b3));
+          }
+          fence_proxy();
+          __syncwarp();
+          // the packed words are in use by now: only here may their slot be filled again
+          if (lane == 0) {
+            mbar_arrive(bar_pempty + 8 * sl);
+            mbar_arrive_cluster(CG == 2 ? map_rank(bar_full + 8 * s, leader) : bar_full + 8 * s);
+          }
+          read_scales(rs[sub], rb[sub]);
         }
-        fence_proxy();
-        __syncwarp();
-        // the packed words are in use by now: only here may their slot be filled again
-        if (lane == 0) {
-          mbar_arrive(bar_pempty + 8 * sl);
-          mbar_arrive_cluster(CG == 2 ? map_rank(bar_full + 8 * s, leader) : bar_full + 8 * s);
-        }
-        read_scales(rs[sub], rb[sub]);
       }
     }
-   }
   } else if (warp == kMmaWarp) {
     // The whole warp walks the steps, so that descriptors and addresses stay in uniform
     // registers; one elected lane issues. The next stage's barrier is asked about before this
