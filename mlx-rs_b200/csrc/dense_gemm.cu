@@ -36,11 +36,14 @@
 // What bounds it. Packed: the dequantising warps, 0.32 / 0.53 us per K step at 64 / 128 weight
 // rows per CTA, and for few steps the 4.5 us of a round's start, first loads and epilogue: 512
 // tokens of the block 2048 x 5632 44.7 us (0.79 PFLOP/s), 5632 -> 2048 22.7 us with the rows
-// summed. Wide: the tensor pipe in the forward products (4096 tokens: 110 us for gate and up,
-// 1.72 PFLOP/s; 60 us for down, 1.57), the epilogue's reads of g and u and writes of dg and du
-// in dh (88 us). Measured against it: a fused pass that leaves 16-bit weights for every size
-// (64.6 us for 512 tokens), cluster-scope arrivals on the step barriers (twice the time per
-// step: each is a fence over global memory), two groups of dequantising warps instead of four.
+// summed. Wide: the tensor pipe, active 87 to 93 % of the cycles in the plain and gated products
+// (block 2048 x 5632, 4096 tokens, with the dequantisation: forward 203 us, 1.40 PFLOP/s; with
+// the gradients 459 us, 1.24). In the product with the gated gradient it is active 57 %: beside
+// the operands g and u are read and dg and du written, 1.1 GB through L2 at 11.7 TB/s. Measured
+// against it: weights left in 16 bits by a launch before for every size (64.6 us for 512
+// tokens), cluster-scope arrivals on the step barriers (twice the time per step: each is a
+// fence over global memory), 12 or 16 epilogue warps in the gated gradient and its g and u one
+// or two chunks ahead (all within 0.6 %).
 #include <cudaTypedefs.h>
 
 #include <algorithm>
