@@ -4,13 +4,16 @@ Host-side mirror of the reference's Rust interface for this path:
   ops.quantized_matmul / ops.gather_qmm / ops.fast_rms_norm
       <- Array::quantized_matmul / Array::gather_qmm / Array::fast_rms_norm
          (crates/mlx-core/src/ops.rs:592-637, 830-891, 691-701)
+  ops.fast_rope, ops.gated_ffn / ops.gated_ffn_vjp, block.DenseMlp
+      <- Array::fast_rope, the dense feed-forward block of layers without experts
+         (DenseMlp of qwen3_moe_python_port.rs and lfm2_moe_python_port.rs) and its gradient
   block.SparseMoeBlock, block.MoeFeedForward, block.RmsNorm, block.MoeStack
       <- SparseMoeBlock::forward (qwen3_moe_python_port.rs:420-488),
          MoeFeedForward::forward (lfm2_moe_python_port.rs:541-740),
          RmsNorm::forward (crates/mlx-nn/src/rms_norm.rs:30-34)
   graph.GraphedForward
       <- the per-step MoE work of the decode loop (generate.rs:811-880), one graph replay
-  checkpoint.load_blocks / load_device_blocks
+  checkpoint.load_blocks / load_device_blocks / load_device_mlps
       <- VarBuilder::from_safetensors + SparseMoeBlock::load / MoeFeedForward::load
          (crates/mlx-nn/src/var_builder.rs:31-46, qwen3_moe_python_port.rs:394-418,
          lfm2_moe_python_port.rs:524-540)

@@ -17,6 +17,8 @@ Mirrors how the reference loads the block's tensors (no MLX needed):
     ``<layer>.feed_forward.switch_mlp.<proj>.*`` (ExpertLinear::load, :435-460), and
     ``<layer>.feed_forward.expert_bias`` is optional (added to the router logits before the
     softmax, :559-567);
+  * the feed-forward block of a layer without experts is ``<layer>.mlp.{gate,up,down}_proj.*``,
+    or ``<layer>.feed_forward.*`` with those names or w1, w3, w2 for gate, up, down;
   * the block shape and quantization come from config.json (Qwen3MoePythonPortConfig /
     Lfm2MoeConfig fields: hidden_size, num_experts or num_local_experts,
     num_experts_per_tok, moe_intermediate_size, shared_expert_intermediate_size,
@@ -264,6 +266,55 @@ def moe_layers(tensors: _Tensors, cfg: dict, prefix: str = "model.layers") -> Li
     return out
 
 
+_DENSE_NAMES = [("mlp", ("gate_proj", "up_proj", "down_proj")), ("feed_forward", ("gate_proj", "up_proj", "down_proj")),
+                ("feed_forward", ("w1", "w3", "w2"))]
+
+
+def _dense_prefixes(tensors: _Tensors, layer_prefix: str):
+    """Prefixes of a layer's packed gate, up and down projections, or None."""
+    for base, names in _DENSE_NAMES:
+        found = [f"{layer_prefix}.{base}.{n}" for n in names]
+        if all(tensors.has(f + ".weight") and tensors.has(f + ".scales") for f in found):
+            return found
+    return None
+
+
+def dense_layers(tensors: _Tensors, cfg: dict, prefix: str = "model.layers") -> List[int]:
+    """Decoder layers whose feed-forward block is dense and quantized."""
+    moe = set(moe_layers(tensors, cfg, prefix))
+    return [i for i in range(int(cfg.get("num_hidden_layers", 0)))
+            if i not in moe and _dense_prefixes(tensors, f"{prefix}.{i}")]
+
+
+def load_dense(tensors: _Tensors, layer_prefix: str, cfg: dict):
+    """((gate, up, down), group_size, bits) of a layer's dense feed-forward block."""
+    found = _dense_prefixes(tensors, layer_prefix)
+    if found is None:
+        raise CheckpointError(f"{layer_prefix}: no quantized dense feed-forward block")
+    qs = tuple(tensors.qweight(f) for f in found)
+    quant = cfg.get("quantization") or cfg.get("quantization_config") or {}
+    gs = int(quant.get("group_size", 64))
+    bits = {infer_bits(q.w.shape, q.scales.shape, gs, int(quant.get("bits", 4))) for q in qs}
+    if len(bits) != 1:
+        raise CheckpointError(f"{layer_prefix}: the projections have {sorted(bits)} bits")
+    return qs, gs, bits.pop()
+
+
+def load_device_mlps(directory: str, device="cuda", layers: Optional[List[int]] = None, prefix: str = "model.layers"):
+    """The checkpoint's dense feed-forward blocks (default: of every layer that has one) as
+    DenseMlp blocks ready to call (weights copied bit for bit; SiLU)."""
+    from .block import DenseMlp
+    from .synth import _q_to
+    tensors, cfg = open_checkpoint(directory)
+    if layers is None:
+        layers = dense_layers(tensors, cfg, prefix)
+    out = []
+    for i in layers:
+        qs, gs, bits = load_dense(tensors, f"{prefix}.{i}", cfg)
+        out.append(DenseMlp(*(_q_to(q, device) for q in qs), group_size=gs, bits=bits))
+    return out
+
+
 def open_checkpoint(directory: str) -> (_Tensors, dict):
     files = sorted(glob.glob(os.path.join(directory, "*.safetensors")))
     if not files:
@@ -297,4 +348,4 @@ def load_device_blocks(directory: str, device="cuda", layers: Optional[List[int]
 
 
 __all__ = ["CheckpointError", "read_safetensors", "write_safetensors", "infer_bits", "block_config",
-           "load_block", "load_blocks", "load_device_blocks", "moe_layers", "open_checkpoint", "SCORING_SIGMOID_BIAS_SELECT"]
+           "load_block", "load_blocks", "load_device_blocks", "moe_layers", "dense_layers", "load_dense", "load_device_mlps", "open_checkpoint", "SCORING_SIGMOID_BIAS_SELECT"]

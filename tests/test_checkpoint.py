@@ -256,3 +256,61 @@ def test_mismatched_scale_shape_is_rejected(tmp_path):
                                                                                 np.asarray(e.array)[..., :3])
     with pytest.raises(C.CheckpointError, match="up"):
         C.load_block(tensors, "model.layers.1", c)
+
+
+def _write_dense(d, gs, layers, conf=None):
+    """Dense blocks [192 x 128] under each of the three name forms, beside what is not one."""
+    names = [("mlp", ("gate_proj", "up_proj", "down_proj")), ("feed_forward", ("gate_proj", "up_proj", "down_proj")),
+             ("feed_forward", ("w1", "w3", "w2"))]
+    rng = np.random.default_rng(3)
+    t, want = {}, []
+    for i, L in enumerate(layers):
+        base, parts = names[i % 3]
+        qs = []
+        for part, (r, c) in zip(parts, ((192, 128), (192, 128), (128, 192))):
+            q = S.QWeight(rng.integers(0, 2 ** 32, (r, c // 8), dtype=np.uint32),
+                          S.f32_to_bf16_bits(rng.random((r, c // gs), dtype=np.float32) * 0.02),
+                          S.f32_to_bf16_bits(rng.random((r, c // gs), dtype=np.float32) * 0.1 - 0.15))
+            _q(f"model.layers.{L}.{base}.{part}", q, t)
+            qs.append(q)
+        want.append(qs)
+    t["model.layers.7.mlp.gate_proj.weight"] = np.zeros((192, 128), np.uint16)  # not quantized
+    C.write_safetensors(os.path.join(d, "model.safetensors"), t)
+    with open(os.path.join(d, "config.json"), "w") as f:
+        json.dump({"hidden_size": 128, "num_hidden_layers": 8, "quantization": {"group_size": gs, "bits": 4}, **(conf or {})}, f)
+    return want
+
+
+@pytest.mark.parametrize("gs", [32, 64])
+def test_dense_blocks_of_a_checkpoint(tmp_path, gs):
+    want = _write_dense(str(tmp_path), gs, [0, 2, 5])
+    tensors, cfg = C.open_checkpoint(str(tmp_path))
+    assert C.dense_layers(tensors, cfg) == [0, 2, 5] and C.moe_layers(tensors, cfg) == []
+    for L, qs in zip([0, 2, 5], want):
+        got, g, bits = C.load_dense(tensors, f"model.layers.{L}", cfg)
+        assert (g, bits) == (gs, 4)
+        for a, b in zip(got, qs):
+            assert np.array_equal(a.w, b.w) and np.array_equal(a.scales, b.scales) and np.array_equal(a.biases, b.biases)
+    for m, qs in zip(C.load_device_mlps(str(tmp_path), device="cpu"), want):
+        assert (m.hidden, m.inter, m.group_size) == (128, 192, gs)
+        assert np.array_equal(m.down.w.numpy().view(np.uint32), qs[2].w)
+    with pytest.raises(C.CheckpointError, match="no quantized dense"):
+        C.load_dense(tensors, "model.layers.7", cfg)
+
+
+def test_moe_layers_are_not_dense_layers(tmp_path):
+    bw = S.host_block(QWEN_SHARED, 5)
+    _write_qwen(str(tmp_path), [bw], [0], QWEN_SHARED, 1)
+    tensors, cfg = C.open_checkpoint(str(tmp_path))
+    assert C.dense_layers(tensors, cfg) == []
+
+
+@pytest.mark.gpu
+def test_dense_blocks_of_a_checkpoint_on_gpu(tmp_path):
+    import torch
+    from mlx_rs_b200.synth import _q_to
+    from mlx_rs_b200 import ops
+    want = _write_dense(str(tmp_path), 64, [1, 3])
+    x = torch.randn(5, 128, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    for m, qs in zip(C.load_device_mlps(str(tmp_path)), want):
+        assert torch.equal(m(x), ops.gated_ffn(x, *(_q_to(q, "cuda") for q in qs)))
