@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_gemm_kernel(const __grid_const
         if (kk < G && ok) {
           const int s = kk % C::kStages;
           const uint32_t st = sbase + s * C::kStageBytes;
-          // the packed weights of K step kk: slot kk % kPackSlots, then release the slot
+          // the packed weights of K step kk: slot kk % kPackSlots
           const int ps = kk % kPackSlots;
           if (!__all_sync(0xffffffffu, mbar_wait(bar_pfull + 8 * ps, (kk / kPackSlots) & 1))) {
             ok = false;  // warp-uniform: the whole warp leaves together
@@ -451,8 +451,6 @@ __global__ void __launch_bounds__(kThreads, 1) tc_gemm_kernel(const __grid_const
             const uint32_t src = pack_s + (uint32_t)((ps * C::kMats + m) * kPackTileBytes + row * 32 + part * 8);
             asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(wr[m].x), "=r"(wr[m].y) : "r"(src) : "memory");
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar_pempty + 8 * ps);
           // dequantise A(kk) into stage s (freed: its empty barrier was awaited when B(kk) was issued)
 #pragma unroll
           for (int m = 0; m < C::kMats; ++m) {
@@ -474,6 +472,11 @@ __global__ void __launch_bounds__(kThreads, 1) tc_gemm_kernel(const __grid_const
           cp_wait<LA - 1>();
           fence_proxy_async();
           mbar_arrive(bar_full + 8 * s);
+          // Release the slot only here, where every lane's words have gone into the stores above:
+          // right after their loads nothing makes those return before the arrival, and the next
+          // copy could overwrite the slot under them.
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_pempty + 8 * ps);
           // issue B(kk + LA) into the stage MMA(kk + LA - kStages) releases
           const int kn = kk + LA;
           if (kn < G) {
