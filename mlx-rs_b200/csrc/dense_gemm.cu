@@ -77,7 +77,7 @@ struct Cfg {
   static constexpr int kDeqWarp = kEpiWarps;
   static constexpr int kTmaWarp = kDeqWarp + 4 * kGroups, kMmaWarp = kTmaWarp + 1, kPackWarp = kTmaWarp + 2;
   static constexpr int kThreads = (kMmaWarp + 1 + (PACKED ? 1 : 0)) * 32;
-  static constexpr int kStages = PACKED ? 5 : 6, kSlots = PACKED ? 8 : 0;
+  static constexpr int kStages = PACKED ? 4 : 6, kSlots = PACKED ? 8 : 0;
   static constexpr int kPackAt = kStages * kStageBytes;
   static constexpr int kStagingAt = kPackAt + kSlots * kPackBytes;
   static constexpr int kBarsAt = kStagingAt + kEpiWarps * kStageBuf;
@@ -88,8 +88,8 @@ struct Cfg {
   // apart; a slot belongs to one group.
   static_assert(kGroups <= kStages && (!PACKED || kSlots % (PACKED ? kGroups : 1) == 0), "phases told apart by parity");
   // the split form leaves its sums, rows of 256 floats and one 16-byte piece (so that a column
-  // of rows spreads over the banks), over the operand stages
-  static_assert(kBM * kSumPitch * 4 <= kPackAt, "sums over the stages");
+  // of rows spreads over the banks), over the operand stages and the packed slots
+  static_assert(kBM * kSumPitch * 4 <= kStagingAt, "sums over the stages and slots");
 };
 
 struct WeightSide {  // scales and biases of one operand pair's weights
@@ -700,7 +700,8 @@ __global__ void __launch_bounds__(Cfg<PACKED>::kThreads, 1) gemm_kernel(const __
       }
       tc_after();
       if constexpr (SPLIT) {
-        // the sums into this CTA's shared memory (the stages are free: every MMA has completed)
+        // the sums into this CTA's shared memory (stages and slots are free: every MMA has completed,
+        // and with them the last use of a slot)
         for (int q = warp >> 2; q < 2 * p.hb / 16; q += kChunkStep) {
           float d[16];
           tmem_ld16(acc + 16 * q, d);
