@@ -40,15 +40,16 @@ struct DequantArgs {
 cudaError_t launch_dequant(const DequantArgs& a, cudaStream_t st);
 // Tokens from which the products take weights dequantised once by launch_dequant; below, the
 // product's own warps dequantise each tile again for every 256 tokens. Per call in us, packed |
-// dequantised once, at 1024, 1536, 2048 and 4096 tokens:
-//   block forward, 2048 x 5632        73 | 78    89 | 92    109 | 112   214 | 203
-//   2048 -> 32768                    103 | 127  155 | 174   201 | 208   395 | 374
-//   2048 -> 2048                      17 | 18    20 | 19     24 | 22     43 | 32
-// and with the weights' rows summed (the gradients), where the 16-bit product is the faster:
-//   block forward and backward       166 | 181  248 | 213   263 | 253   506 | 449
-//   5632 -> 2048                      36 | 33    54 | 41     55 | 42    104 | 74
-// The fifth tile of 256 tokens is what turns the second pair.
-constexpr int64_t kWideMinM = 2048, kWideMinRowsM = 1025;
+// dequantised once, at 1024, 1536, 2048, 2560 and 4096 tokens:
+//   block forward, 2048 x 5632, group 64     71 | 82    91 | 95   110 | 114  148 | 142  217 | 208
+//   2048 -> 32768, group 128                103 | 130  157 | 179  205 | 214  256 | 260  402 | 385
+//   2048 -> 2048, group 32                   17 | 18    18 | 20    21 | 23    30 | 25    36 | 32
+// so from the ninth tile of 256 tokens on; and with the weights' rows summed (the gradients):
+//   block 2048 x 5632 and gradients         168 | 184  219 | 216  266 | 260  365 | 353  520 | 464
+//   block 2048 x 768 and gradients           54 | 62    61 | 66    74 | 70    86 | 79   116 | 98
+//   5632 -> 2048, group 32                   28 | 34    40 | 41    41 | 43    79 | 73    80 | 74
+// where the two are level from the fifth tile to the eighth and the second is ahead above.
+constexpr int64_t kWideMinM = 2049, kWideMinRowsM = 1025;
 
 // out[r][0..cols) = x[r][0..cols), rows ld elements apart, the rest of each row zero
 // (dense_pad.cu).

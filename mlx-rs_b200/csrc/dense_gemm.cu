@@ -33,17 +33,21 @@
 // Every wait is bounded (2 s): on expiry the CTA records a code in the device's status word,
 // stops working and leaves through the same barriers as the rest of its cluster.
 //
-// What bounds it. Packed: the dequantising warps, 0.32 / 0.53 us per K step at 64 / 128 weight
-// rows per CTA, and for few steps the 4.5 us of a round's start, first loads and epilogue: 512
-// tokens of the block 2048 x 5632 44.7 us (0.79 PFLOP/s), 5632 -> 2048 22.7 us with the rows
-// summed. Wide: the tensor pipe, active 87 to 93 % of the cycles in the plain and gated products
-// (block 2048 x 5632, 4096 tokens, with the dequantisation: forward 203 us, 1.40 PFLOP/s; with
-// the gradients 459 us, 1.24). In the product with the gated gradient it is active 57 %: beside
-// the operands g and u are read and dg and du written, 1.1 GB through L2 at 11.7 TB/s. Measured
-// against it: weights left in 16 bits by a launch before for every size (64.6 us for 512
-// tokens), cluster-scope arrivals on the step barriers (twice the time per step: each is a
-// fence over global memory), 12 or 16 epilogue warps in the gated gradient and its g and u one
-// or two chunks ahead (all within 0.6 %).
+// What bounds it. Packed: not the tensor pipe (active 47 % in the gated product of 512 tokens)
+// nor the issue slots (46 %): a K step takes 0.3 / 0.5 us at 64 / 128 weight rows per CTA, of
+// which a group of warps dequantises for about 40 %, waits for its stage for 20 % and spends
+// 15 to 20 % on issuing the next scales' loads; and a round has 4.5 us of start, first loads and
+// epilogue. 512 tokens of the block 2048 x 5632 44.7 us (0.79 PFLOP/s), 5632 -> 2048 20.4 us with
+// the rows summed. Wide: the tensor pipe, active 87 to 93 % of the cycles in the plain and gated
+// products (block 2048 x 5632, 4096 tokens, with the dequantisation: forward 208 us, 1.36
+// PFLOP/s; with the gradients 464 us, 1.22). In the product with the gated gradient it is active
+// 57 %: beside the operands g and u are read and dg and du written, 1.1 GB through L2 at 11.7
+// TB/s. Measured against it: weights left in 16 bits by a launch before for every size (64.6 us
+// for 512 tokens), cluster-scope arrivals on the step barriers (twice the time per step: each is
+// a fence over global memory), 12 or 16 epilogue warps in the gated gradient and its g and u one
+// or two chunks ahead (all within 0.6 %); in the packed form five stages instead of four (up to
+// 2.5 % slower), scales staged in shared memory by the packing warp (9 to 88 % slower), rows
+// dequantised into registers before the wait for their stage (1 to 5 % slower).
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -905,9 +909,12 @@ struct Plan {
 // tiles, by a line fitted to every allowed pair of 16 products (64 to 800 tokens, 768 to 5632
 // summed, both directions). With r weight rows per CTA a K step costs 0.11 + 0.21 r / 64 us, a
 // round 4.5 us (its start and epilogue), the exchange of a split's sums 1 + 1.4 r / 64 us. The
-// pair taken is within 1.5 % of the fastest measured one for those 16, and within 3.4 % (0.3 %
-// in the mean) for 16 others that had no part in the fit (40 to 1500 tokens, 1024 to 7168
-// summed). Over 16-bit weights a step takes 0.36 us at 128 rows and no less than 0.2.
+// line was fitted before the last steps of the kernel; with it as it is the pair taken is 1.3 %
+// (group 32) and 1.9 % (128) behind the fastest measured one in the mean of those 16, 11 % at
+// worst (512 tokens, 5632 -> 2048, rows summed, group 128: 21.3 us, 19.1 with 128 x 3 splits), and
+// 1.4 % and 10 % (group 32) for 16 others that had no part in the fit (40 to 1500 tokens). A new
+// fit and a search over the five constants found none better. Over 16-bit weights a step takes
+// 0.36 us at 128 rows and no less than 0.2.
 Plan plan(int64_t M, int N, int K, int pairs, bool gated, bool rows_k, bool wide) {
   Plan best{};
   double least = 0;
