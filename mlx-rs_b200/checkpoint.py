@@ -300,18 +300,39 @@ def load_dense(tensors: _Tensors, layer_prefix: str, cfg: dict):
     return qs, gs, bits.pop()
 
 
+# names of the activations a dense block has, as configurations write them; "gelu" alone is the
+# error-function form there, which it does not have
+_ACTIVATIONS = {"silu": "silu", "swish": "silu", "gelu_pytorch_tanh": "gelu", "gelu_new": "gelu", "gelu_tanh": "gelu"}
+
+
+def dense_activation(cfg: dict) -> str:
+    """DenseMlp's activation by config.json: hidden_activation, else hidden_act, at the top or in
+    text_config; SiLU where neither is given, as in the families this package reads, Gemma's
+    excepted. Any other activation is refused."""
+    for c in (cfg, cfg.get("text_config") or {}):
+        name = c.get("hidden_activation") or c.get("hidden_act")
+        if name is not None:
+            if name not in _ACTIVATIONS:
+                raise CheckpointError(f"activation {name!r}: dense blocks have {sorted(_ACTIVATIONS)}")
+            return _ACTIVATIONS[name]
+    if str(cfg.get("model_type", "")).startswith("gemma"):
+        raise CheckpointError(f"{cfg['model_type']}: config.json names no activation (hidden_activation)")
+    return "silu"
+
+
 def load_device_mlps(directory: str, device="cuda", layers: Optional[List[int]] = None, prefix: str = "model.layers"):
     """The checkpoint's dense feed-forward blocks (default: of every layer that has one) as
-    DenseMlp blocks ready to call (weights copied bit for bit; SiLU)."""
+    DenseMlp blocks ready to call (weights copied bit for bit, the configuration's activation)."""
     from .block import DenseMlp
     from .synth import _q_to
     tensors, cfg = open_checkpoint(directory)
     if layers is None:
         layers = dense_layers(tensors, cfg, prefix)
+    act = dense_activation(cfg) if layers else None
     out = []
     for i in layers:
         qs, gs, bits = load_dense(tensors, f"{prefix}.{i}", cfg)
-        out.append(DenseMlp(*(_q_to(q, device) for q in qs), group_size=gs, bits=bits))
+        out.append(DenseMlp(*(_q_to(q, device) for q in qs), activation=act, group_size=gs, bits=bits))
     return out
 
 
@@ -348,4 +369,5 @@ def load_device_blocks(directory: str, device="cuda", layers: Optional[List[int]
 
 
 __all__ = ["CheckpointError", "read_safetensors", "write_safetensors", "infer_bits", "block_config",
-           "load_block", "load_blocks", "load_device_blocks", "moe_layers", "dense_layers", "load_dense", "load_device_mlps", "open_checkpoint", "SCORING_SIGMOID_BIAS_SELECT"]
+           "load_block", "load_blocks", "load_device_blocks", "moe_layers", "dense_layers", "load_dense",
+           "dense_activation", "load_device_mlps", "open_checkpoint", "SCORING_SIGMOID_BIAS_SELECT"]

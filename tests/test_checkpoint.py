@@ -314,3 +314,26 @@ def test_dense_blocks_of_a_checkpoint_on_gpu(tmp_path):
     x = torch.randn(5, 128, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
     for m, qs in zip(C.load_device_mlps(str(tmp_path)), want):
         assert torch.equal(m(x), ops.gated_ffn(x, *(_q_to(q, "cuda") for q in qs)))
+
+
+@pytest.mark.parametrize("conf,want", [
+    ({}, "silu"), ({"hidden_act": "silu"}, "silu"), ({"hidden_act": "swish"}, "silu"),
+    ({"hidden_act": "gelu_pytorch_tanh"}, "gelu"), ({"hidden_act": "gelu_new"}, "gelu"),
+    ({"model_type": "gemma3_text", "hidden_activation": "gelu_pytorch_tanh"}, "gelu"),
+    # the newer entry holds where both are there; an empty one names nothing
+    ({"hidden_act": "gelu", "hidden_activation": "gelu_pytorch_tanh"}, "gelu"),
+    ({"hidden_act": "silu", "hidden_activation": None}, "silu"),
+    ({"text_config": {"hidden_activation": "gelu_pytorch_tanh"}}, "gelu")])
+def test_dense_blocks_have_the_configurations_activation(tmp_path, conf, want):
+    _write_dense(str(tmp_path), 32, [0], conf)
+    (m,) = C.load_device_mlps(str(tmp_path), device="cpu")
+    assert m.activation == want
+
+
+@pytest.mark.parametrize("conf", [{"hidden_act": "gelu"}, {"hidden_act": "relu"}, {"hidden_activation": "relu2"},
+                                  {"model_type": "gemma2"}])
+def test_dense_blocks_with_another_activation_are_refused(tmp_path, conf):
+    """The error-function GELU and other activations, and a family of GELU models that names none."""
+    _write_dense(str(tmp_path), 32, [0], conf)
+    with pytest.raises(C.CheckpointError, match="activation"):
+        C.load_device_mlps(str(tmp_path), device="cpu")
