@@ -25,10 +25,11 @@ Mirrors how the reference loads the block's tensors (no MLX needed):
     norm_topk_prob, quantization.{group_size, bits}); bits are re-inferred from the packed
     and scale shapes as infer_bits does (:221-239).
 
-The device path computes with bf16 scales, biases and expert_bias, the type MLX 4-bit
+The MoE blocks compute with bf16 scales, biases and expert_bias, the type MLX 4-bit
 checkpoints of these models store them in; the reference keeps tensors in their stored
 type (VarBuilder::get casts nothing), so a checkpoint with F16 or F32 scales is rounded to
-bf16 here (nearest even) and then differs from the reference by that rounding.
+bf16 here (nearest even) and then differs from the reference by that rounding. The dense
+blocks keep bf16 and F16 as they are, and refuse F32 values that bf16 does not hold.
 """
 from __future__ import annotations
 
@@ -42,7 +43,7 @@ from typing import Dict, Iterable, List, Optional
 import numpy as np
 
 from .synth import (SCORING_SIGMOID_BIAS_SELECT, SCORING_SOFTMAX, SCORING_SOFTMAX_BIAS, BlockWeights, MoeConfig,
-                    QWeight, f32_to_bf16_bits)
+                    QWeight, bf16_bits_to_f32, f32_to_bf16_bits)
 
 _DTYPES = {
     "U8": np.uint8, "I8": np.int8, "U16": np.uint16, "I16": np.int16, "U32": np.uint32, "I32": np.int32,
@@ -149,6 +150,24 @@ class _Tensors:
         s = self.get(prefix + ".scales")
         b = self.get(prefix + ".biases") if self.has(prefix + ".biases") else None
         return QWeight(np.asarray(w.array).view(np.uint32), _to_bf16(s), None if b is None else _to_bf16(b))
+
+    def qweight_exact(self, prefix) -> QWeight:
+        """The matrix with its scales and biases in the type they are stored in, bf16 (as bits) or
+        f16; f32 where bf16 holds every value."""
+        w = self.get(prefix + ".weight")
+        if w.dtype not in ("U32", "I32"):
+            raise CheckpointError(f"{prefix}.weight is {w.dtype}: not a packed quantized weight")
+        parts = []
+        for name in (prefix + ".scales", prefix + ".biases"):
+            if name.endswith("biases") and not self.has(name):
+                parts.append(None)
+                continue
+            e = self.get(name)
+            a = np.asarray(e.array) if e.dtype == "F16" else _to_bf16(e)
+            if e.dtype not in ("F16", "BF16") and not np.array_equal(bf16_bits_to_f32(a), np.asarray(e.array)):
+                raise CheckpointError(f"{name}: {e.dtype} values that bf16 does not hold")
+            parts.append(a)
+        return QWeight(np.asarray(w.array).view(np.uint32), *parts)
 
     def stacked(self, prefix, proj, n) -> QWeight:
         """Per-expert tensors <prefix>.<e>.<proj>.* stacked along a new axis 0."""
@@ -287,11 +306,14 @@ def dense_layers(tensors: _Tensors, cfg: dict, prefix: str = "model.layers") -> 
 
 
 def load_dense(tensors: _Tensors, layer_prefix: str, cfg: dict):
-    """((gate, up, down), group_size, bits) of a layer's dense feed-forward block."""
+    """((gate, up, down), group_size, bits) of a layer's dense feed-forward block; scales and
+    biases as stored, bf16 (bits, uint16) or float16."""
     found = _dense_prefixes(tensors, layer_prefix)
     if found is None:
         raise CheckpointError(f"{layer_prefix}: no quantized dense feed-forward block")
-    qs = tuple(tensors.qweight(f) for f in found)
+    qs = tuple(tensors.qweight_exact(f) for f in found)
+    if len({a.dtype for q in qs for a in (q.scales, q.biases) if a is not None}) != 1:
+        raise CheckpointError(f"{layer_prefix}: scales and biases of several types")
     quant = cfg.get("quantization") or cfg.get("quantization_config") or {}
     gs = int(quant.get("group_size", 64))
     bits = {infer_bits(q.w.shape, q.scales.shape, gs, int(quant.get("bits", 4))) for q in qs}

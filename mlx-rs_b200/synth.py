@@ -153,6 +153,8 @@ def _t(a, device):
         return torch.from_numpy(a.view(np.int16)).to(device).view(torch.bfloat16)
     if a.dtype == np.uint32:
         return torch.from_numpy(a.view(np.int32)).to(device)
+    if a.dtype == np.float16:
+        return torch.from_numpy(a).to(device)
     raise TypeError(a.dtype)
 
 

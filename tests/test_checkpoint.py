@@ -337,3 +337,54 @@ def test_dense_blocks_with_another_activation_are_refused(tmp_path, conf):
     _write_dense(str(tmp_path), 32, [0], conf)
     with pytest.raises(C.CheckpointError, match="activation"):
         C.load_device_mlps(str(tmp_path), device="cpu")
+
+
+def _retype(d, kind, only=None):
+    """The same checkpoint with its scales and biases (or those whose name has `only`) in another type."""
+    path = os.path.join(d, "model.safetensors")
+    old = {k: (e.dtype, np.array(e.array)) for k, e in C.read_safetensors(path).items()}
+    new, types = {}, {}
+    for k, (dt, a) in old.items():
+        if k.endswith((".scales", ".biases")) and (only is None or only in k):
+            a, dt = S.bf16_bits_to_f32(a).astype(kind) * kind(1.001), {np.float16: "F16", np.float32: "F32"}[kind]
+        new[k], types[k] = a, dt
+    C.write_safetensors(path, new, types)
+    return new
+
+
+def test_dense_blocks_keep_f16_scales(tmp_path):
+    """Bit for bit: b is near -8 s, so that rounding s and b apart moves a weight by percents of s."""
+    import torch
+    _write_dense(str(tmp_path), 64, [0])
+    t = _retype(str(tmp_path), np.float16)
+    (m,) = C.load_device_mlps(str(tmp_path), device="cpu")
+    assert m.dtype == torch.float16
+    for name in ("gate", "up", "down"):
+        q = getattr(m, name)
+        for part in ("scales", "biases"):
+            assert np.array_equal(getattr(q, part).numpy(), t[f"model.layers.0.mlp.{name}_proj.{part}"])
+
+
+def test_dense_blocks_refuse_scales_they_cannot_keep(tmp_path):
+    _write_dense(str(tmp_path), 64, [0])
+    _retype(str(tmp_path), np.float32, "up_proj")
+    with pytest.raises(C.CheckpointError, match="up_proj.scales"):
+        C.load_device_mlps(str(tmp_path), device="cpu")
+
+
+def test_dense_blocks_refuse_scales_of_several_types(tmp_path):
+    _write_dense(str(tmp_path), 64, [0])
+    _retype(str(tmp_path), np.float16, "down_proj.biases")
+    with pytest.raises(C.CheckpointError, match="types"):
+        C.load_device_mlps(str(tmp_path), device="cpu")
+
+
+def test_dense_blocks_take_f32_scales_that_bf16_holds(tmp_path):
+    import torch
+    want = _write_dense(str(tmp_path), 32, [0])
+    path = os.path.join(str(tmp_path), "model.safetensors")
+    t = {k: np.array(e.array) for k, e in C.read_safetensors(path).items()}
+    C.write_safetensors(path, {k: S.bf16_bits_to_f32(a) if k.endswith((".scales", ".biases")) else a for k, a in t.items()})
+    (m,) = C.load_device_mlps(str(tmp_path), device="cpu")
+    assert m.dtype == torch.bfloat16
+    assert np.array_equal(m.up.scales.view(torch.int16).numpy().view(np.uint16), want[0][1].scales)
