@@ -6,8 +6,10 @@ namespace moe {
 
 namespace {
 
-__global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* __restrict__ x, int64_t rows, int64_t cols,
-                                                       uint16_t* __restrict__ out, int64_t ld) {
+// x is not __restrict__: the launch before may write it while this kernel already runs, so it may
+// not be read by read-only loads.
+__global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* x, int64_t rows, int64_t cols, uint16_t* out,
+                                                       int64_t ld) {
   pdl_wait();
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows * ld) return;

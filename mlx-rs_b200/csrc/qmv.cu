@@ -188,7 +188,9 @@ __global__ void __maxnreg__(NC == 4 ? 128 : 96) qmv_kernel(const __grid_constant
     pdl_trigger();
   }
 
-  // Columns of the MMA without a token read the last token again and are not stored.
+  // Columns of the MMA without a token read the last token again and are not stored. The tokens
+  // are read by plain loads: the launch before may write them while this kernel already runs, so
+  // they are not read-only for its lifetime, which the read-only loads of the weights ask for.
   const int mbase = blockIdx.y * kCols;
   const uint16_t* xr[NC];
 #pragma unroll
@@ -224,7 +226,7 @@ __global__ void __maxnreg__(NC == 4 ? 128 : 96) qmv_kernel(const __grid_constant
           uint32_t e[NC][4];
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
-            const uint4 q = __ldg(reinterpret_cast<const uint4*>(xr[c] + xoff + gr * G + j * 8));
+            const uint4 q = *reinterpret_cast<const uint4*>(xr[c] + xoff + gr * G + j * 8);
             e[c][0] = __byte_perm(q.x, q.z, 0x5410), e[c][1] = __byte_perm(q.x, q.z, 0x7632);
             e[c][2] = __byte_perm(q.y, q.w, 0x5410), e[c][3] = __byte_perm(q.y, q.w, 0x7632);
           }
