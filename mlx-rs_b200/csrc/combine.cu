@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(256) combine_kernel(CombineArgs a) {
   *reinterpret_cast<uint4*>(a.out + (size_t)t * a.H + h) = ov;
 }
 
-__global__ void __launch_bounds__(256) rms_norm_kernel(const uint16_t* __restrict__ x,
+__global__ void __launch_bounds__(256) rms_norm_kernel(const uint16_t* x,
                                                        const uint16_t* __restrict__ w, float eps,
                                                        int64_t rows, int dim, uint16_t* __restrict__ out) {
   const int lane = threadIdx.x & 31;
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(256) combine_f32_kernel(CombineArgs a) {
 // out[r] = f32(bf16(x[r] * rsqrt(mean(x[r]^2) + eps))) * root * f32(scale): the Gemma4
 // router's input (gemma4.rs:911-919: fast_rms_norm with a ones weight, then two multiplies
 // by 0-d f32 arrays, which makes the rest of the router f32). The norm as rms_norm_kernel.
-__global__ void __launch_bounds__(256) gemma_router_input_kernel(const uint16_t* __restrict__ x,
+__global__ void __launch_bounds__(256) gemma_router_input_kernel(const uint16_t* x,
                                                                  const uint16_t* __restrict__ scale, float root,
                                                                  float eps, int64_t rows, int dim,
                                                                  float* __restrict__ out) {

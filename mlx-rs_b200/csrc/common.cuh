@@ -82,7 +82,9 @@ MOE_DEV uint16_t gelu_mul_bf16(float g, float u) {
 // Programmatic dependent launch: kernels of the block are launched so that each may
 // start while its predecessor in the stream drains. pdl_wait() blocks until the
 // predecessor grid has completed and its writes are visible (a no-op when the kernel
-// was launched normally); it must precede every read of a predecessor's output.
+// was launched normally); it must precede every read of a predecessor's output, and such
+// reads are plain loads: what a predecessor may still write is not read-only for this
+// kernel's lifetime, which __ldg and const __restrict__ pointers claim.
 // pdl_trigger() lets the next kernel start launching once every CTA has called it.
 MOE_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 MOE_DEV void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }

@@ -79,7 +79,7 @@ MOE_DEV void router_tile(const RouterArgs& a, int row0, int t0, int lane) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const int tok = t0 + t;
-        xv[t] = tok < a.T ? __ldg(reinterpret_cast<const uint4*>(a.x + (size_t)tok * a.K + c * 32 + word * 8))
+        xv[t] = tok < a.T ? *reinterpret_cast<const uint4*>(a.x + (size_t)tok * a.K + c * 32 + word * 8)
                           : make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
@@ -183,8 +183,8 @@ MOE_DEV void router_tile_f32(const RouterArgs& a, int row0, int t0, int lane) {
         const int tok = t0 + t;
         if (tok < a.T) {
           const float4* p = reinterpret_cast<const float4*>(a.xf + (size_t)tok * a.K + c * 32 + word * 8);
-          xl[t] = __ldg(p);
-          xh[t] = __ldg(p + 1);
+          xl[t] = p[0];
+          xh[t] = p[1];
         } else {
           xl[t] = xh[t] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }

@@ -70,8 +70,8 @@ __global__ void __launch_bounds__(kRsMaxWarps * 32, 2) router_logits_smem_kernel
   for (int i = threadIdx.x; i < (kRsTok / 2) * nkb; i += blockDim.x) {
     const int tp = i / nkb, kb = i - tp * nkb;
     uint4 va = make_uint4(0, 0, 0, 0), vb = make_uint4(0, 0, 0, 0);
-    if (2 * tp < nt) va = __ldg(reinterpret_cast<const uint4*>(a.x + (size_t)(t0 + 2 * tp) * K) + kb);
-    if (2 * tp + 1 < nt) vb = __ldg(reinterpret_cast<const uint4*>(a.x + (size_t)(t0 + 2 * tp + 1) * K) + kb);
+    if (2 * tp < nt) va = *(reinterpret_cast<const uint4*>(a.x + (size_t)(t0 + 2 * tp) * K) + kb);
+    if (2 * tp + 1 < nt) vb = *(reinterpret_cast<const uint4*>(a.x + (size_t)(t0 + 2 * tp + 1) * K) + kb);
     const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {

@@ -14,7 +14,8 @@ def _code(name):
 
 
 @pytest.mark.parametrize("name,tokens", [("qmv.cu", r"xr|a\.x|residual"), ("rope.cu", r"a\.x|xb|offsets"),
-                                         ("dense_gemm.cu", r"residual|e\.gate|e\.up")])
+                                         ("dense_gemm.cu", r"residual|e\.gate|e\.up"),
+                                         ("route.cuh", r"a\.x|a\.xf|p"), ("router.cu", r"a\.x")])
 def test_tokens_are_not_read_through_the_read_only_path(name, tokens):
     for call in re.findall(r"(?:__ldg|ldg_\w+)(?:<\w+>)?\(([^;]*);", _code(name)):
         assert not re.search(rf"\b(?:{tokens})\b", call), call
@@ -22,6 +23,12 @@ def test_tokens_are_not_read_through_the_read_only_path(name, tokens):
 
 def test_padded_rows_are_not_read_through_the_read_only_path():
     assert "__restrict__" not in _code("dense_pad.cu") and "__ldg" not in _code("dense_pad.cu")
+
+
+@pytest.mark.parametrize("kernel", ["rms_norm_kernel", "gemma_router_input_kernel"])
+def test_norms_do_not_take_their_input_as_read_only(kernel):
+    first = re.search(rf"{kernel}\(([^,]*),", _code("combine.cu")).group(1)
+    assert first.split() == ["const", "uint16_t*", "x"]
 
 
 @pytest.mark.gpu
