@@ -10,6 +10,8 @@ import ctypes as C
 import os
 import threading
 
+import torch
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 library_path = os.path.join(_HERE, "libmoe_b200.so")
 
@@ -161,12 +163,16 @@ def library():
     return _lib
 
 
+# Whether torch's current stream is being captured.
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: False)
+
+
 class Context:
-    """A moe_ctx on one CUDA device; follows torch's current stream per call."""
+    """A moe_ctx on one CUDA device, used by one thread; follows torch's current stream per call."""
 
     def __init__(self, device: int):
         self.device = device
-        self.lock = threading.Lock()  # held from binding a stream to the end of the call on it
+        self.captured = False  # a graph may hold calls on it, and with them its scratch
         h = C.c_void_p()
         rc = library().moe_ctx_create(device, None, C.byref(h))
         if rc != MOE_OK:
@@ -175,6 +181,8 @@ class Context:
 
     def bind_stream(self, stream_handle: int):
         library().moe_ctx_set_stream(self.handle, stream_handle)
+        if not self.captured and _capturing():
+            self.captured = True
 
     def check(self, fn: str, rc: int):
         if rc != MOE_OK:
@@ -193,12 +201,33 @@ class Context:
             pass
 
 
-_contexts: dict[int, Context] = {}
+_kept: list[Context] = []  # contexts of ended threads whose scratch captured graphs may use
+
+
+class _Contexts(dict):
+    """One thread's contexts by device. They end with the thread (freeing the scratch waits for the
+    work that uses it), except those that a graph captured there may still use."""
+
+    def __del__(self):
+        try:
+            _kept.extend(c for c in self.values() if c.captured)
+        except Exception:  # the interpreter is going
+            pass
+
+
+class _Thread(threading.local):
+    def __init__(self):
+        self.contexts = _Contexts()
+
+
+_thread = _Thread()
 
 
 def context_for(device_index: int) -> Context:
-    ctx = _contexts.get(device_index)
+    """This thread's context of a device: a moe_ctx has one stream at a time and one scratch, so two
+    threads may not share it."""
+    contexts = _thread.contexts
+    ctx = contexts.get(device_index)
     if ctx is None:
-        ctx = Context(device_index)
-        _contexts[device_index] = ctx
+        ctx = contexts[device_index] = Context(device_index)
     return ctx

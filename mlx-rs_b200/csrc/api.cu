@@ -82,8 +82,25 @@ struct Carve {
   }
 };
 
-int ensure_scratch(moe_ctx* ctx, size_t bytes) {
-  if (bytes <= ctx->scratch_bytes) return MOE_OK;
+// Lets this thread allocate and free while a stream is being captured (by itself or another).
+struct RelaxedCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
+// Zeroes the status block of a new scratch on a stream of its own: the context's may be captured.
+cudaError_t clear_status_block(void* scratch) {
+  cudaStream_t s = nullptr;
+  cudaError_t e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+  if (e != cudaSuccess) return e;
+  e = cudaMemsetAsync(scratch, 0, 256, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  const cudaError_t d = cudaStreamDestroy(s);
+  return e != cudaSuccess ? e : d;
+}
+
+int alloc_scratch(moe_ctx* ctx, size_t bytes) {
   if (ctx->scratch) {
     // cudaFree waits for work in flight that may still use the old buffer.
     cudaFree(ctx->scratch);
@@ -98,9 +115,20 @@ int ensure_scratch(moe_ctx* ctx, size_t bytes) {
   }
   ctx->scratch_bytes = want;
   // the first word holds the device status (bounded waits that expired); start clean
-  e = cudaMemset(ctx->scratch, 0, 256);
+  e = clear_status_block(ctx->scratch);
   if (e != cudaSuccess) return fail(ctx, MOE_ERR_CUDA, "scratch status reset failed: %s", cudaGetErrorString(e));
   return MOE_OK;
+}
+
+int ensure_scratch(moe_ctx* ctx, size_t bytes) {
+  if (bytes <= ctx->scratch_bytes) return MOE_OK;
+  // A context's first scratch may come in a capture: a thread that captures what another one
+  // warmed up. Growing it there is refused by the runtime, since captured calls use the old one.
+  if (!ctx->scratch) {
+    RelaxedCapture relaxed;
+    return alloc_scratch(ctx, bytes);
+  }
+  return alloc_scratch(ctx, bytes);
 }
 
 int check_quant(moe_ctx* ctx, const char* fn, int64_t K, int group_size, int bits) {
@@ -924,6 +952,7 @@ void moe_ctx_destroy(moe_ctx* ctx) {
   if (!ctx) return;
   if (ctx->scratch || ctx->side) {
     DeviceGuard g(ctx->device);
+    RelaxedCapture relaxed;
     if (ctx->scratch) cudaFree(ctx->scratch);
     if (ctx->side) cudaStreamDestroy(ctx->side);
     if (ctx->fork_ev) cudaEventDestroy(ctx->fork_ev);

@@ -67,12 +67,13 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 
 
 def _context(fn, t):
-    """The context of the tensor's device. Its lock is held from binding torch's current
-    stream to the end of the call: another thread may bind another stream."""
+    """This thread's context of the tensor's device, on torch's current stream."""
     index = t.get_device()
     if index < 0:
         raise MlxError(fn, 1, "tensors must be on a CUDA device")
-    return context_for(index)
+    ctx = context_for(index)
+    ctx.bind_stream(_raw_stream(index))
+    return ctx
 
 
 def _workspace(nbytes, device):
@@ -140,12 +141,10 @@ def _quantized_matmul_ex(x, w, scales, biases, transpose, group_size, bits):
     need = _qmm_workspace(dt, M, K, N, tr, group_size, bits)
     ws = _workspace(need, x.device) if need else None
     ctx = _context(fn, x)
-    with ctx.lock:
-        ctx.bind_stream(_raw_stream(ctx.device))
-        rc = library().moe_quantized_matmul_ex(ctx.handle, dt, x.data_ptr(), M, K, w.data_ptr(), scales.data_ptr(),
-                                               biases.data_ptr() if biases is not None else None, N, tr, group_size, bits,
-                                               out.data_ptr(), ws.data_ptr() if need else None, need)
-        ctx.check(fn, rc)
+    rc = library().moe_quantized_matmul_ex(ctx.handle, dt, x.data_ptr(), M, K, w.data_ptr(), scales.data_ptr(),
+                                           biases.data_ptr() if biases is not None else None, N, tr, group_size, bits,
+                                           out.data_ptr(), ws.data_ptr() if need else None, need)
+    ctx.check(fn, rc)
     return out
 
 
@@ -300,13 +299,11 @@ def _ffn_forward(cfg, wts, x, residual, save):
     need = _ffn_workspace(cfg.hidden, cfg.inter, cfg.group_size, cfg.dtype, T, 0)
     ws = _workspace(need, x.device) if need else None
     ctx = _context(fn, x)
-    with ctx.lock:
-        ctx.bind_stream(_raw_stream(ctx.device))
-        rc = library().moe_gated_ffn_forward(ctx.handle, cfg, wts, x.data_ptr(), T,
-                                             None if residual is None else residual.data_ptr(),
-                                             g.data_ptr() if save else None, u.data_ptr() if save else None,
-                                             out.data_ptr(), ws.data_ptr() if need else None, need)
-        ctx.check(fn, rc)
+    rc = library().moe_gated_ffn_forward(ctx.handle, cfg, wts, x.data_ptr(), T,
+                                         None if residual is None else residual.data_ptr(),
+                                         g.data_ptr() if save else None, u.data_ptr() if save else None,
+                                         out.data_ptr(), ws.data_ptr() if need else None, need)
+    ctx.check(fn, rc)
     return (out, g, u) if save else out
 
 
@@ -323,12 +320,10 @@ def _ffn_backward(cfg, wts, g, u, dy):
     need = _ffn_workspace(cfg.hidden, cfg.inter, cfg.group_size, cfg.dtype, T, 1)
     ws = _workspace(need, dy.device) if need else None
     ctx = _context(fn, dy)
-    with ctx.lock:
-        ctx.bind_stream(_raw_stream(ctx.device))
-        rc = library().moe_gated_ffn_backward(ctx.handle, cfg, wts, g.data_ptr(), u.data_ptr(), dy.data_ptr(), T,
-                                              dgate.data_ptr(), dup.data_ptr(), dx.data_ptr(),
-                                              ws.data_ptr() if need else None, need)
-        ctx.check(fn, rc)
+    rc = library().moe_gated_ffn_backward(ctx.handle, cfg, wts, g.data_ptr(), u.data_ptr(), dy.data_ptr(), T,
+                                          dgate.data_ptr(), dup.data_ptr(), dx.data_ptr(),
+                                          ws.data_ptr() if need else None, need)
+    ctx.check(fn, rc)
     return dx, dgate, dup
 
 
@@ -416,9 +411,7 @@ def fast_rope(x, dims, traditional=False, base=10000.0, scale=1.0, offset=0, fre
         raise MlxError(fn, 1, f"freqs: contiguous float32 [{dims // 2}] on {x.device} expected")
     cfg = RopeConfig(dt, dims, 1 if traditional else 0, 1 if inverse else 0, 0.0 if base is None else base, scale, mscale)
     ctx = _context(fn, x)
-    with ctx.lock:
-        ctx.bind_stream(_raw_stream(ctx.device))
-        rc = library().moe_fast_rope(ctx.handle, cfg, x.data_ptr(), _I64x3(*xs[:3]), B, H, L, D, off, offs, offs_bits,
-                                     None if freqs is None else freqs.data_ptr(), out.data_ptr(), _I64x3(*os_[:3]))
-        ctx.check(fn, rc)
+    rc = library().moe_fast_rope(ctx.handle, cfg, x.data_ptr(), _I64x3(*xs[:3]), B, H, L, D, off, offs, offs_bits,
+                                 None if freqs is None else freqs.data_ptr(), out.data_ptr(), _I64x3(*os_[:3]))
+    ctx.check(fn, rc)
     return out
