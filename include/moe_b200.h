@@ -315,12 +315,20 @@ int moe_block_profile(moe_ctx* ctx, const moe_block_config* cfg, const moe_block
 
 /*
  * Status word of the context's device work: nonzero after a bounded device-side wait
- * expired in a kernel launched on this context (the kernel then stopped early and its
- * outputs are invalid; for the dense operators' kernels: launched by any context on its
- * device). Synchronises the context's stream. No counterpart in the
+ * expired (the kernel then stopped early and its outputs are invalid). Bits 0 to 15: in a
+ * MoE kernel launched on this context, from then on. Bits 16 to 31: in a kernel of the dense
+ * operators, launched by any context on its device; these are reported once and cleared.
+ * Synchronises the context's stream; not in a capture. No counterpart in the
  * reference (MLX kernels do not wait on barriers with a time limit).
  */
 int moe_ctx_status(moe_ctx* ctx, int32_t* status);
+
+/*
+ * Lets one of the dense operators' bounded waits expire, on a barrier of its own that nothing
+ * arrives at, after limit_us (1 to 1000000) microseconds: a host can test what it does with a
+ * nonzero status (bit 24). Nothing else is touched.
+ */
+int moe_ctx_expire_wait(moe_ctx* ctx, int64_t limit_us);
 
 /*
  * Expert parallelism (EP) over `world` ranks, one process and one context per GPU.

@@ -114,6 +114,7 @@ SIGNATURES = {
                                   C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
                                   C.c_void_p]),
     "moe_ctx_status": (C.c_int, [C.c_void_p, C.POINTER(C.c_int32)]),
+    "moe_ctx_expire_wait": (C.c_int, [C.c_void_p, C.c_int64]),
     "moe_ep_route": (C.c_int, [C.c_void_p, C.POINTER(BlockConfig), C.POINTER(BlockWeights),
                                C.c_void_p, C.c_int64, C.c_void_p]),
     "moe_ep_experts": (C.c_int, [C.c_void_p, C.POINTER(BlockConfig), C.POINTER(BlockWeights),

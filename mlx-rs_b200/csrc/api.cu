@@ -1512,13 +1512,22 @@ int moe_ctx_status(moe_ctx* ctx, int32_t* status) {
   *status = 0;
   DeviceGuard g(ctx->device);
   if (!g.ok) return fail(ctx, MOE_ERR_CUDA, "cudaSetDevice(%d) failed", ctx->device);
-  int32_t dense = 0;  // the dense operators' products share one word per device
-  MOE_CUDA(ctx, moe::dense_gemm_status(&dense, ctx->stream));
-  if (ctx->scratch) {
-    MOE_CUDA(ctx, cudaMemcpyAsync(status, ctx->scratch, sizeof(int32_t), cudaMemcpyDeviceToHost, ctx->stream));
-    MOE_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
-  }
-  *status |= dense;
+  int32_t own = 0, dense = 0;  // the dense operators' products share one word per device
+  if (ctx->scratch)
+    MOE_CUDA(ctx, cudaMemcpyAsync(&own, ctx->scratch, sizeof(int32_t), cudaMemcpyDeviceToHost, ctx->stream));
+  MOE_CUDA(ctx, moe::dense_gemm_status(&dense, ctx->stream));  // synchronises
+  *status = own | (int32_t)((uint32_t)dense << 16);
+  return MOE_OK;
+}
+
+int moe_ctx_expire_wait(moe_ctx* ctx, int64_t limit_us) {
+  if (!ctx) return MOE_ERR_INVALID;
+  ctx->last_error.clear();
+  if (limit_us < 1 || limit_us > 1000000)
+    return fail(ctx, MOE_ERR_INVALID, "moe_ctx_expire_wait: limit_us=%lld (1 to 1000000)", (long long)limit_us);
+  DeviceGuard g(ctx->device);
+  if (!g.ok) return fail(ctx, MOE_ERR_CUDA, "cudaSetDevice(%d) failed", ctx->device);
+  MOE_CUDA(ctx, moe::launch_expire_wait((uint64_t)limit_us * 1000, ctx->stream));
   return MOE_OK;
 }
 

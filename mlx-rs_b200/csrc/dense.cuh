@@ -84,8 +84,12 @@ struct DenseGemm {
   DenseEpi e;
 };
 cudaError_t launch_dense_gemm(const DenseGemm& g, cudaStream_t st);
-// Device status word of these kernels on the current device (bounded waits that expired).
+// Device status word of these kernels on the current device (bounded waits that expired: codes
+// below 2^16); what it reports is cleared. Synchronises the stream.
 cudaError_t dense_gemm_status(int32_t* status, cudaStream_t st);
+// A wait of `limit_ns` that nothing ends: code kExpiredWait.
+constexpr int32_t kExpiredWait = 256;
+cudaError_t launch_expire_wait(uint64_t limit_ns, cudaStream_t st);
 
 // ---- 4-bit products for few tokens (qmv.cu): out = x m[0]^T, or gated out = act(g) * u
 struct QmvArgs {
@@ -176,11 +180,11 @@ MOE_DEV uint64_t now_ns() {
 }
 // Bounded wait; false when it gave up. `gone` is the CTA's abort flag: once one role has
 // given up, the others stop waiting.
-MOE_DEV bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* gone) {
+MOE_DEV bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* gone, uint64_t limit_ns = kWaitLimitNs) {
   if (mbar_try(bar, parity)) return true;
   const uint64_t t0 = now_ns();
   while (!mbar_try(bar, parity))
-    if (*gone || now_ns() - t0 > kWaitLimitNs) return false;
+    if (*gone || now_ns() - t0 > limit_ns) return false;
   return true;
 }
 MOE_DEV void mbar_arrive(uint32_t bar) {

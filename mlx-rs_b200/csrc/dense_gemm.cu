@@ -847,6 +847,15 @@ __global__ void __launch_bounds__(Cfg<PACKED>::kThreads, 1) gemm_kernel(const __
   }
 }
 
+__global__ void clear_status_kernel(int32_t reported) { atomicAnd(&g_dense_status, ~reported); }
+
+__global__ void expire_wait_kernel(uint64_t limit_ns) {
+  __shared__ __align__(8) uint64_t bar;
+  int gone = 0;
+  mbar_init(smem_u32(&bar), 1);
+  if (!mbar_wait(smem_u32(&bar), 0, &gone, limit_ns)) atomicOr(&g_dense_status, kExpiredWait);
+}
+
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
     void* p = nullptr;
@@ -1037,7 +1046,16 @@ cudaError_t launch_dense_gemm(const DenseGemm& g, cudaStream_t st) {
 
 cudaError_t dense_gemm_status(int32_t* status, cudaStream_t st) {
   cudaError_t err = cudaMemcpyFromSymbolAsync(status, g_dense_status, sizeof(int32_t), 0, cudaMemcpyDeviceToHost, st);
+  if (err == cudaSuccess) err = cudaStreamSynchronize(st);
+  if (err != cudaSuccess || *status == 0) return err;
+  clear_status_kernel<<<1, 1, 0, st>>>(*status);
+  err = cudaGetLastError();
   return err != cudaSuccess ? err : cudaStreamSynchronize(st);
+}
+
+cudaError_t launch_expire_wait(uint64_t limit_ns, cudaStream_t st) {
+  expire_wait_kernel<<<1, 1, 0, st>>>(limit_ns);
+  return cudaGetLastError();
 }
 
 }  // namespace moe
