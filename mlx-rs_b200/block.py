@@ -212,7 +212,8 @@ class DenseMlp:
     weights: down(act(gate(x)) * up(x)), activation "silu" or "gelu" (tanh form); gate, up
     [I, H] and down [H, I], bf16 or f16, group_size 32, 64 or 128. ``forward`` is one call of
     moe_gated_ffn_forward. For training through the frozen weights ``forward_saved`` keeps
-    what ``vjp`` needs."""
+    what ``vjp`` needs. gate, up and down may be replaced by weights of the same form; each call
+    reads them as they are."""
 
     def __init__(self, gate: QWeight, up: QWeight, down: QWeight, activation: str = "silu", group_size: int = 64,
                  bits: int = 4):
@@ -233,8 +234,11 @@ class DenseMlp:
         for name, q, rows, cols in (("gate", gate, self.inter, self.hidden), ("up", up, self.inter, self.hidden),
                                     ("down", down, self.hidden, self.inter)):
             ops.check_qweight(fn, name, q, rows, cols, self.dtype, gate.w.get_device(), group_size)
-        self._cfg, self._wts = ops.ffn_structs(self.hidden, self.inter, self.dtype, gate, up, down, activation,
-                                               group_size, bits)
+        self._cfg = ops.ffn_config(self.hidden, self.inter, self.dtype, activation, group_size, bits)
+
+    def _weights(self):
+        # as they are now: gate, up, down and their tensors may be replaced by others of the same form
+        return ops.ffn_tensors(self.gate, self.up, self.down)
 
     def _check(self, fn, x):
         if (x.dtype != self.dtype or x.device != self.device or not x.is_contiguous() or x.dim() < 1
@@ -244,7 +248,7 @@ class DenseMlp:
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         self._check("moe_gated_ffn_forward", x)
-        return ops._ffn_forward(self._cfg, self._wts, x, None, False)
+        return ops._ffn_forward(self._cfg, self._weights(), x, None, False)
 
     __call__ = forward
 
@@ -252,19 +256,19 @@ class DenseMlp:
         """The feed-forward half of a decoder layer, x + block(RmsNorm(x)); the residual is
         added in the down projection's epilogue, before its one rounding. bf16."""
         self._check("moe_gated_ffn_forward", x)
-        return ops._ffn_forward(self._cfg, self._wts, ops.fast_rms_norm(x, norm_weight, eps), x, False)
+        return ops._ffn_forward(self._cfg, self._weights(), ops.fast_rms_norm(x, norm_weight, eps), x, False)
 
     def forward_saved(self, x: torch.Tensor):
         """(forward(x), saved): the same call, which also stores the two projections' outputs."""
         self._check("moe_gated_ffn_forward", x)
-        out, g, u = ops._ffn_forward(self._cfg, self._wts, x, None, True)
+        out, g, u = ops._ffn_forward(self._cfg, self._weights(), x, None, True)
         return out, (g, u)
 
     def vjp(self, saved, dy: torch.Tensor):
         """(dx, dg, du): gradients with respect to x and to the two projections' outputs (for
         adapters beside the frozen weights), given the gradient dy of the output."""
         self._check("moe_gated_ffn_backward", dy)
-        return ops._ffn_backward(self._cfg, self._wts, saved[0], saved[1], dy)
+        return ops._ffn_backward(self._cfg, self._weights(), saved[0], saved[1], dy)
 
 
 class RmsNorm:

@@ -120,19 +120,46 @@ PyObject* quantized_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// ffn_forward(config address, weights address, x, residual, save): the structs are ops.py's,
-// the weights they point to have been checked against them.
+// The block's weights from a tuple (w, scales, biases of gate, of up, of down), on the device and of
+// the type of `like`; false where one does not fit the config. Pointers are taken anew in every
+// call: a tensor of the block may have been replaced since the last.
+bool ffn_weights(PyObject* o, const moe_ffn_config* cfg, const at::Tensor& like, moe_ffn_weights& out) {
+  if (!PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != 9 || cfg->group_size <= 0) return false;
+  moe_qweight* q[3] = {&out.gate, &out.up, &out.down};
+  const int dev = like.get_device();
+  for (int i = 0; i < 3; ++i) {
+    const int64_t rows = i < 2 ? cfg->inter : cfg->hidden, cols = i < 2 ? cfg->hidden : cfg->inter;
+    const void* at[3] = {};
+    for (int j = 0; j < 3; ++j) {
+      PyObject* p = PyTuple_GET_ITEM(o, 3 * i + j);
+      if (j == 2 && p == Py_None) continue;
+      if (!THPVariable_Check(p)) return false;
+      const at::Tensor& t = THPVariable_Unpack(p);
+      if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.dim() != 2 || t.size(0) != rows ||
+          t.size(1) != cols / (j ? cfg->group_size : 8))
+        return false;
+      if (j ? !contiguous_on(&t, like.scalar_type(), dev)
+            : !contiguous_on(&t, at::kInt, dev) && !contiguous_on(&t, at::kUInt32, dev))
+        return false;
+      at[j] = t.data_ptr();
+    }
+    *q[i] = {static_cast<const uint32_t*>(at[0]), at[1], at[2]};
+  }
+  return true;
+}
+
+// ffn_forward(config address, weights, x, residual, save): the config is ops.py's struct.
 PyObject* ffn_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 5) return PyErr_Format(PyExc_TypeError, "5 arguments expected");
   return guarded([&]() -> PyObject* {
     const auto* cfg = static_cast<const moe_ffn_config*>(PyLong_AsVoidPtr(a[0]));
-    const auto* wts = static_cast<const moe_ffn_weights*>(PyLong_AsVoidPtr(a[1]));
+    moe_ffn_weights wts;
     if (PyErr_Occurred()) return nullptr;
     const at::Tensor* x = tensor(a[2]);
     const at::Tensor* r = a[3] == Py_None ? nullptr : tensor(a[3]);
     const bool save = a[4] == Py_True;
-    if (!cfg || !wts || !x || (a[3] != Py_None && !r) || dtype_of(x->scalar_type()) != cfg->dtype || !x->is_contiguous() ||
-        x->dim() < 1 || x->size(-1) != cfg->hidden)
+    if (!cfg || !x || (a[3] != Py_None && !r) || dtype_of(x->scalar_type()) != cfg->dtype || !x->is_contiguous() ||
+        x->dim() < 1 || x->size(-1) != cfg->hidden || !ffn_weights(a[1], cfg, *x, wts))
       Py_RETURN_NONE;
     const int dev = x->get_device();
     if (r && (!contiguous_on(r, x->scalar_type(), dev) || r->sizes() != x->sizes())) Py_RETURN_NONE;
@@ -149,7 +176,7 @@ PyObject* ffn_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (need) ws = scratch(need, *x);
     moe_ctx* ctx = context_for(dev);
     if (!ctx) return raise("moe_ctx_create", MOE_ERR_CUDA, "");
-    const int rc = moe_gated_ffn_forward(ctx, cfg, wts, x->data_ptr(), T, r ? r->data_ptr() : nullptr,
+    const int rc = moe_gated_ffn_forward(ctx, cfg, &wts, x->data_ptr(), T, r ? r->data_ptr() : nullptr,
                                          save ? g.data_ptr() : nullptr, save ? u.data_ptr() : nullptr, out.data_ptr(),
                                          need ? ws.data_ptr() : nullptr, need);
     if (rc) return raise("moe_gated_ffn_forward", rc, moe_last_error(ctx));
@@ -159,16 +186,16 @@ PyObject* ffn_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// ffn_backward(config address, weights address, g, u, dy)
+// ffn_backward(config address, weights, g, u, dy)
 PyObject* ffn_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 5) return PyErr_Format(PyExc_TypeError, "5 arguments expected");
   return guarded([&]() -> PyObject* {
     const auto* cfg = static_cast<const moe_ffn_config*>(PyLong_AsVoidPtr(a[0]));
-    const auto* wts = static_cast<const moe_ffn_weights*>(PyLong_AsVoidPtr(a[1]));
+    moe_ffn_weights wts;
     if (PyErr_Occurred()) return nullptr;
     const at::Tensor *g = tensor(a[2]), *u = tensor(a[3]), *dy = tensor(a[4]);
-    if (!cfg || !wts || !g || !u || !dy || dtype_of(dy->scalar_type()) != cfg->dtype || !dy->is_contiguous() ||
-        dy->dim() < 1 || dy->size(-1) != cfg->hidden)
+    if (!cfg || !g || !u || !dy || dtype_of(dy->scalar_type()) != cfg->dtype || !dy->is_contiguous() ||
+        dy->dim() < 1 || dy->size(-1) != cfg->hidden || !ffn_weights(a[1], cfg, *dy, wts))
       Py_RETURN_NONE;
     const int dev = dy->get_device();
     c10::SmallVector<int64_t, 6> shape(dy->sizes().begin(), dy->sizes().end());
@@ -183,7 +210,7 @@ PyObject* ffn_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (need) ws = scratch(need, *dy);
     moe_ctx* ctx = context_for(dev);
     if (!ctx) return raise("moe_ctx_create", MOE_ERR_CUDA, "");
-    const int rc = moe_gated_ffn_backward(ctx, cfg, wts, g->data_ptr(), u->data_ptr(), dy->data_ptr(), T, dg.data_ptr(),
+    const int rc = moe_gated_ffn_backward(ctx, cfg, &wts, g->data_ptr(), u->data_ptr(), dy->data_ptr(), T, dg.data_ptr(),
                                           du.data_ptr(), dx.data_ptr(), need ? ws.data_ptr() : nullptr, need);
     if (rc) return raise("moe_gated_ffn_backward", rc, moe_last_error(ctx));
     return Py_BuildValue("NNN", THPVariable_Wrap(std::move(dx)), THPVariable_Wrap(std::move(dg)),

@@ -257,7 +257,7 @@ def fast_rms_norm(x, weight, eps):
 
 
 def _ffn_call(fn, x, gate, up, down, activation, group_size, bits):
-    """Config and weight structs of a checked feed-forward call."""
+    """Config and weights of a feed-forward call whose arguments have been checked."""
     if activation not in ACTIVATIONS:
         raise MlxError(fn, 1, f"activation {activation!r} is not one of {sorted(ACTIVATIONS)}")
     if x.dtype not in (torch.bfloat16, torch.float16) or x.dim() < 1 or not x.is_contiguous():
@@ -269,14 +269,26 @@ def _ffn_call(fn, x, gate, up, down, activation, group_size, bits):
         raise MlxError(fn, 1, f"hidden={H} and inter={I} must be positive multiples of group_size={group_size}")
     for name, q, rows, cols in (("gate", gate, I, H), ("up", up, I, H), ("down", down, H, I)):
         check_qweight(fn, name, q, rows, cols, x.dtype, x.get_device(), group_size)
-    return ffn_structs(H, I, x.dtype, gate, up, down, activation, group_size, bits)
+    return ffn_config(H, I, x.dtype, activation, group_size, bits), ffn_tensors(gate, up, down)
 
 
-def ffn_structs(H, I, dtype, gate, up, down, activation, group_size, bits):
-    cfg = FfnConfig(H, I, ACTIVATIONS[activation], group_size, bits, _DTYPES[dtype])
-    ptrs = [QWeight(q.w.data_ptr(), q.scales.data_ptr(), None if q.biases is None else q.biases.data_ptr())
-            for q in (gate, up, down)]
-    return cfg, FfnWeights(*ptrs)
+def ffn_config(H, I, dtype, activation, group_size, bits):
+    return FfnConfig(H, I, ACTIVATIONS[activation], group_size, bits, _DTYPES[dtype])
+
+
+def ffn_tensors(gate, up, down):
+    return (gate.w, gate.scales, gate.biases, up.w, up.scales, up.biases, down.w, down.scales, down.biases)
+
+
+def ffn_weights(fn, cfg, weights, x):
+    """The weight structs of a call on x, checked against its config."""
+    H, I = cfg.hidden, cfg.inter
+    parts = []
+    for i, (name, rows, cols) in enumerate((("gate", I, H), ("up", I, H), ("down", H, I))):
+        w, s, b = weights[3 * i:3 * i + 3]
+        _check_packed(fn, name, w, s, b, rows, cols, x.dtype, x.get_device(), cfg.group_size)
+        parts.append(QWeight(w.data_ptr(), s.data_ptr(), None if b is None else b.data_ptr()))
+    return FfnWeights(*parts)
 
 
 def _like(fn, name, t, shape, x):
@@ -284,12 +296,13 @@ def _like(fn, name, t, shape, x):
         raise MlxError(fn, 1, f"{name}: contiguous {x.dtype} {tuple(shape)} on {x.device} expected")
 
 
-def _ffn_forward(cfg, wts, x, residual, save):
+def _ffn_forward(cfg, weights, x, residual, save):
     fn = "moe_gated_ffn_forward"
     if _calls is not None:
-        r = _calls.ffn_forward(C.addressof(cfg), C.addressof(wts), x, residual, save)
+        r = _calls.ffn_forward(C.addressof(cfg), weights, x, residual, save)
         if r is not None:
             return r
+    wts = ffn_weights(fn, cfg, weights, x)
     T = x.numel() // cfg.hidden
     out = torch.empty_like(x)
     g = u = None
@@ -307,12 +320,13 @@ def _ffn_forward(cfg, wts, x, residual, save):
     return (out, g, u) if save else out
 
 
-def _ffn_backward(cfg, wts, g, u, dy):
+def _ffn_backward(cfg, weights, g, u, dy):
     fn = "moe_gated_ffn_backward"
     if _calls is not None:
-        r = _calls.ffn_backward(C.addressof(cfg), C.addressof(wts), g, u, dy)
+        r = _calls.ffn_backward(C.addressof(cfg), weights, g, u, dy)
         if r is not None:
             return r
+    wts = ffn_weights(fn, cfg, weights, dy)
     T = dy.numel() // cfg.hidden
     _like(fn, "gate", g, (*dy.shape[:-1], cfg.inter), dy)
     _like(fn, "up", u, (*dy.shape[:-1], cfg.inter), dy)
@@ -332,18 +346,18 @@ def gated_ffn(x, gate, up, down, activation="silu", group_size=64, bits=4, resid
     weights (QWeight triples; gate, up [I, H], down [H, I]), activation "silu" or "gelu"
     (tanh form). With save, (out, g, u): the two projections' outputs, what gated_ffn_vjp
     takes. bf16 or f16, group_size 32, 64 or 128."""
-    cfg, wts = _ffn_call("moe_gated_ffn_forward", x, gate, up, down, activation, group_size, bits)
+    cfg, weights = _ffn_call("moe_gated_ffn_forward", x, gate, up, down, activation, group_size, bits)
     if residual is not None:
         _like("moe_gated_ffn_forward", "residual", residual, x.shape, x)
-    return _ffn_forward(cfg, wts, x, residual, save)
+    return _ffn_forward(cfg, weights, x, residual, save)
 
 
 def gated_ffn_vjp(g, u, dy, gate, up, down, activation="silu", group_size=64, bits=4):
     """(dx, dg, du): the gradients of gated_ffn with respect to x and to the projections'
     outputs g, u (as saved by it), for the gradient dy of its output. The quantised weights
     are frozen."""
-    cfg, wts = _ffn_call("moe_gated_ffn_backward", dy, gate, up, down, activation, group_size, bits)
-    return _ffn_backward(cfg, wts, g, u, dy)
+    cfg, weights = _ffn_call("moe_gated_ffn_backward", dy, gate, up, down, activation, group_size, bits)
+    return _ffn_backward(cfg, weights, g, u, dy)
 
 
 def fast_rope(x, dims, traditional=False, base=10000.0, scale=1.0, offset=0, freqs=None, mscale=1.0, inverse=False,

@@ -166,3 +166,18 @@ def test_dense_mlp_refuses_a_scalar():
     mk = lambda r, c: (lambda q: QWeight(q.w, q.scales, q.biases))(R.QW(gen, r, c, 32, torch.bfloat16))  # noqa: E731
     mlp = DenseMlp(mk(96, 64), mk(96, 64), mk(64, 96), group_size=32)
     assert "expected" in _refused(mlp, torch.zeros((), dtype=torch.bfloat16))
+
+
+def test_dense_mlp_checks_the_weights_it_has_now():
+    """Weights put in place of others are looked at by the next call (it refuses what does not fit)."""
+    gen = _gen(10)
+    mk = lambda r, c, d=torch.bfloat16: (lambda q: QWeight(q.w, q.scales, q.biases))(R.QW(gen, r, c, 32, d))  # noqa: E731
+    x = torch.zeros(2, 64, dtype=torch.bfloat16)
+    mlp = DenseMlp(mk(96, 64), mk(96, 64), mk(64, 96), group_size=32)
+    mlp.up = mk(64, 64)
+    assert "up.w" in _refused(mlp, x)
+    mlp.up = mk(96, 64)
+    mlp.down.scales = mlp.down.scales.half()
+    assert "down.scales" in _refused(mlp, x)
+    mlp.down = mk(64, 96)
+    assert "CUDA" in _refused(mlp, x)

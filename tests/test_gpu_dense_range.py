@@ -116,7 +116,8 @@ def test_block_of_infinite_tokens_with_a_residual(T, in_place):
     out = r.clone() if in_place else torch.empty_like(r)
     lib, ctx = mlx_rs_b200.library(), _lib.context_for(0)
     ctx.bind_stream(torch.cuda.current_stream().cuda_stream)
-    cfg, wts = ops.ffn_structs(64, 96, BF16, *w, "silu", 32, 4)
+    cfg = ops.ffn_config(64, 96, BF16, "silu", 32, 4)
+    wts = ops.ffn_weights("ffn", cfg, ops.ffn_tensors(*w), x)
     need = C.c_size_t()
     assert lib.moe_gated_ffn_workspace(C.byref(cfg), T, 0, C.byref(need)) == 0
     ws = torch.empty(need.value, dtype=torch.uint8, device="cuda")
