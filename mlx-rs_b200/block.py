@@ -62,6 +62,10 @@ class _Block:
         self._wts = _CWeights(_cq(w.router), eb, _cq(w.gate), _cq(w.up), _cq(w.down),
                               _cq(w.shared_gate), _cq(w.shared_up), _cq(w.shared_down),
                               _cq(w.shared_expert_gate))
+        # the structs above hold addresses: their tensors live as long as the block, whatever becomes
+        # of `weights` (a block computes with the weights it was made of)
+        qs = (w.router, w.gate, w.up, w.down, w.shared_gate, w.shared_up, w.shared_down, w.shared_expert_gate)
+        self._held = [t for q in qs if q is not None for t in (q.w, q.scales, q.biases)] + [w.expert_bias]
         self.device = w.router.w.device
 
     def reserve(self, max_tokens: int):
