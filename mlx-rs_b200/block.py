@@ -216,7 +216,8 @@ class DenseMlp:
     weights: down(act(gate(x)) * up(x)), activation "silu" or "gelu" (tanh form); gate, up
     [I, H] and down [H, I], bf16 or f16, group_size 32, 64 or 128. ``forward`` is one call of
     moe_gated_ffn_forward. For training through the frozen weights ``forward_saved`` keeps
-    what ``vjp`` needs. gate, up and down may be replaced by weights of the same form; each call
+    what ``vjp`` needs; no call records a graph, and an x that requires a gradient is refused
+    outside torch.no_grad(). gate, up and down may be replaced by weights of the same form; each call
     reads them as they are."""
 
     def __init__(self, gate: QWeight, up: QWeight, down: QWeight, activation: str = "silu", group_size: int = 64,

@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -50,6 +51,12 @@ const at::Tensor* tensor(PyObject* o) {
   const at::Tensor& t = THPVariable_Unpack(o);
   return t.defined() && t.is_cuda() && t.layout() == at::kStrided ? &t : nullptr;
 }
+// The same for an input: not one that torch would look for a gradient of (no graph is recorded here;
+// ops.py refuses it).
+const at::Tensor* input(PyObject* o) {
+  const at::Tensor* t = tensor(o);
+  return t && !(t->requires_grad() && c10::GradMode::is_enabled()) ? t : nullptr;
+}
 bool contiguous_on(const at::Tensor* t, c10::ScalarType type, int device) {
   return t && t->scalar_type() == type && t->get_device() == device && t->is_contiguous();
 }
@@ -81,7 +88,7 @@ PyObject* guarded(F&& f) {
 PyObject* quantized_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 6) return PyErr_Format(PyExc_TypeError, "6 arguments expected");
   return guarded([&]() -> PyObject* {
-    const at::Tensor *x = tensor(a[0]), *w = tensor(a[1]), *s = tensor(a[2]);
+    const at::Tensor *x = input(a[0]), *w = tensor(a[1]), *s = tensor(a[2]);
     const at::Tensor* b = a[3] == Py_None ? nullptr : tensor(a[3]);
     const int transpose = PyObject_IsTrue(a[4]);
     const long g = PyLong_AsLong(a[5]);
@@ -155,8 +162,8 @@ PyObject* ffn_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const auto* cfg = static_cast<const moe_ffn_config*>(PyLong_AsVoidPtr(a[0]));
     moe_ffn_weights wts;
     if (PyErr_Occurred()) return nullptr;
-    const at::Tensor* x = tensor(a[2]);
-    const at::Tensor* r = a[3] == Py_None ? nullptr : tensor(a[3]);
+    const at::Tensor* x = input(a[2]);
+    const at::Tensor* r = a[3] == Py_None ? nullptr : input(a[3]);
     const bool save = a[4] == Py_True;
     if (!cfg || !x || (a[3] != Py_None && !r) || dtype_of(x->scalar_type()) != cfg->dtype || !x->is_contiguous() ||
         x->dim() < 1 || x->size(-1) != cfg->hidden || !ffn_weights(a[1], cfg, *x, wts))
@@ -193,7 +200,7 @@ PyObject* ffn_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const auto* cfg = static_cast<const moe_ffn_config*>(PyLong_AsVoidPtr(a[0]));
     moe_ffn_weights wts;
     if (PyErr_Occurred()) return nullptr;
-    const at::Tensor *g = tensor(a[2]), *u = tensor(a[3]), *dy = tensor(a[4]);
+    const at::Tensor *g = input(a[2]), *u = input(a[3]), *dy = input(a[4]);
     if (!cfg || !g || !u || !dy || dtype_of(dy->scalar_type()) != cfg->dtype || !dy->is_contiguous() ||
         dy->dim() < 1 || dy->size(-1) != cfg->hidden || !ffn_weights(a[1], cfg, *dy, wts))
       Py_RETURN_NONE;
@@ -223,7 +230,7 @@ PyObject* ffn_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* fast_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 9) return PyErr_Format(PyExc_TypeError, "9 arguments expected");
   return guarded([&]() -> PyObject* {
-    const at::Tensor* x = tensor(a[0]);
+    const at::Tensor* x = input(a[0]);
     const at::Tensor* f = a[6] == Py_None ? nullptr : tensor(a[6]);
     if (!x || x->dim() != 4 || (a[6] != Py_None && !f)) Py_RETURN_NONE;
     const int type = dtype_of(x->scalar_type()), dev = x->get_device();

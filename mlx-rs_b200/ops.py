@@ -76,6 +76,13 @@ def _context(fn, t):
     return ctx
 
 
+def _no_graph(fn, *tensors):
+    """Refuses inputs whose gradient torch would look for: the calls record no graph."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise MlxError(fn, 1, "an input requires a gradient, and this call records no graph: make it under "
+                              "torch.no_grad(); its gradient has a call of its own")
+
+
 def _workspace(nbytes, device):
     # from torch's allocator on the current stream: each call and each captured graph has its own
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
@@ -135,6 +142,7 @@ def _quantized_matmul_ex(x, w, scales, biases, transpose, group_size, bits):
         raise MlxError(fn, 1, f"x [..., {K}] does not fit w {tuple(w.shape)} (transpose={bool(transpose)}, "
                               f"group_size={group_size})")
     _check_packed(fn, "w", w, scales, biases, rows, cols, x.dtype, x.get_device(), group_size)
+    _no_graph(fn, x)
     M = x.numel() // K
     tr = 1 if transpose else 0
     out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
@@ -151,7 +159,9 @@ def _quantized_matmul_ex(x, w, scales, biases, transpose, group_size, bits):
 def quantized_matmul(x, w, scales, biases=None, transpose=True, group_size=64, bits=4):
     """out[..., N] = x[..., K] @ dequant(w)^T (transpose=True), or x[..., K] @ dequant(w)
     for w [K, N*bits/32] (transpose=False: the gradient of the first with respect to x).
-    bf16 or f16, group_size 32, 64 or 128, bits 4."""
+    bf16 or f16, group_size 32, 64 or 128, bits 4. Records no graph: an x that requires a gradient
+    is refused outside torch.no_grad(), except at bf16, group_size 64 and transpose, where the
+    result has none, as with the package's other operators."""
     if group_size != 64 or x.dtype != torch.bfloat16 or not transpose:
         if _calls is not None and bits == 4:
             out = _calls.quantized_matmul(x, w, scales, biases, transpose, group_size)
@@ -302,6 +312,7 @@ def _ffn_forward(cfg, weights, x, residual, save):
         r = _calls.ffn_forward(C.addressof(cfg), weights, x, residual, save)
         if r is not None:
             return r
+    _no_graph(fn, x, residual)
     wts = ffn_weights(fn, cfg, weights, x)
     T = x.numel() // cfg.hidden
     out = torch.empty_like(x)
@@ -326,6 +337,7 @@ def _ffn_backward(cfg, weights, g, u, dy):
         r = _calls.ffn_backward(C.addressof(cfg), weights, g, u, dy)
         if r is not None:
             return r
+    _no_graph(fn, g, u, dy)
     wts = ffn_weights(fn, cfg, weights, dy)
     T = dy.numel() // cfg.hidden
     _like(fn, "gate", g, (*dy.shape[:-1], cfg.inter), dy)
@@ -345,7 +357,8 @@ def gated_ffn(x, gate, up, down, activation="silu", group_size=64, bits=4, resid
     """(act(x gate^T) * (x up^T)) down^T (+ residual): the dense feed-forward block on 4-bit
     weights (QWeight triples; gate, up [I, H], down [H, I]), activation "silu" or "gelu"
     (tanh form). With save, (out, g, u): the two projections' outputs, what gated_ffn_vjp
-    takes. bf16 or f16, group_size 32, 64 or 128."""
+    takes. bf16 or f16, group_size 32, 64 or 128. Records no graph: inputs that require a gradient
+    are refused outside torch.no_grad(); gated_ffn_vjp gives it."""
     cfg, weights = _ffn_call("moe_gated_ffn_forward", x, gate, up, down, activation, group_size, bits)
     if residual is not None:
         _like("moe_gated_ffn_forward", "residual", residual, x.shape, x)
@@ -370,7 +383,8 @@ def fast_rope(x, dims, traditional=False, base=10000.0, scale=1.0, offset=0, fre
     int, or an int32 / int64 tensor [B] with one offset per batch element. inverse: the
     transposed rotation, the gradient with respect to x. out: where to write, x itself
     included, else memory apart from x's (default: a new contiguous tensor). An int offset is
-    at most 2**53 in magnitude. bf16, f16 or f32."""
+    at most 2**53 in magnitude. bf16, f16 or f32. Records no graph: an x that requires a gradient
+    is refused outside torch.no_grad()."""
     if out is None and _calls is not None:
         r = _calls.fast_rope(x, dims, traditional, base, scale, offset, freqs, mscale, inverse)
         if r is not None:
@@ -380,6 +394,7 @@ def fast_rope(x, dims, traditional=False, base=10000.0, scale=1.0, offset=0, fre
     nd = x.dim()
     if dt is None or nd < 2:
         raise MlxError(fn, 1, "x must be bf16, f16 or f32 [..., L, D]")
+    _no_graph(fn, x)
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:

@@ -168,6 +168,25 @@ def test_dense_mlp_refuses_a_scalar():
     assert "expected" in _refused(mlp, torch.zeros((), dtype=torch.bfloat16))
 
 
+def test_inputs_that_require_gradients_are_refused():
+    """No call records a graph, so that a backward pass would pass by it in silence."""
+    gen = _gen(11)
+    mk = lambda r, c, d=torch.bfloat16: (lambda q: QWeight(q.w, q.scales, q.biases))(R.QW(gen, r, c, 32, d))  # noqa: E731
+    x = torch.zeros(2, 64, dtype=torch.bfloat16, requires_grad=True)
+    p, mlp = mk(96, 64), DenseMlp(mk(96, 64), mk(96, 64), mk(64, 96), group_size=32)
+    w = (mlp.gate, mlp.up, mlp.down)
+    h, z = torch.zeros(2, 96, dtype=torch.bfloat16), x.detach()
+    calls = [lambda: ops.quantized_matmul(x, p.w, p.scales, p.biases, group_size=32), lambda: mlp(x), lambda: mlp.forward_saved(x),
+             lambda: ops.gated_ffn(x, *w, group_size=32), lambda: ops.gated_ffn(z, *w, group_size=32, residual=x),
+             lambda: mlp.vjp((h, h), x), lambda: ops.gated_ffn_vjp(h.requires_grad_(), h, z, *w, group_size=32),
+             lambda: ops.fast_rope(x[None, None], 64)]
+    for f in calls:
+        assert "requires a gradient" in _refused(f)
+    with torch.no_grad():  # this gets as far as the device
+        for f in calls:
+            assert "CUDA" in _refused(f)
+
+
 def test_dense_mlp_checks_the_weights_it_has_now():
     """Weights put in place of others are looked at by the next call (it refuses what does not fit)."""
     gen = _gen(10)
