@@ -151,16 +151,21 @@ def library():
     if _lib is not None:
         return _lib
     with _lock:
+        built = False
         if _lib is None:
             if not os.path.exists(library_path):
                 from . import build as _build
                 _build.build()
+                built = True
             L = C.CDLL(library_path)
             for name, (res, args) in SIGNATURES.items():
                 f = getattr(L, name)
                 f.restype = res
                 f.argtypes = args
             _lib = L
+    if built:
+        from . import ops
+        ops.load_calls()
     return _lib
 
 

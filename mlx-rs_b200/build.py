@@ -1,5 +1,6 @@
 """Build libmoe_b200.so (the C-ABI library) in-tree with nvcc for sm_100a, and _calls.so (the
-dense operators' calls from Python) with g++ against torch's headers.
+dense operators' calls from Python) with g++ against torch's headers. The second is optional:
+without it those calls go through ctypes, with the same results.
 
 Usage: python mlx-rs_b200/build.py [--force] [--verbose]
 Objects go to mlx-rs_b200/_build/, the libraries to mlx-rs_b200/.
@@ -18,6 +19,7 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libmoe_b200.so")
 CALLS = os.path.join(HERE, "_calls.so")
+CALLS_FOR = os.path.join(BUILD, "calls.for")  # what it was built against
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -65,7 +67,7 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None) -> str:
             print(" ".join(cmd), flush=True)
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
-            raise RuntimeError(f"nvcc failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+            raise RuntimeError(f"build failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
         if verbose and (r.stdout or r.stderr):
             print(r.stdout + r.stderr, flush=True)
 
@@ -75,9 +77,30 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None) -> str:
         cmd = [nvcc()] + ARCH + ["-shared", "-o", LIB] + objs + ["-lcudart"]
         run(cmd)
     src = os.path.join(CSRC, "torch_calls.cpp")
-    if force or _stale(CALLS, [src] + [h for h in hdrs if h.startswith(INCLUDE)]):
-        run(calls_command(src))
+    try:
+        if force or _stale(CALLS, [src] + [h for h in hdrs if h.startswith(INCLUDE)]) or _built_for() != calls_for():
+            run(calls_command(src))
+            with open(CALLS_FOR, "w") as f:
+                f.write(calls_for())
+    except (RuntimeError, OSError, ImportError) as e:  # no compiler, no headers of torch, no torch
+        if os.path.exists(CALLS):
+            os.remove(CALLS)  # it may not fit the library
+        print(f"{os.path.basename(CALLS)} was not built, the calls go through ctypes: {e}", file=sys.stderr)
     return LIB
+
+
+def calls_for() -> str:
+    """What _calls.so is built against."""
+    import torch
+    return f"{torch.__version__} {os.path.dirname(os.path.abspath(torch.__file__))} {sys.version}"
+
+
+def _built_for():
+    try:
+        with open(CALLS_FOR) as f:
+            return f.read()
+    except OSError:
+        return None
 
 
 def calls_command(src: str):

@@ -19,17 +19,39 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import importlib
+import os
+import warnings
 
 import torch
 
 from ._lib import (ACT_GELU, ACT_SILU, DTYPE_BF16, DTYPE_F16, DTYPE_F32, FfnConfig, FfnWeights, MlxError, QWeight,
                    RopeConfig, context_for, library)
 
-try:  # the dense operators' calls without ctypes (build.py); what it declines is made here
-    from . import _calls
-    _calls.set_error(MlxError)
-except ImportError:
+_calls = None
+
+
+def load_calls():
+    """The dense operators' calls without ctypes (build.py), where they were built for this torch;
+    what they decline is made here."""
+    global _calls
     _calls = None
+    if not os.path.exists(os.path.join(os.path.dirname(os.path.abspath(__file__)), "_calls.so")):
+        return None
+    try:
+        importlib.invalidate_caches()
+        module = importlib.import_module(__package__ + "._calls")
+        if not torch.__version__.startswith(module.torch_version):
+            raise ImportError(f"built for torch {module.torch_version}")
+    except ImportError as e:
+        warnings.warn(f"_calls.so is not used, the calls go through ctypes: {e}")
+        return None
+    module.set_error(MlxError)
+    _calls = module
+    return module
+
+
+load_calls()
 
 _WORD_DTYPES = {torch.int32} | ({torch.uint32} if hasattr(torch, "uint32") else set())
 
