@@ -152,8 +152,10 @@ def _quantized_matmul_ex(x, w, scales, biases, transpose, group_size, bits):
     dt = _DTYPES.get(x.dtype)
     if dt is None or dt == DTYPE_F32 or x.dim() < 1 or not x.is_contiguous():
         raise MlxError(fn, 1, "x must be contiguous bf16 or f16 [..., K]")
-    if bits != 4 or group_size not in (32, 64, 128):
-        raise MlxError(fn, 2, f"bits={bits}, group_size={group_size} is not implemented")
+    if bits not in (2, 3, 4, 5, 6, 8) or group_size not in (32, 64, 128):
+        raise MlxError(fn, 1, f"bits={bits}, group_size={group_size} is not a valid MLX affine format")
+    if bits != 4:
+        raise MlxError(fn, 2, f"bits={bits} is not implemented")
     if w.dim() != 2:
         raise MlxError(fn, 1, "w must be [rows, cols*bits/32]")
     K = x.shape[-1]

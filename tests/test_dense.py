@@ -168,6 +168,13 @@ def test_dense_mlp_refuses_a_scalar():
     assert "expected" in _refused(mlp, torch.zeros((), dtype=torch.bfloat16))
 
 
+@pytest.mark.parametrize("bits,group,rc", [(7, 32, 1), (0, 128, 1), (3, 32, 2), (8, 128, 2), (4, 16, 1)])
+def test_quantized_matmul_tells_invalid_from_unsupported(bits, group, rc):
+    """rc 1: no format of MLX; rc 2: one that is not implemented. As the C entries do."""
+    q, x = R.QW(_gen(12), 40, 64, 32, torch.float16), torch.zeros(3, 64, dtype=torch.float16)
+    assert f"rc={rc}" in _refused(ops.quantized_matmul, x, q.w, q.scales, q.biases, group_size=group, bits=bits)
+
+
 def test_inputs_that_require_gradients_are_refused():
     """No call records a graph, so that a backward pass would pass by it in silence."""
     gen = _gen(11)
