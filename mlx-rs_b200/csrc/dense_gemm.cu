@@ -203,14 +203,13 @@ MOE_DEV void tmem_ld16(uint32_t taddr, float (&r)[16]) {
 }
 MOE_DEV void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 
-// ---- W (4 or 8) consecutive elements of a 16-bit row, at column c of n (vec: rows of 16-byte
+// ---- W (4 or 8) consecutive elements of a 16-bit row, at column c of n (vec, four: rows of 16-byte
 // aligned multiples of 8; otherwise element by element, columns beyond n left alone)
 template <int TYPE, int W>
 MOE_DEV void load_n(const uint16_t* row, int c, int n, bool vec, float (&v)[W]) {
-  if (vec) {
+  if (W == 4 && vec) {
     uint32_t q[W / 2];
-    if constexpr (W == 8) *reinterpret_cast<uint4*>(q) = *reinterpret_cast<const uint4*>(row + c);
-    else *reinterpret_cast<uint2*>(q) = *reinterpret_cast<const uint2*>(row + c);
+    *reinterpret_cast<uint2*>(q) = *reinterpret_cast<const uint2*>(row + c);
 #pragma unroll
     for (int i = 0; i < W / 2; ++i) v[2 * i] = Elem<TYPE>::lo(q[i]), v[2 * i + 1] = Elem<TYPE>::hi(q[i]);
   } else {
@@ -223,9 +222,8 @@ MOE_DEV void store_n(uint16_t* row, int c, int n, bool vec, const float (&v)[W])
   uint32_t q[W / 2];
 #pragma unroll
   for (int i = 0; i < W / 2; ++i) q[i] = Elem<TYPE>::pack(v[2 * i], v[2 * i + 1]);
-  if (vec) {
-    if constexpr (W == 8) *reinterpret_cast<uint4*>(row + c) = make_uint4(q[0], q[1], q[2], q[3]);
-    else *reinterpret_cast<uint2*>(row + c) = make_uint2(q[0], q[1]);
+  if (W == 4 && vec) {
+    *reinterpret_cast<uint2*>(row + c) = make_uint2(q[0], q[1]);
   } else {
 #pragma unroll
     for (int i = 0; i < W; ++i)
