@@ -110,17 +110,35 @@ MOE_DEV void row_words(uint32_t span, int row, int gr, int t, uint32_t (&w)[G / 
 // sum_k (s q_k + b) x_k of one row and one token in 64 bits, over the lanes of a warp.
 template <int TYPE, int G>
 __device__ __noinline__ float exact_sum(const PackedMatrix& m, int row, const uint16_t* x, int K, int lane) {
-  double sum = 0.0;
-#pragma unroll 1
+  double lo = 0.0, hi = 0.0;
+#pragma unroll 4
   for (int i = lane; i < K >> 3; i += 32) {
     const uint32_t q = m.w[(size_t)row * (K >> 3) + i];
     const size_t g = (size_t)row * (K / G) + i / (G / 8);
     const double s = Elem<TYPE>::to_f(m.s[g]), b = m.b ? Elem<TYPE>::to_f(m.b[g]) : 0.0f;
-#pragma unroll 1
-    for (int j = 0; j < 8; ++j) sum = fma(fma((double)(q >> 4 * j & 15u), s, b), (double)Elem<TYPE>::to_f(x[8 * i + j]), sum);
+    const uint4 v = *reinterpret_cast<const uint4*>(x + 8 * i);
+    const uint32_t t[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      lo = fma(fma((double)(q >> 8 * j & 15u), s, b), (double)Elem<TYPE>::lo(t[j]), lo);
+      hi = fma(fma((double)(q >> (8 * j + 4) & 15u), s, b), (double)Elem<TYPE>::hi(t[j]), hi);
+    }
   }
+  double sum = lo + hi;
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return (float)sum;
+}
+// Whether a token holds a NaN, over the lanes of a warp: its sums are right as they are.
+template <int TYPE>
+__device__ __noinline__ bool has_nan(const uint16_t* x, int K, int lane) {
+  bool is = false;
+  for (int i = lane; i < K >> 3; i += 32) {
+    const uint4 v = *reinterpret_cast<const uint4*>(x + 8 * i);
+    const uint32_t t[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) is |= isnan(Elem<TYPE>::lo(t[j])) || isnan(Elem<TYPE>::hi(t[j]));
+  }
+  return __any_sync(0xffffffffu, is);
 }
 
 // IN_PLACE: out is the residual
@@ -235,13 +253,20 @@ __global__ void __maxnreg__(NC == 4 ? 128 : 96) qmv_kernel(const __grid_constant
   };
   // A sum that is not finite may have left the range only by its factors of 16 + q (tokens from
   // 2^128 / 31 on, and infinities, which give inf - inf): the lanes whose sum is `bad` get it
-  // again, from the weights themselves. Whole warps.
-  auto again = [&](bool bad, int n, int m, float& v, float& u) {
+  // again, from the weights themselves, unless the token holds a NaN. Whole warps. known, nans:
+  // columns whose token was looked at, that hold one.
+  auto again = [&](bool bad, int n, int m, float& v, float& u, uint32_t& known, uint32_t& nans) {
 #pragma unroll 1
     for (uint32_t todo = __ballot_sync(0xffffffffu, bad); todo; todo &= todo - 1) {
       const int src = __ffs(todo) - 1;
-      const int row = __shfl_sync(0xffffffffu, n, src);
-      const uint16_t* x = a.x + (int64_t)__shfl_sync(0xffffffffu, m, src) * K;
+      const int row = __shfl_sync(0xffffffffu, n, src), token = __shfl_sync(0xffffffffu, m, src);
+      const uint16_t* x = a.x + (int64_t)token * K;
+      const uint32_t bit = 1u << (token - mbase);
+      if (!(known & bit)) {
+        known |= bit;
+        if (has_nan<TYPE>(x, K, lane)) nans |= bit;
+      }
+      if (nans & bit) continue;
       const float ev = exact_sum<TYPE, G>(a.m[0], row, x, K, lane);
       const float eu = GATED ? exact_sum<TYPE, G>(a.m[1], row, x, K, lane) : 0.0f;
       if (lane == src) v = ev, u = eu;
@@ -347,25 +372,29 @@ __global__ void __maxnreg__(NC == 4 ? 128 : 96) qmv_kernel(const __grid_constant
           if (GATED) u += rb[(w * 16 + 8 + row) * kCols + col];
         }
       const bool bad = !isfinite(v) || (GATED && !isfinite(u));
-      if constexpr (IN_PLACE) again(bad, n, m, v, u);
+      if constexpr (IN_PLACE) {
+        uint32_t known = 0, nans = 0;
+        again(bad, n, m, v, u, known, nans);
+      }
       lost |= bad;
       if (in) store(n, m, v, u);
     }
   }
   asm volatile("cp.async.wait_all;\n" ::: "memory");
   // Such an element's output is not finite either. Done here, and not in the tiles' loop, whose
-  // registers are all taken: a call without such elements takes 0 to 2 % longer for it up to 8
-  // tokens and -4 to +4 % from 9 to 32, there it would be 0 to 6 %. In place the output cannot be
-  // formed twice.
+  // registers are all taken: a call without such elements takes 0 to 3 % longer for it up to 8
+  // tokens and -2 to +3 % from 9 to 32, there it would be up to 6 %. In place the output cannot be
+  // formed twice. A token with an infinity, 2048 -> 32768, takes 93 us, one with a NaN 20 (14.7).
   if (!IN_PLACE && __any_sync(0xffffffffu, lost)) {
+    uint32_t known = 0, nans = 0;
 #pragma unroll 1
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x)
 #pragma unroll 1
       for (int i = threadIdx.x; i < kOut * kCols; i += blockDim.x) {
         const int n = tile * kOut + i % kOut, m = mbase + i / kOut;
         const bool bad = n < rows && m < a.M && !isfinite(Elem<TYPE>::to_f(a.out[(int64_t)m * rows + n]));
-        float v, u;
-        again(bad, n, m, v, u);
+        float v = __int_as_float(0x7fffffff), u = v;  // of a token with a NaN
+        again(bad, n, m, v, u, known, nans);
         if (bad) store(n, m, v, u);
       }
   }
