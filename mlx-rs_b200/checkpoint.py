@@ -112,6 +112,8 @@ def write_safetensors(path: str, tensors: Dict[str, np.ndarray], dtypes: Optiona
 def _to_bf16(e: _Entry) -> np.ndarray:
     if e.dtype == "BF16":
         return np.asarray(e.array)
+    if e.dtype not in ("F16", "F32", "F64"):
+        raise CheckpointError(f"scales, biases or expert_bias of type {e.dtype}: not an affine format")
     return f32_to_bf16_bits(np.asarray(e.array, dtype=np.float32))
 
 

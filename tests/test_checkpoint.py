@@ -388,3 +388,24 @@ def test_dense_blocks_take_f32_scales_that_bf16_holds(tmp_path):
     (m,) = C.load_device_mlps(str(tmp_path), device="cpu")
     assert m.dtype == torch.bfloat16
     assert np.array_equal(m.up.scales.view(torch.int16).numpy().view(np.uint16), want[0][1].scales)
+
+
+def test_scales_that_are_no_floats_are_refused(tmp_path):
+    """Formats with exponents as bytes in place of scales are not the affine one."""
+    _write_dense(str(tmp_path), 32, [0])
+    path = os.path.join(str(tmp_path), "model.safetensors")
+    t = {k: np.array(e.array) for k, e in C.read_safetensors(path).items() if not k.endswith(".biases")}
+    t = {k: np.full(a.shape, 120, np.uint8) if k.endswith(".scales") else a for k, a in t.items()}
+    C.write_safetensors(path, t)
+    with pytest.raises(C.CheckpointError, match="U8"):
+        C.load_device_mlps(str(tmp_path), device="cpu")
+
+
+def test_scales_of_a_moe_block_that_are_no_floats_are_refused(tmp_path):
+    cfg = S.MoeConfig(256, 8, 2, 128, 0, S.SCORING_SOFTMAX, True, False)
+    _write_lfm2(str(tmp_path), [S.with_scoring(S.host_block(cfg, 82), S.SCORING_SOFTMAX_BIAS, 1, 0.5)], [1], cfg, 2)
+    tensors, c = C.open_checkpoint(str(tmp_path))
+    e = tensors.t["model.layers.1.feed_forward.switch_mlp.up_proj.scales"]
+    tensors.t["model.layers.1.feed_forward.switch_mlp.up_proj.scales"] = C._Entry("U8", e.shape, np.full(e.shape, 120, np.uint8))
+    with pytest.raises(C.CheckpointError, match="U8"):
+        C.load_block(tensors, "model.layers.1", c)
