@@ -122,3 +122,31 @@ def test_a_thread_captures_what_another_warmed_up():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, want[1])
+
+
+@pytest.mark.gpu
+def test_a_thread_may_end_while_another_captures():
+    """Its context's scratch is freed meanwhile; the capture goes on."""
+    step, xs = _layers()
+    want = [step(x) for x in xs]
+    torch.cuda.synchronize()
+    used, end = threading.Event(), threading.Event()
+
+    def worker():
+        step(xs[0])
+        torch.cuda.synchronize()
+        used.set()
+        end.wait(60)
+    t = threading.Thread(target=worker)
+    t.start()
+    assert used.wait(60)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = step(xs[1])
+        end.set()
+        t.join()
+        gc.collect()
+        z = step(xs[2])
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want[1]) and torch.equal(z, want[2])
