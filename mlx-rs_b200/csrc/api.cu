@@ -25,6 +25,9 @@ struct moe_ctx {
   cudaStream_t stream = nullptr;
   void* scratch = nullptr;
   size_t scratch_bytes = 0;
+  bool captured = false;      // a graph may hold calls that use the scratch
+  void* kept[64] = {};        // outgrown scratches that such graphs may use
+  int num_kept = 0;
   std::string last_error;
   bool last_block_fused = false;  // the last block call ran the one-launch decode kernel
   // side stream for the tcgen05 half of a hybrid expert step (created on first use
@@ -100,10 +103,24 @@ cudaError_t clear_status_block(void* scratch) {
   return e != cudaSuccess ? e : d;
 }
 
-int alloc_scratch(moe_ctx* ctx, size_t bytes) {
+// Every call that uses the scratch comes by here. An outgrown scratch is freed, which waits for the
+// work in flight on it, or kept as long as the context once a call has been captured: the graph's
+// replays go on using it. Scratch may also come, or grow, in a capture.
+int ensure_scratch(moe_ctx* ctx, size_t bytes) {
+  if (!ctx->captured) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(ctx->stream, &st) != cudaSuccess) (void)cudaGetLastError();
+    ctx->captured = st != cudaStreamCaptureStatusNone;
+  }
+  if (bytes <= ctx->scratch_bytes) return MOE_OK;
+  RelaxedCapture relaxed;
   if (ctx->scratch) {
-    // cudaFree waits for work in flight that may still use the old buffer.
-    cudaFree(ctx->scratch);
+    if (!ctx->captured)
+      cudaFree(ctx->scratch);
+    else if (ctx->num_kept < 64)
+      ctx->kept[ctx->num_kept++] = ctx->scratch;
+    else
+      return fail(ctx, MOE_ERR_NO_MEMORY, "the scratch of captured calls has grown too often (moe_ctx_reserve)");
     ctx->scratch = nullptr;
     ctx->scratch_bytes = 0;
   }
@@ -118,17 +135,6 @@ int alloc_scratch(moe_ctx* ctx, size_t bytes) {
   e = clear_status_block(ctx->scratch);
   if (e != cudaSuccess) return fail(ctx, MOE_ERR_CUDA, "scratch status reset failed: %s", cudaGetErrorString(e));
   return MOE_OK;
-}
-
-int ensure_scratch(moe_ctx* ctx, size_t bytes) {
-  if (bytes <= ctx->scratch_bytes) return MOE_OK;
-  // A context's first scratch may come in a capture: a thread that captures what another one
-  // warmed up. Growing it there is refused by the runtime, since captured calls use the old one.
-  if (!ctx->scratch) {
-    RelaxedCapture relaxed;
-    return alloc_scratch(ctx, bytes);
-  }
-  return alloc_scratch(ctx, bytes);
 }
 
 int check_quant(moe_ctx* ctx, const char* fn, int64_t K, int group_size, int bits) {
@@ -950,10 +956,11 @@ int moe_ctx_create(int device, void* stream, moe_ctx** out) {
 
 void moe_ctx_destroy(moe_ctx* ctx) {
   if (!ctx) return;
-  if (ctx->scratch || ctx->side) {
+  if (ctx->scratch || ctx->num_kept || ctx->side) {
     DeviceGuard g(ctx->device);
     RelaxedCapture relaxed;
     if (ctx->scratch) cudaFree(ctx->scratch);
+    for (int i = 0; i < ctx->num_kept; ++i) cudaFree(ctx->kept[i]);
     if (ctx->side) cudaStreamDestroy(ctx->side);
     if (ctx->fork_ev) cudaEventDestroy(ctx->fork_ev);
     if (ctx->join_ev) cudaEventDestroy(ctx->join_ev);
@@ -1513,8 +1520,14 @@ int moe_ctx_status(moe_ctx* ctx, int32_t* status) {
   DeviceGuard g(ctx->device);
   if (!g.ok) return fail(ctx, MOE_ERR_CUDA, "cudaSetDevice(%d) failed", ctx->device);
   int32_t own = 0, dense = 0;  // the dense operators' products share one word per device
-  if (ctx->scratch)
-    MOE_CUDA(ctx, cudaMemcpyAsync(&own, ctx->scratch, sizeof(int32_t), cudaMemcpyDeviceToHost, ctx->stream));
+  for (int i = -1; i < ctx->num_kept; ++i) {  // captured calls still write the scratch they were made with
+    int32_t word = 0;
+    const void* scratch = i < 0 ? ctx->scratch : ctx->kept[i];
+    if (!scratch) continue;
+    MOE_CUDA(ctx, cudaMemcpyAsync(&word, scratch, sizeof(int32_t), cudaMemcpyDeviceToHost, ctx->stream));
+    MOE_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+    own |= word;
+  }
   MOE_CUDA(ctx, moe::dense_gemm_status(&dense, ctx->stream));  // synchronises
   *status = own | (int32_t)((uint32_t)dense << 16);
   return MOE_OK;

@@ -150,3 +150,34 @@ def test_a_thread_may_end_while_another_captures():
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, want[1]) and torch.equal(z, want[2])
+
+
+@pytest.mark.gpu
+def test_a_graph_outlives_the_growth_of_its_scratch():
+    """After the capture a larger eager call makes the context's scratch grow, and a larger capture
+    again; each graph goes on with the scratch it was captured with."""
+    import mlx_rs_b200.synth as S
+    from gpu_util import make_block
+
+    def thread():  # a context of its own, whose scratch starts small
+        blk = make_block(S.host_block(S.MoeConfig(256, 8, 2, 128, 0, S.SCORING_SOFTMAX, True, False), 3))
+        gen = torch.Generator().manual_seed(29)
+        xs = [torch.randn(T, 256, generator=gen).to(torch.bfloat16).cuda() for T in (20, 6000, 12000, 24000)]
+        graphs = []
+        for x in (xs[0], xs[2]):
+            blk.forward(xs[0])
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                y = blk.forward(x)
+            graphs.append((g, x, y))
+            blk.forward(xs[1])
+        blk.forward(xs[3])
+        junk = [torch.full((1 << 22,), 0x7f, dtype=torch.uint8, device="cuda") for _ in range(8)]  # noqa: F841
+        for g, x, y in graphs * 2:
+            y.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, blk.forward(x))
+        return True
+    assert _run(thread) == [True]
