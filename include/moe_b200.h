@@ -16,7 +16,8 @@
  *   - calls are asynchronous and ordered on the context's stream (MLX's lazy graph
  *     + default stream, array.rs:28-40); the caller synchronises;
  *   - scratch memory is owned by the context and grows on demand (moe_ctx_reserve
- *     sizes it up front); a context must not be used by two threads at once.
+ *     sizes it up front), and what captured calls use stays allocated as long as the
+ *     context; a context must not be used by two threads at once.
  *
  * Quantized weights use the MLX affine layout (mlx_quantize, mode "affine"):
  *   w      [rows, K * bits / 32] uint32, element e of a row is bits (e % (32/bits))*bits
@@ -137,6 +138,8 @@ enum moe_dtype { MOE_DTYPE_BF16 = 0, MOE_DTYPE_F16 = 1, MOE_DTYPE_F32 = 2 };
  * is 0) must be a multiple of group_size; all pointers 16-byte aligned; out overlaps no
  * input. The workspace (moe_quantized_matmul_workspace bytes, 32-byte aligned, contents
  * irrelevant) belongs to the call until it has run: calls that may overlap need one each.
+ * Each weight may be rounded once to dtype, depending on M and the matrix's size; sums are fp32,
+ * and a token's infinities, or values near the end of the range, give what the definition gives.
  * Array::quantized_matmul, crates/mlx-core/src/ops.rs:592-637.
  */
 int moe_quantized_matmul_workspace(int dtype, int64_t M, int64_t K, int64_t N, int transpose, int group_size,
