@@ -138,8 +138,8 @@ enum moe_dtype { MOE_DTYPE_BF16 = 0, MOE_DTYPE_F16 = 1, MOE_DTYPE_F32 = 2 };
  * is 0) must be a multiple of group_size; all pointers 16-byte aligned; out overlaps no
  * input. The workspace (moe_quantized_matmul_workspace bytes, 32-byte aligned, contents
  * irrelevant) belongs to the call until it has run: calls that may overlap need one each.
- * Each weight may be rounded once to dtype, depending on M and the matrix's size; sums are fp32,
- * and a token's infinities, or values near the end of the range, give what the definition gives.
+ * Each weight may be rounded once to dtype, depending on M and the matrix's size; sums are fp32;
+ * a token's infinities give what the definition gives.
  * Array::quantized_matmul, crates/mlx-core/src/ops.rs:592-637.
  */
 int moe_quantized_matmul_workspace(int dtype, int64_t M, int64_t K, int64_t N, int transpose, int group_size,

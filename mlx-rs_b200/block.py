@@ -69,6 +69,7 @@ class _Block:
         self.device = w.router.w.device
 
     def reserve(self, max_tokens: int):
+        """Sizes the scratch of the calling thread's context for calls of up to max_tokens tokens."""
         ctx = _ctx(self.weights.router.w)
         ctx.check("moe_ctx_reserve", library().moe_ctx_reserve(ctx.handle, C.byref(self._cfg), max_tokens))
 

@@ -109,8 +109,10 @@ cudaError_t clear_status_block(void* scratch) {
 int ensure_scratch(moe_ctx* ctx, size_t bytes) {
   if (!ctx->captured) {
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(ctx->stream, &st) != cudaSuccess) (void)cudaGetLastError();
-    ctx->captured = st != cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(ctx->stream, &st) == cudaSuccess)
+      ctx->captured = st != cudaStreamCaptureStatusNone;
+    else
+      (void)cudaGetLastError();  // the legacy stream beside a captured one is not captured itself
   }
   if (bytes <= ctx->scratch_bytes) return MOE_OK;
   RelaxedCapture relaxed;

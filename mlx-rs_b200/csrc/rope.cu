@@ -9,16 +9,16 @@
 // float: at position 10^6 a 32-bit angle is already off by a few hundredths of a radian.
 // The floor is the bytes (one read and one write of the tensor; at 4096 positions the writes stay
 // in L2, and neither DRAM nor the issue slots, 57 % active, are full; what bounds it has not been
-// shown). A CTA takes `tokens` positions
-// with all of their heads: it fills a table of cosines and sines in shared memory once, one
-// pair per thread, so that the 64-bit work is spread over the threads and shared by the heads,
-// then moves the heads through two vectors per item, the loads of two items in flight.
+// shown). A CTA takes `tokens` positions with all of their heads: it fills a table of cosines and
+// sines in shared memory once, one pair per thread, so that the 64-bit work is spread over the
+// threads and shared by the heads, then moves the heads through two vectors per item, the loads of
+// two items in flight.
 // 36 heads of 128 bf16 channels out of a fused projection: 4096 positions 15.8 us (4.8 TB/s),
 // 8192 30.9 us (4.9 TB/s); one position of 64 sequences 2.5 us; 2 x 1023 x 16 heads of 80, f32,
 // interleaved, 5.3 us. Measured against it, the same four in us: one item in flight 15.4, 28.1,
-// 2.5, 6.3 (faster for 16-bit prompts, slower for f32); three 18.2, 36.1, 2.6, 7.1 (registers); one in flight as two named copies, with CTAs
-// of 128 threads 16.5, 31.0, 2.7, 6.3, of 256 17.5, 34.5, 2.4, 6.1, of 512 22.1, 36.6, 2.2, 7.7;
-// 64-bit index arithmetic 19.2, 33.1, 3.0, 6.6.
+// 2.5, 6.3 (faster for 16-bit prompts, slower for f32); three 18.2, 36.1, 2.6, 7.1 (registers);
+// one in flight as two named copies, with CTAs of 128 threads 16.5, 31.0, 2.7, 6.3, of 256 17.5,
+// 34.5, 2.4, 6.1, of 512 22.1, 36.6, 2.2, 7.7; 64-bit index arithmetic 19.2, 33.1, 3.0, 6.6.
 #include "dense.cuh"
 
 namespace moe {
