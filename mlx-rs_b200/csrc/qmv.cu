@@ -20,9 +20,10 @@
 // The tokens are read to match (x is small and stays in L1), each 16-byte piece permuted to
 // the order in which the fields leave a word.
 // Bound by the instructions of a span (about 280 for 16 x 128 weights: 64 to extract the
-// fields, 16 MMAs) at the 20 warps per SM that 96 registers allow: one token, 2048 -> 32768
-// 16 us (2.2 TB/s), 2048 -> 11264 7.4 us, 5632 -> 2048 5.1 us, 2048 -> 2048 2.9 us. Measured
-// against it: a warp that does the copies of a CTA, bulk copies and scales through shared
+// fields, 16 MMAs) and their latency (issue slots 55 %) at the 20 warps per SM that 96 registers
+// allow: one token, on the device, group 128 2048 -> 32768 14.7 us (2.4 TB/s; 16.0 a call), group
+// 64 2048 -> 11264 6.8 us and 5632 -> 2048 5.1 us, group 32 2048 -> 2048 3.4 us. Measured against
+// earlier forms of it (16 us a call for 2048 -> 32768, 2.9 for 2048 -> 2048): a warp that does the copies of a CTA, bulk copies and scales through shared
 // memory (fewer instructions, but 1.5 us more before the first product: 2048 -> 2048 4.5 us),
 // 32 rows per warp (19.7 us for 2048 -> 32768), the span's tokens loaded ahead (19.2 us: the
 // registers), 24 warps of 80 registers (21 us).
